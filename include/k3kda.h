@@ -360,6 +360,88 @@ size_t k3hip_mla_cache_floats(const K3Cfg *c, int cap);   /* per sequence: cap*(
 int k3hip_mla_decode(const k3hip_mla_weights *w, int B, int pos, int cap, float *cache,
                      const float *x, float *out, void *stream);
 
+/* ---------------------------------------------- trees of drafted tokens ---- *
+ * Speculative decoding scores several drafted tokens of a sequence in one step. The operators
+ * below take them as a tree and replace, for a stack of KDA and MLA layers, the snapshot, one decode
+ * step per token and restore of the reference's loop (src/cli/k3_run.c:1969-1984): the state and the
+ * cache are only committed along the path that was accepted.
+ *   lens    [B] committed positions of each sequence
+ *   counts  [B] drafted tokens (nodes) of each sequence, at most N; NULL: N each
+ *   parents [B][N] the node each node follows, a lower number; anything else: the committed context.
+ *           NULL: a chain
+ *   accept  [B] the last accepted node; anything that is no node of its sequence: none
+ * all int32 device memory, read when the call runs. N is at most 64 (a chain's append: any). Rows of
+ * nodes past counts[b] are not read and their results are left as they were. Values out of range are
+ * taken as said, never as an address: lengths are limited to what the table holds.
+ *
+ * A paged latent cache holds what k3hip_mla_decode's cache holds per position, the rmsnorm'd latent
+ * (kv_lora) and the rope slot (rope), fp32 or bf16:
+ *   pages [n_pages][page][kv_lora + rope]   table [B][max_pages] int32 page numbers
+ * Position t of sequence b is row t % page of page table[b][t / page]; a number that is no page holds
+ * nothing: its positions are not written and not seen. Node n stands at position lens[b] + n until it
+ * is committed, and is rotated as position lens[b] + (number of its ancestors).
+ * All calls are stream-ordered, allocate nothing (k3hip_mla_tree_attention: unless workspace is NULL),
+ * are bit-reproducible and may be captured into a graph. */
+enum { K3HIP_ROPE_PAIRS = 0, K3HIP_ROPE_HALVES = 1 };
+
+/* New rows into the cache: row (b, n) of rows [B][N] (stride rows_ld elements) holds the kv_a output,
+ * kv_lora + rope wide; its latent is RMS-normalised with norm_w (NULL: copied; eps inside the root, as
+ * src/core/k3_ops.c:94-102), its rope slot rotated: pair i by position * inv_freq[i], pairs (2i, 2i+1)
+ * or (i, i + rope/2) by rope_style; inv_freq NULL: copied (NoPE). With q, the rope slots of the
+ * queries, q [B][N][H][rope] (row stride q_ld, head stride q_head), are rotated the same way into q_out
+ * (its own strides; it may be q itself with q's strides and dtype). rope even, at most 256.
+ * Dtypes K3HIP_F32 or K3HIP_BF16 each. */
+int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pages, int dtype, int n_pages, int page,
+                        const int *table, int max_pages, const int *lens, const int *counts, const int *parents,
+                        const void *rows, int rows_dtype, long rows_ld, const float *norm_w, float eps,
+                        const float *inv_freq, int rope_style, int H, const void *q, int q_dtype, long q_ld,
+                        long q_head, void *q_out, int q_out_dtype, long q_out_ld, long q_out_head, void *stream);
+
+/* Attention of the nodes (appended before) over the committed positions, their ancestors and themselves:
+ *   q [B][N][H][kv_lora + rope] in the cache's dtype, each row [W_UK_h^T q_nope, q_rope] (absorbed)
+ *   o [B][N][H][kv_lora] (o_dtype) = softmax(scale q . cache^T) . latent; lse [B][N][H] fp32 or NULL:
+ *   the natural log of the sum of exp(scale q . cache^T). N = 1 is a decode step of sequences of different
+ *   lengths. A row that sees nothing (no pages) gives o = 0, lse = -inf. What a row does not see does not
+ *   reach it, infinities and NaN neither.
+ * bf16 caches: the products on bf16, weights rounded to bf16, sums in fp32. fp32 caches: fp32 throughout.
+ * kv_lora at most 512, kv_lora + rope at most 576, both multiples of 8; q, pages, o 16-byte aligned.
+ * workspace: k3hip_mla_tree_workspace bytes (of any call with these B, N, H, kv_lora), 16-byte aligned,
+ * used by one call at a time; NULL: taken from the library's scratch for the call. */
+size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora);
+int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int rope, float scale, const void *q,
+                             const void *pages, int dtype, int n_pages, int page, const int *table, int max_pages,
+                             const int *lens, const int *counts, const int *parents, void *o, int o_dtype,
+                             float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The accepted path's rows (width elements each) to positions lens[b], lens[b] + 1, ... in order;
+ * lens_out[b] (may be NULL, may be lens) = lens[b] + the path's length. Every layer's cache is moved with
+ * the lens of before. */
+int k3hip_latent_commit(int B, int N, int width, void *pages, int dtype, int n_pages, int page, const int *table,
+                        int max_pages, const int *lens, const int *counts, const int *parents, const int *accept,
+                        int *lens_out, void *stream);
+
+/* One KDA layer's core over the trees: what k3hip_kda_decode_step computes for a token, for every node
+ * from its parent's state and conv history (src/core/k3_ops.c:888-947 at T = 1 along each branch), with
+ * the committed S and conv_state only read. Arguments as there, with a node dimension:
+ *   q_in,k_in,v_in [B][N][P] (in_dtype)   z [B][N][P] fp32   b_logit [B][N][H] fp32
+ *   gate [B][N][P] (gate_dtype)           y [B][N][P] (y_dtype)
+ *   S [H][D][D] and conv_state [3][P][K-1] of sequence b at b * s_stride and b * conv_stride floats (so
+ *   that slots of k3hip_kda_layer_decode serve as they are). S 16-byte aligned, s_stride a multiple of 4. */
+int k3hip_kda_tree_step(int B, int N, int H, int D, int K, float gate_lb, float rms_eps, int in_dtype,
+                        const void *q_in, const void *k_in, const void *v_in, const float *z, const float *b_logit,
+                        const void *gate, int gate_dtype, const float *q_conv, const float *k_conv,
+                        const float *v_conv, const float *A_log, const float *dt_bias, const float *o_norm,
+                        const float *conv_state, long conv_stride, float q_scale, const float *S, long s_stride,
+                        const int *counts, const int *parents, void *y, int y_dtype, void *stream);
+
+/* S and conv_state of each sequence moved to those of its accepted node, from the same inputs as the step;
+ * a sequence that accepted none is left as it was. */
+int k3hip_kda_tree_commit(int B, int N, int H, int D, int K, float gate_lb, int in_dtype, const void *q_in,
+                          const void *k_in, const void *v_in, const float *z, const float *b_logit,
+                          const float *q_conv, const float *k_conv, const float *v_conv, const float *A_log,
+                          const float *dt_bias, float *conv_state, long conv_stride, float *S, long s_stride,
+                          const int *counts, const int *parents, const int *accept, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

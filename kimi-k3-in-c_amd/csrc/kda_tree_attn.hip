@@ -1,0 +1,572 @@
+// SPDX-License-Identifier: Apache-2.0
+// kda_tree_attn.hip - attention of drafted token trees over a paged cache of MLA latents, in one pass
+// over the cache, for gfx950 (k3hip_mla_tree_attention).
+//
+// Query row (n, h) of sequence b, in absorbed form (qcat = [W_UK_h^T q_nope, q_rope], CW wide), sees the
+// lens[b] committed rows c_t of the cache and the rows of node n and its ancestors:
+//   p_t = softmax_t(scale qcat . c_t),   o = sum_t p_t c_t[0 .. KL).
+// Every head of every node reads the same rows, so a sequence is one product of (nodes x heads) rows with
+// its cache: bytes bind for one node, the matrix cores from a few nodes on.
+//
+//  * A workgroup (four waves, one a SIMD) owns a tile of query rows and a range of positions and walks it
+//    in tiles of 64 (bf16) or 32 (fp32) positions, staged as they lie by loads that write LDS directly,
+//    two buffers, one barrier a tile. Rows that have no page, or lie past the last node, are staged as zeros.
+//  * A wave owns 16 NR query rows (RG such groups a workgroup) and the tile's 16-row blocks of its
+//    position group (PG of them): scores^T (positions x query rows), the online softmax in base 2 and
+//    o^T (latent channels x query rows) += latents^T . p. With the query row in the column, a softmax
+//    row is a lane: its max, its sum, its rescale and its mask are per-lane values, and p goes from the score
+//    product's output layout into the second product's operand without leaving the lane. Position groups
+//    are merged through LDS at the end.
+//  * The 16 rows of a block stand in the score product in the order 4 (m % 4) + m / 4, so that the four
+//    positions a lane quarter ends up with are four rows apart: its transposed reads (bf16,
+//    ds_read_b64_tr_b16) and the 16-byte reads of the score product then both fall on distinct banks, with
+//    16-byte unit u of row r at u ^ ((r / 2) % 8) (bf16) or u ^ (r % 16) (fp32).
+//  * fp32 runs on v_mfma_f32_16x16x4_f32.
+//  * The reference max of a row moves only when a score passes it by AT_LAZY, so sums are rescaled rarely.
+//  * Ranges of a sequence leave unnormalised sums with (M, l); a second launch merges them in order.
+//
+// What a row does not see cannot reach it: masked scores are selected away, and where a masked position
+// of a tile holds an infinity or a NaN (its scores show it) the tile's sum is taken position by position
+// instead of by the product, whose zero weights would still spread it.
+#include <math.h>
+
+#include <algorithm>
+
+#include "kda_internal.h"
+#include "kda_tree.h"
+
+namespace k3kda {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef s16x4 __attribute__((address_space(3))) *lds_s16x4_ptr;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void glb_void;
+
+constexpr int TA_NT = 256;
+constexpr int TA_KL = 512, TA_CW = 576;        // widest latent and cache row
+constexpr int TA_TILE = 64 * TA_CW * 2;        // bytes a staged tile: 64 bf16 or 32 fp32 rows
+constexpr int TA_LDS = 2 * TA_TILE + 64;       // two tiles, their rows' validity bits
+constexpr float TA_LOG2E = 1.4426950408889634f, TA_LN2 = 0.6931471805599453f;
+constexpr float TA_LAZY = 8.0f;                // log2 of the largest weight before a rescale
+
+// What rows without a page and channels past CW are staged from.
+__device__ const uint4 ta_zeros[TA_CW * 4 / 16] = {};
+
+struct AttnArgs {
+    TreeSeqs t;
+    PagedRows c;
+    int H, CW, KL;
+    const void *pages, *q;
+    void *o;
+    int o_dt;
+    float *lse;
+    float scale2;     // scale log2(e)
+    int nsplit, nrt;  // position ranges a sequence, row tiles a sequence
+    float *po, *pm, *pl;   // partials [B][nrt][nsplit][rows of a tile] ( x KL)
+};
+
+template <bool F32, int NR, int RG, int PG>
+__global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn_kernel(const AttnArgs a)
+{
+    constexpr int ROWS = 16 * NR * RG;
+    constexpr int ROWB = TA_CW * (F32 ? 4 : 2), UNITS = ROWB / 16;   // a staged row, its 16-byte units
+    constexpr int TP = TA_TILE / ROWB, NB = TP / 16;                 // positions and 16-row blocks a tile
+    constexpr int PB = NB / PG;                                      // blocks a wave
+    constexpr int NP = F32 ? PB : (PB + 1) / 2;                      // K = 16 (fp32) or 32 (bf16) groups of the second product
+    constexpr int DT = TA_KL / 16;                                   // latent tiles
+    constexpr int KS = F32 ? TA_CW / 16 : TA_CW / 32;                // K-steps of a 16-byte unit a lane
+    static_assert(PB * PG == NB, "position groups");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    uint16_t *s_ok = reinterpret_cast<uint16_t *>(smem + 2 * TA_TILE);   // [2][NB] a bit a row
+
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c16 = lane & 15, kq = lane >> 4;
+    const int sp = blockIdx.x, rt = blockIdx.y, b = blockIdx.z;
+    const int rg = wv % RG, pg = wv / RG;
+    const bool works = pg < PG;                       // waves past the groups only stage
+    const int cnt = tree_count(a.t, b), rows = cnt * a.H, r0 = rt * ROWS;
+    if (r0 >= rows) return;
+    const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
+    const int ntile = (end + TP - 1) / TP;
+    const int t0 = (int)((long)ntile * sp / a.nsplit), t1 = (int)((long)ntile * (sp + 1) / a.nsplit);
+    const int H = a.H, CW = a.CW, KL = a.KL;
+    const size_t part = ((size_t)b * a.nrt + rt) * a.nsplit + sp;
+
+    // this lane's query rows: column c16 of each of the wave's NR row tiles
+    int row[NR];
+    uint64_t anc[NR];
+    {
+        const uint64_t m = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            row[r] = r0 + 16 * (NR * rg + r) + c16;
+            const int n = row[r] < rows ? row[r] / H : 0;
+            anc[r] = ((uint64_t)__shfl((uint32_t)(m >> 32), n, 64) << 32) | __shfl((uint32_t)m, n, 64);
+        }
+    }
+    // B fragments of the score product: 16-byte unit 4 ks + kq of the row
+    bf16x8 qb[F32 ? 1 : KS][NR];
+    f32x4 qf[F32 ? KS : 1][NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const char *src = reinterpret_cast<const char *>(a.q) + ((size_t)b * a.t.N * H + (row[r] < rows ? row[r] : 0)) * CW * (F32 ? 4 : 2);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int u = 4 * ks + kq;
+            uint4 v = {0, 0, 0, 0};
+            if (works && row[r] < rows && u < CW / (F32 ? 4 : 8)) v = *reinterpret_cast<const uint4 *>(src + 16 * u);
+            if constexpr (F32) qf[ks][r] = __builtin_bit_cast(f32x4, v);
+            else qb[ks][r] = __builtin_bit_cast(bf16x8, v);
+        }
+    }
+
+    // staging: NB / 4 (at least one) blocks of 16 rows a wave; fp32 tiles have two blocks of twice the units
+    auto load_tile = [&](int t) {
+        const int buf = t & 1;
+        constexpr int RW = TP / 4;   // rows a wave: 16 (bf16) or 8 (fp32)
+        const int pos = t * TP + RW * wv + (lane % RW);
+        const long at = pos < end ? paged_row(a.c, b, pos) : -1;
+        const char *p = at >= 0 ? reinterpret_cast<const char *>(a.pages) + (size_t)at * CW * (F32 ? 4 : 2)
+                                : reinterpret_cast<const char *>(ta_zeros);
+        const uint64_t okb = __ballot(at >= 0);
+        if (lane == 0) {
+            if constexpr (F32) reinterpret_cast<uint8_t *>(s_ok)[8 * buf + wv] = (uint8_t)okb;
+            else s_ok[4 * buf + wv] = (uint16_t)okb;
+        }
+        const uint32_t plo = (uint32_t)(uintptr_t)p, phi = (uint32_t)((uintptr_t)p >> 32);
+        char *dst = smem + buf * TA_TILE + RW * wv * ROWB;
+        const int units = CW / (F32 ? 4 : 8);
+#pragma unroll
+        for (int i = 0; i < RW * UNITS / 64; i++) {
+            const int L = 64 * i + lane, r = L / UNITS, rr = RW * wv + r;
+            const int u = (L % UNITS) ^ (F32 ? rr & 15 : (rr >> 1) & 7);
+            const char *g = reinterpret_cast<const char *>(((uintptr_t)(uint32_t)__shfl(phi, r, 64) << 32) | (uint32_t)__shfl(plo, r, 64));
+            g = u < units ? g + 16 * u : reinterpret_cast<const char *>(ta_zeros);
+            __builtin_amdgcn_global_load_lds((glb_void *)g, (lds_void *)(dst + 1024 * i), 16, 0, 0);
+        }
+    };
+
+    f32x4 acc[DT][NR];
+    float M[NR], lsum[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        M[r] = -INFINITY;
+        lsum[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d][r] = 0.0f;
+    }
+    const int pi = 4 * (c16 & 3) + (c16 >> 2);   // LDS row of score row c16 in its block
+
+    if (t0 < t1) load_tile(t0);
+    for (int t = t0; t < t1; t++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 1 < t1) load_tile(t + 1);
+        if (!works) continue;
+        const char *tile = smem + (t & 1) * TA_TILE + 16 * PB * pg * ROWB;   // this wave's blocks
+
+        f32x4 S[PB][NR];
+#pragma unroll
+        for (int i = 0; i < PB; i++)
+#pragma unroll
+            for (int r = 0; r < NR; r++) S[i][r] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int u = (4 * ks + kq) ^ (F32 ? pi & 15 : (pi >> 1) & 7);
+#pragma unroll
+            for (int i = 0; i < PB; i++) {
+                const char *at = tile + (16 * i + pi) * ROWB + 16 * u;
+                if constexpr (F32) {
+                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(at);
+#pragma unroll
+                    for (int r = 0; r < NR; r++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            S[i][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[ks][r][j], S[i][r], 0, 0, 0);
+                } else {
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(at);
+#pragma unroll
+                    for (int r = 0; r < NR; r++) S[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[ks][r], S[i][r], 0, 0, 0);
+                }
+            }
+        }
+
+        // masks: bit p of a row's word is position t TP + p; this lane's element e of block i is
+        // position 16 i + 4 e + kq of the wave's blocks
+        const int p0 = t * TP;
+        uint64_t ok = F32 ? (uint64_t) reinterpret_cast<const uint32_t *>(s_ok)[2 * (t & 1)]
+                          : reinterpret_cast<const uint64_t *>(s_ok)[t & 1];
+        const uint64_t full = F32 ? 0xffffffffull : ~0ull;
+        const bool masked = ok != full || p0 + TP > len;   // uniform
+        uint64_t see[NR];
+        bool bad = false;
+        if (masked) {
+            const int s = len - p0;   // tile position of the first node
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                uint64_t w = s >= 64 ? ~0ull : s <= 0 ? 0ull : (1ull << s) - 1;
+                if (s >= 0 && s < 64) w |= anc[r] << s;
+                else if (s < 0 && s > -64) w |= anc[r] >> -s;
+                see[r] = (w & ok) >> (16 * PB * pg);
+#pragma unroll
+                for (int i = 0; i < PB; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!(see[r] >> (16 * i + 4 * e + kq) & 1)) {
+                            bad = bad || !(fabsf(S[i][r][e]) < INFINITY);
+                            S[i][r][e] = -INFINITY;
+                        }
+            }
+        }
+
+        // online softmax, a row per lane column; p takes the place of S
+        float al[NR];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            float mt = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < PB; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mt = fmaxf(mt, S[i][r][e]);
+            mt *= a.scale2;
+            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const bool up = mt > M[r] + TA_LAZY;
+            const float mn = up ? mt : M[r];
+            al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
+            moved = moved || up;
+            M[r] = mn;
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            float l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PB; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][r][e], a.scale2, -ref));
+                    S[i][r][e] = p;
+                    l += p;
+                }
+            lsum[r] = lsum[r] * al[r] + l;
+        }
+        if (__ballot(moved)) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < NR; r++) acc[d][r] *= al[r];
+        }
+
+        if (masked && __ballot(bad)) {
+            // position by position on the vector unit, only into the rows that see it
+            for (int x = 0; x < 16 * PB; x++) {
+                float p[NR];
+                bool sees[NR], any = false;
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    p[r] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < PB; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if ((x >> 2) == 4 * i + e) p[r] = S[i][r][e];
+                    p[r] = __shfl(p[r], c16 + 16 * (x & 3), 64);
+                    sees[r] = see[r] >> x & 1;
+                    any = any || sees[r];
+                }
+                if (!__ballot(any)) continue;
+                const char *vrow = tile + x * ROWB;
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    float v[4];
+                    if constexpr (F32) {   // acc[4 D + j][e]: channel 64 D + 16 kq + 4 e + j
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            v[e] = *reinterpret_cast<const float *>(vrow + 16 * ((16 * (d >> 2) + 4 * kq + e) ^ (x & 15)) + 4 * (d & 3));
+                    } else {               // acc[d][e]: channel 16 d + 4 kq + e
+                        const uint2 w = *reinterpret_cast<const uint2 *>(vrow + 16 * ((2 * d + (kq >> 1)) ^ ((x >> 1) & 7)) + 8 * (kq & 1));
+                        v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
+                        v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+                    }
+#pragma unroll
+                    for (int r = 0; r < NR; r++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            acc[d][r][e] = sees[r] ? __builtin_fmaf(p[r], v[e], acc[d][r][e]) : acc[d][r][e];
+                }
+            }
+            continue;
+        }
+#pragma unroll
+        for (int g = 0; g < NP; g++) {
+            if constexpr (F32) {
+                // K = 4 products on rows 16 g + 4 e + kq; a lane's 16 bytes are its column of four tiles:
+                // tile 4 D + j holds channels 64 D + 4 m + j
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int rr = 4 * e + kq;
+#pragma unroll
+                    for (int D = 0; D < DT / 4; D++) {
+                        const f32x4 v = *reinterpret_cast<const f32x4 *>(tile + (16 * g + rr) * ROWB + 16 * ((16 * D + c16) ^ rr));
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int r = 0; r < NR; r++)
+                                acc[4 * D + j][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], S[g][r][e], acc[4 * D + j][r], 0, 0, 0);
+                    }
+                }
+            } else {
+                constexpr bool HALF = PB == 1;   // a single block: the other half of K is zero
+                bf16x8 pf[NR];
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    bf16x2 w[4];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const f32x4 x = j == 0 || !HALF ? S[HALF ? 0 : 2 * g + j][r] : f32x4(0.0f);
+                        w[2 * j] = __builtin_convertvector(f2{x[0], x[1]}, bf16x2);
+                        w[2 * j + 1] = __builtin_convertvector(f2{x[2], x[3]}, bf16x2);
+                    }
+                    pf[r] = bf16x8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
+                }
+                const int rr = 4 * ((lane >> 2) & 3) + kq;   // row of the block this lane's address names
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const int u = (2 * d + ((lane >> 1) & 1)) ^ ((rr >> 1) & 7);
+                    const char *at = tile + (32 * g + rr) * ROWB + 16 * u + 8 * (lane & 1);
+                    const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+                    s16x4 x1 = {0, 0, 0, 0};
+                    if constexpr (!HALF) x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 16 * ROWB));
+                    const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
+                    const bf16x8 vf = __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
+#pragma unroll
+                    for (int r = 0; r < NR; r++) acc[d][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r], acc[d][r], 0, 0, 0);
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        lsum[r] += __shfl_xor(lsum[r], 16, 64);
+        lsum[r] += __shfl_xor(lsum[r], 32, 64);
+    }
+    if constexpr (PG > 1) {
+        // position groups 1 .. PG - 1 hand their sums to group 0, 16 bytes a lane and tile
+        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);
+        float *xm = reinterpret_cast<float *>(smem + (PG - 1) * RG * NR * DT * 64 * 16);
+        static_assert((PG - 1) * RG * NR * (DT * 64 * 16 + 512) <= 2 * TA_TILE, "exchange fits the tiles");
+        __syncthreads();
+        if (works && pg > 0) {
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const int at = (((pg - 1) * RG + rg) * NR + r) * 64 + lane;
+                xm[2 * at] = M[r];
+                xm[2 * at + 1] = lsum[r];
+#pragma unroll
+                for (int d = 0; d < DT; d++) xo[(size_t)(((pg - 1) * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] = acc[d][r];
+            }
+        }
+        __syncthreads();
+        if (!works || pg > 0) return;
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+#pragma unroll
+            for (int g = 0; g < PG - 1; g++) {
+                const int at = ((g * RG + rg) * NR + r) * 64 + lane;
+                const float m2 = xm[2 * at], l2 = xm[2 * at + 1], mm = fmaxf(M[r], m2);
+                const float w1 = M[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[r] - mm);
+                const float w2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mm);
+                lsum[r] = lsum[r] * w1 + l2 * w2;
+                M[r] = mm;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+                    acc[d][r] = acc[d][r] * w1 + xo[(size_t)((g * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] * w2;
+            }
+    }
+    if (!works) return;
+
+    // results: o, or this range's sums
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        if (row[r] >= rows) continue;
+        const bool split = a.nsplit > 1;
+        const size_t orow = (size_t)b * a.t.N * H + row[r];
+        const size_t prow = part * ROWS + (row[r] - r0);
+        if (split) {
+            if (kq == 0) {
+                a.pm[prow] = M[r];
+                a.pl[prow] = lsum[r];
+            }
+            if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
+        } else if (kq == 0 && a.lse) {
+            a.lse[orow] = lsum[r] == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(lsum[r])) * TA_LN2;
+        }
+        const float inv = split ? 1.0f : lsum[r] == 0.0f ? 0.0f : 1.0f / lsum[r];
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            f32x4 v;
+            int ch;
+            if constexpr (F32) {   // element d % 4 of group d / 4: channels ch .. ch + 3 from the four tiles
+                ch = 64 * (d >> 2) + 16 * kq + 4 * (d & 3);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] = acc[4 * (d >> 2) + j][r][d & 3] * inv;
+            } else {
+                ch = 16 * d + 4 * kq;
+                v = acc[d][r] * inv;
+            }
+            if (ch >= KL) continue;
+            if (split) *reinterpret_cast<f32x4 *>(a.po + prow * KL + ch) = v;
+            else if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * KL + ch) = v;
+            else
+                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * KL + ch) =
+                    uint2{(uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16)};
+        }
+    }
+}
+
+// The ranges of a row merged in order, a wave per row: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s.
+// A range that saw nothing (M_s = -inf) left no sums.
+__global__ __launch_bounds__(TA_NT) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows)
+{
+    const int b = blockIdx.y, lane = threadIdx.x & 63, row = blockIdx.x * (TA_NT / 64) + (threadIdx.x >> 6);
+    if (row >= tree_count(a.t, b) * a.H) return;
+    const int rt = row / tile_rows;
+    const size_t p0 = ((size_t)b * a.nrt + rt) * a.nsplit * tile_rows + row % tile_rows;
+    float M = -INFINITY, l = 0.0f;
+    for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, a.pm[p0 + (size_t)s * tile_rows]);
+    for (int c0 = 0; c0 < a.KL; c0 += 256) {
+        const int c = c0 + 4 * lane;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        l = 0.0f;
+        for (int s = 0; s < a.nsplit; s++) {
+            const float m = a.pm[p0 + (size_t)s * tile_rows];
+            if (m == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(m - M);
+            l += w * a.pl[p0 + (size_t)s * tile_rows];
+            if (c < a.KL) v += w * *reinterpret_cast<const f32x4 *>(a.po + (p0 + (size_t)s * tile_rows) * a.KL + c);
+        }
+        if (c < a.KL) {
+            const size_t at = ((size_t)b * a.t.N * a.H + row) * a.KL + c;
+            v *= l == 0.0f ? 0.0f : 1.0f / l;
+            if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + at) = v;
+            else
+                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + at) =
+                    uint2{(uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16)};
+        }
+    }
+    if (a.lse && lane == 0)
+        a.lse[(size_t)b * a.t.N * a.H + row] = l == 0.0f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * TA_LN2;
+}
+
+// Query rows a workgroup takes: the fewest tiles of a sequence that its rows fill.
+int ta_rows(bool f32, long rows)
+{
+    if (f32) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+}
+
+int ta_split(int B, int nrt, int tiles)
+{
+    int ncu = 256;
+    (void)cu_count(ncu);
+    const long wg = (long)B * nrt;
+    return (int)std::max(1L, std::min({(long)tiles, ncu / wg, 64L}));
+}
+
+size_t ta_ws_bytes(int B, int rows, int nrt, int nsplit, int KL)
+{
+    if (nsplit <= 1) return 0;
+    const size_t r = (size_t)B * nrt * nsplit * rows;
+    return ((r * KL * 4 + 255) & ~(size_t)255) + 2 * ((r * 4 + 255) & ~(size_t)255);
+}
+
+}  // namespace
+
+}  // namespace k3kda
+
+using namespace k3kda;
+
+extern "C" size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora)
+{
+    if (B <= 0 || N <= 0 || N > TREE_MAX || H <= 0 || kv_lora <= 0 || kv_lora > TA_KL) return 0;
+    size_t most = 0;
+    for (int f32 = 0; f32 < 2; f32++) {
+        const int rows = ta_rows(f32, (long)N * H), nrt = (int)(((long)N * H + rows - 1) / rows);
+        most = std::max(most, ta_ws_bytes(B, rows, nrt, ta_split(B, nrt, 1 << 20), kv_lora));
+    }
+    return std::max<size_t>(most, 256);
+}
+
+extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int rope, float scale, const void *q,
+                                        const void *pages, int dtype, int n_pages, int page, const int *table,
+                                        int max_pages, const int *lens, const int *counts, const int *parents, void *o,
+                                        int o_dtype, float *lse, void *workspace, size_t workspace_bytes, void *stream)
+{
+    clear_error();
+    static const char *who = "k3hip_mla_tree_attention";
+    if (int rc = paged_check(who, B, N, n_pages, page, max_pages, pages, table, lens)) return rc;
+    if (H <= 0) K3_FAIL(K3HIP_EINVAL, "%s: H=%d", who, H);
+    if (N > TREE_MAX) K3_FAIL(K3HIP_EUNSUPPORTED, "%s: a tree of %d nodes (at most %d)", who, N, TREE_MAX);
+    if (dtype != K3HIP_F32 && dtype != K3HIP_BF16) K3_FAIL(K3HIP_EINVAL, "%s: cache dtype=%d", who, dtype);
+    if (o_dtype != K3HIP_F32 && o_dtype != K3HIP_BF16) K3_FAIL(K3HIP_EINVAL, "%s: o_dtype=%d", who, o_dtype);
+    const int CW = kv_lora + rope;
+    if (kv_lora <= 0 || rope < 0 || kv_lora > TA_KL || CW > TA_CW || kv_lora % 8 || rope % 8)
+        K3_FAIL(K3HIP_EUNSUPPORTED, "%s: kv_lora=%d rope=%d (multiples of 8, at most %d and %d together)", who, kv_lora,
+                rope, TA_KL, TA_CW);
+    if (!(scale > 0.0f)) K3_FAIL(K3HIP_EINVAL, "%s: scale=%g (positive)", who, scale);
+    if (B > 65535 || (long)N * H > 65535L * 16) K3_FAIL(K3HIP_EINVAL, "%s: B=%d N=%d H=%d", who, B, N, H);
+    if (B == 0 || N == 0) return K3HIP_OK;
+    if (!q || !o) K3_FAIL(K3HIP_EINVAL, "%s: NULL q or o", who);
+    if (((uintptr_t)q | (uintptr_t)pages | (uintptr_t)o) & 15)
+        K3_FAIL(K3HIP_EINVAL, "%s: q, pages and o need 16-byte alignment", who);
+    hipStream_t st = as_stream(stream);
+    const bool f32 = dtype == K3HIP_F32;
+    AttnArgs a{};
+    a.t = TreeSeqs{N, lens, counts, parents};
+    a.c = PagedRows{table, n_pages, page, max_pages};
+    a.H = H; a.CW = CW; a.KL = kv_lora;
+    a.pages = pages; a.q = q; a.o = o; a.o_dt = o_dtype; a.lse = lse;
+    a.scale2 = scale * TA_LOG2E;
+    const int rows = ta_rows(f32, (long)N * H);
+    a.nrt = (int)(((long)N * H + rows - 1) / rows);
+    const long tiles = ((long)max_pages * page + N + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
+    a.nsplit = ta_split(B, a.nrt, (int)tiles);
+    const size_t need = ta_ws_bytes(B, rows, a.nrt, a.nsplit, kv_lora);
+    StreamBuf buf;
+    if (need) {
+        if (!workspace) {
+            if (int rc = stream_alloc(buf, need, st)) return rc;
+            workspace = buf.p;
+        } else if (workspace_bytes < need || ((uintptr_t)workspace & 15)) {
+            K3_FAIL(K3HIP_EINVAL, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
+        }
+        const size_t r = (size_t)B * a.nrt * a.nsplit * rows;
+        a.po = (float *)workspace;
+        a.pm = (float *)((char *)workspace + ((r * kv_lora * 4 + 255) & ~(size_t)255));
+        a.pl = (float *)((char *)a.pm + ((r * 4 + 255) & ~(size_t)255));
+    }
+    const void *kern;
+    if (f32)
+        kern = rows == 16 ? (const void *)tree_attn_kernel<true, 1, 1, 2> : rows == 32 ? (const void *)tree_attn_kernel<true, 1, 2, 2>
+                                                                                      : (const void *)tree_attn_kernel<true, 1, 4, 1>;
+    else
+        kern = rows == 16   ? (const void *)tree_attn_kernel<false, 1, 1, 4>
+               : rows == 32 ? (const void *)tree_attn_kernel<false, 1, 2, 2>
+               : rows == 64 ? (const void *)tree_attn_kernel<false, 2, 2, 2>
+                            : (const void *)tree_attn_kernel<false, 2, 4, 1>;
+    K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, TA_LDS));
+    void *args[] = {&a};
+    K3_HIP(hipLaunchKernel(kern, dim3(a.nsplit, a.nrt, B), dim3(TA_NT), args, TA_LDS, st));
+    K3_LAUNCHED();
+    if (a.nsplit > 1) {
+        const int per = TA_NT / 64;
+        hipLaunchKernelGGL(tree_attn_merge_kernel, dim3((unsigned)(((long)N * H + per - 1) / per), (unsigned)B), dim3(TA_NT),
+                           0, st, a, rows);
+        K3_LAUNCHED();
+    }
+    return K3HIP_OK;
+}

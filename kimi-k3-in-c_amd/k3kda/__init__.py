@@ -34,6 +34,8 @@ EXPORTS = (
     "k3hip_kda_layer_decode", "k3hip_kda_upload_ex", "k3hip_kda_weights_bytes",
     "k3hip_kda_dropin_bytes", "k3hip_proj_gemm", "k3hip_kda_layer_decode_noalloc",
     "k3hip_set_projection_gemm", "k3hip_kda_decode_step",
+    "k3hip_latent_append", "k3hip_latent_commit", "k3hip_mla_tree_workspace", "k3hip_mla_tree_attention",
+    "k3hip_kda_tree_step", "k3hip_kda_tree_commit",
 )
 
 
@@ -98,7 +100,7 @@ def lib() -> C.CDLL:
     if not LIB_PATH.exists():
         raise RuntimeError(f"{LIB_PATH} is not built; run __graft_entry__.build()")
     L = C.CDLL(str(LIB_PATH))
-    i, f, sz = C.c_int, C.c_float, C.c_size_t
+    i, f, sz, lg = C.c_int, C.c_float, C.c_size_t, C.c_long
     sig = {
         "k3_kda_scratch": (sz, [C.POINTER(K3Cfg), i]),
         "k3_kda_layer": (None, [_P, _P, C.POINTER(K3KdaW), C.POINTER(K3Cfg), i, _P, _P]),
@@ -139,6 +141,15 @@ def lib() -> C.CDLL:
         "k3hip_set_projection_gemm": (i, [i]),
         "k3hip_kda_decode_step": (i, [i, i, i, i, f, f, i, _P, _P, _P, _P, _P, _P, i, _P, _P, _P, _P, _P, _P,
                                       _P, f, _P, _P, i, _P]),
+        "k3hip_latent_append": (i, [i, i, i, i, _P, i, i, i, _P, i, _P, _P, _P, _P, i, lg, _P, f, _P, i, i, _P, i,
+                                    lg, lg, _P, i, lg, lg, _P]),
+        "k3hip_latent_commit": (i, [i, i, i, _P, i, i, i, _P, i, _P, _P, _P, _P, _P, _P]),
+        "k3hip_mla_tree_workspace": (sz, [i, i, i, i]),
+        "k3hip_mla_tree_attention": (i, [i, i, i, i, i, f, _P, _P, i, i, i, _P, i, _P, _P, _P, _P, i, _P, _P, sz, _P]),
+        "k3hip_kda_tree_step": (i, [i, i, i, i, i, f, f, i, _P, _P, _P, _P, _P, _P, i, _P, _P, _P, _P, _P, _P, _P, lg,
+                                    f, _P, lg, _P, _P, _P, i, _P]),
+        "k3hip_kda_tree_commit": (i, [i, i, i, i, i, f, i, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, lg, _P, lg, _P,
+                                      _P, _P, _P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -299,6 +310,143 @@ def kda_epilogue(o, gate, o_norm, y, H: int, D: int, rms_eps: float, stream=None
     T = o.shape[0]
     _check(lib().k3hip_kda_epilogue(T, H, D, rms_eps, _ptr(o), _ptr(gate), _dt(gate),
                                     _ptr(o_norm), _ptr(y), _dt(y), _stream(stream)))
+
+
+# ------------------------------------------------- trees of drafted tokens ----
+# pages [n_pages, page, kv_lora + rope] (fp32 or bf16), table [B, max_pages], lens / counts / accept [B] and
+# parents [B, N] int32, all on the device; counts None: N nodes each, parents None: a chain.
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+
+
+def _i32(t, *shape):
+    if t is None:
+        return None
+    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape:
+        raise ValueError(f"k3kda: int32 tensor of shape {shape} required, got {t.dtype} {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _shape(t, *shape):
+    if t is not None and tuple(t.shape) != shape:
+        raise ValueError(f"k3kda: shape {shape} required, got {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _f32(t, *shape):
+    if t is not None and str(t.dtype) != "torch.float32":
+        raise ValueError(f"k3kda: float32 required, got {t.dtype}")
+    return _shape(t, *shape)
+
+
+def _rows(t, inner: int):
+    """(address, stride of the dimension before the last `inner`) of a tensor whose leading dimensions are
+    dense and whose last one has unit stride."""
+    if not t.is_cuda:
+        raise ValueError("k3kda: device tensor required")
+    st, sh = t.stride(), t.shape
+    dims = [d for d in range(t.dim() - inner) if sh[d] > 1]
+    ok = sh[-1] <= 1 or st[-1] == 1
+    for d, e in zip(dims, dims[1:]):
+        ok = ok and st[d] == st[e] * sh[e]
+    if t.numel() and not ok:
+        raise ValueError(f"k3kda: strides {st} of shape {tuple(sh)}: rows of one stride and unit columns required")
+    return t.data_ptr(), st[dims[-1]] if dims else sh[-1]   # of one row: any
+
+
+def latent_append(rows, pages, table, lens, kv_lora: int, norm_w=None, eps: float = 1e-5, inv_freq=None,
+                  rope_style: int = ROPE_PAIRS, q=None, q_out=None, counts=None, parents=None, stream=None) -> None:
+    """rows [B, N, kv_lora + rope] normalised, rotated and written to the cache at lens[b] + n; q [B, N, H, rope]
+    rotated into q_out (either may be a slice of wider rows)."""
+    B, N, W = rows.shape
+    n_pages, page, width = pages.shape
+    if width != W:
+        raise ValueError(f"k3kda: rows of {W} for a cache of {width}")
+    R = W - kv_lora
+    at, ld = _rows(rows, 1)
+    H = qp = qd = ql = qh = op = od = ol = oh = 0
+    if q is not None:
+        H = q.shape[2]
+        if tuple(q.shape) != (B, N, H, R) or q_out is None or q_out.shape != q.shape:
+            raise ValueError(f"k3kda: q and q_out of shape {(B, N, H, R)} required")
+        (qp, ql), (op, ol) = _rows(q, 2), _rows(q_out, 2)
+        qd, od, qh, oh = _dt(q), _dt(q_out), q.stride(2), q_out.stride(2)
+    _check(lib().k3hip_latent_append(B, N, kv_lora, R, _ptr(pages), _dt(pages), n_pages, page,
+                                     _i32(table, B, table.shape[1]), table.shape[1], _i32(lens, B), _i32(counts, B),
+                                     _i32(parents, B, N), at, _dt(rows), ld, _f32(norm_w, kv_lora), eps,
+                                     _f32(inv_freq, R // 2), rope_style, H, qp, qd, ql, qh, op, od, ol, oh,
+                                     _stream(stream)))
+
+
+def mla_tree_workspace(B: int, N: int, H: int, kv_lora: int) -> int:
+    return int(lib().k3hip_mla_tree_workspace(B, N, H, kv_lora))
+
+
+def mla_tree_attention(q, pages, table, lens, o, kv_lora: int, scale: float, counts=None, parents=None, lse=None,
+                       workspace=None, stream=None) -> None:
+    """q [B, N, H, kv_lora + rope] (absorbed, the cache's dtype) over the cache and each node's ancestors;
+    o [B, N, H, kv_lora], lse [B, N, H] fp32."""
+    B, N, H, W = q.shape
+    n_pages, page, width = pages.shape
+    if width != W or q.dtype != pages.dtype:
+        raise ValueError(f"k3kda: q rows of {W} {q.dtype} for a cache of {width} {pages.dtype}")
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().k3hip_mla_tree_attention(B, N, H, kv_lora, W - kv_lora, scale, _ptr(q), _ptr(pages), _dt(pages), n_pages,
+                                          page, _i32(table, B, table.shape[1]), table.shape[1], _i32(lens, B),
+                                          _i32(counts, B), _i32(parents, B, N), _shape(o, B, N, H, kv_lora), _dt(o),
+                                          _f32(lse, B, N, H), _ptr(workspace), ws_bytes, _stream(stream)))
+
+
+def latent_commit(pages, table, lens, accept, N: int, lens_out=None, counts=None, parents=None, stream=None) -> None:
+    """The accepted path's rows moved to lens[b], lens[b] + 1, ...; lens_out = lens + the path's length."""
+    n_pages, page, width = pages.shape
+    B = lens.shape[0]
+    _check(lib().k3hip_latent_commit(B, N, width, _ptr(pages), _dt(pages), n_pages, page,
+                                     _i32(table, B, table.shape[1]), table.shape[1], _i32(lens, B), _i32(counts, B),
+                                     _i32(parents, B, N), _i32(accept, B), _i32(lens_out, B), _stream(stream)))
+
+
+def _slots(t, *shape):
+    """(address, stride between sequences) of per-sequence state that is dense within a sequence."""
+    if t is None:
+        return None, 0
+    if not t.is_cuda or str(t.dtype) != "torch.float32" or tuple(t.shape) != shape:
+        raise ValueError(f"k3kda: float32 device tensor of shape {shape} required, got {t.dtype} {tuple(t.shape)}")
+    if t.shape[0] and not t[0].is_contiguous():
+        raise ValueError("k3kda: state must be contiguous within a sequence")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else 0
+
+
+def _tree_inputs(q_in, k_in, v_in, z, b_logit, convs, A_log, dt_bias, H: int, D: int, K: int):
+    B, N, P = q_in.shape
+    if P != H * D or k_in.dtype != q_in.dtype or v_in.dtype != q_in.dtype:
+        raise ValueError(f"k3kda: q_in, k_in, v_in [B, N, {H * D}] of one dtype required")
+    return (_dt(q_in), _ptr(q_in), _shape(k_in, B, N, P), _shape(v_in, B, N, P), _f32(z, B, N, P), _f32(b_logit, B, N, H),
+            *(_f32(w, P, K) for w in convs), _f32(A_log, H), _f32(dt_bias, P))
+
+
+def kda_tree_step(q_in, k_in, v_in, z, b_logit, gate, q_conv, k_conv, v_conv, A_log, dt_bias, o_norm, conv_state, S, y,
+                  H: int, D: int, K: int, gate_lb: float, rms_eps: float, q_scale: float, counts=None, parents=None,
+                  stream=None) -> None:
+    """kda_decode_step for every node of a tree: inputs and y [B, N, P]; S [B, H, D, D] and conv_state
+    [B, 3, P, K-1] (dense within a sequence) are only read."""
+    B, N, P = q_in.shape
+    dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp = _tree_inputs(q_in, k_in, v_in, z, b_logit, (q_conv, k_conv, v_conv), A_log,
+                                                              dt_bias, H, D, K)
+    (Sp, ss), (hp, hs) = _slots(S, B, H, D, D), _slots(conv_state, B, 3, P, K - 1)
+    _check(lib().k3hip_kda_tree_step(B, N, H, D, K, gate_lb, rms_eps, dt, qp, kp, vp, zp, bp, _shape(gate, B, N, P),
+                                     _dt(gate), cq, ck, cv, Ap, dp, _f32(o_norm, D), hp, hs, q_scale, Sp, ss,
+                                     _i32(counts, B), _i32(parents, B, N), _shape(y, B, N, P), _dt(y), _stream(stream)))
+
+
+def kda_tree_commit(q_in, k_in, v_in, z, b_logit, q_conv, k_conv, v_conv, A_log, dt_bias, conv_state, S, accept, H: int,
+                    D: int, K: int, gate_lb: float, counts=None, parents=None, stream=None) -> None:
+    """S and conv_state moved to those of each sequence's accepted node (-1: left), from the step's inputs."""
+    B, N, P = q_in.shape
+    dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp = _tree_inputs(q_in, k_in, v_in, z, b_logit, (q_conv, k_conv, v_conv), A_log,
+                                                              dt_bias, H, D, K)
+    (Sp, ss), (hp, hs) = _slots(S, B, H, D, D), _slots(conv_state, B, 3, P, K - 1)
+    _check(lib().k3hip_kda_tree_commit(B, N, H, D, K, gate_lb, dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp, hp, hs, Sp, ss,
+                                       _i32(counts, B), _i32(parents, B, N), _i32(accept, B), _stream(stream)))
 
 
 class DeviceWeights:
