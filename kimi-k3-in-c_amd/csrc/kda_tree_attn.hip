@@ -46,6 +46,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef s16x4 __attribute__((address_space(3))) *lds_s16x4_ptr;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) const char lds_cchar;
 
 constexpr int TA_NT = 256;
 constexpr int TA_KL = 512, TA_CW = 576;        // widest latent and cache row
@@ -428,6 +430,450 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     }
 }
 
+// The 16x16x32 MFMAs of the bf16 kernel. With 32 query rows a wave the second product's 256 accumulators fill
+// the accumulation registers: with the builtin the compiler moves them between the register files and
+// spills hundreds, so ASM issues the instruction itself, acc tied to its registers, everything else in
+// ordinary ones. The compiler then knows no MFMA, so the wait states between their writes and other
+// instructions' reads (18 at most), and between other instructions' writes and their reads, are statements
+// that take the registers as operands: nothing that uses them moves past.
+template <bool ASM>
+__device__ __forceinline__ void mfma_acc(const bf16x8 &a, const bf16x8 &b, f32x4 &c)
+{
+    if constexpr (ASM) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// In ordinary registers, operands straight from LDS.
+template <bool ASM>
+__device__ __forceinline__ void mfma_vec(const bf16x8 &a, const bf16x8 &b, f32x4 &c, bool first)
+{
+    if constexpr (ASM) {
+        if (first) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+        else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    } else {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, first ? f32x4(0.0f) : c, 0, 0, 0);
+    }
+}
+
+// c += column sums of b; b, c and the ones may have been written just before, b is settled after it.
+template <bool ASM>
+__device__ __forceinline__ void mfma_sum(bf16x8 &b, f32x4 &c)
+{
+    const bf16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    if constexpr (ASM) asm("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %1, %0" : "+v"(c), "+v"(b) : "v"(ones));
+    else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b, c, 0, 0, 0);
+}
+
+template <bool ASM, int D, int NR>
+__device__ __forceinline__ void settle(f32x4 (&c)[D][NR])
+{
+    static_assert(D * NR % 8 == 0, "groups of eight");
+    if constexpr (ASM) {
+        f32x4 *x = &c[0][0];
+#pragma unroll
+        for (int i = 0; i < D * NR; i += 8)
+            asm("s_nop 15\n\ts_nop 3" : "+a"(x[i]), "+a"(x[i + 1]), "+a"(x[i + 2]), "+a"(x[i + 3]), "+a"(x[i + 4]),
+                "+a"(x[i + 5]), "+a"(x[i + 6]), "+a"(x[i + 7]));
+    }
+}
+
+template <bool ASM, int B, int NR>
+__device__ __forceinline__ void settle_vec(f32x4 (&c)[B][NR])
+{
+    static_assert(B * NR == 4 || B * NR <= 2, "accumulators");
+    if constexpr (ASM) {
+        f32x4 *x = &c[0][0];
+        if constexpr (B * NR == 4) asm("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+        else if constexpr (B * NR == 2) asm("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]));
+        else asm("s_nop 15\n\ts_nop 3" : "+v"(x[0]));
+    }
+}
+
+// c *= m, a register at a time through one ordinary register (left to the compiler, all of them are brought
+// over at once and spill). The accumulators are settled before and after.
+template <bool ASM>
+__device__ __forceinline__ void acc_scale(f32x4 &c, float m)
+{
+    if constexpr (ASM) {
+        float t;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float v = c[e];
+            asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+                         : "+a"(v), "=&v"(t) : "v"(m));
+            c[e] = v;
+        }
+    } else {
+        c *= m;
+    }
+}
+
+// Eight lanes a row that agree: a bit a row.
+__device__ __forceinline__ uint32_t gather_rows(uint64_t ballot)
+{
+    return (uint32_t)(((ballot & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
+}
+
+// Either of two bf16 is an infinity or a NaN.
+__device__ __forceinline__ bool not_finite16(uint32_t w)
+{
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// bf16 caches. A tile of 64 positions stands in LDS as nine column groups [64 rows][8 units of 16 bytes], so
+// that one load of 64 lanes fills 8 rows of a group and a lane's row, unit and swizzle are the same in all
+// of them: two row addresses a lane and tile, the groups by immediate offset.
+template <bool FULL, int NR, int RG, int PG>
+__global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn16_kernel(const AttnArgs a)
+{
+    constexpr int ROWS = 16 * NR * RG, TP = 64, NB = 4, PB = NB / PG;
+    constexpr bool HALF = PB == 1;              // a wave's share of a tile is one block: half of K is zero
+    constexpr int NH = HALF ? 1 : PB / 2;       // steps of 32 positions
+    constexpr int SB = HALF ? 1 : 2;            // blocks a step
+    constexpr int DT = TA_KL / 16, KS = TA_CW / 32;
+    constexpr int GRP = TP * 128;               // bytes a column group
+    constexpr bool ASM = NR == 2;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    uint16_t *s_ok = reinterpret_cast<uint16_t *>(smem + 2 * TA_TILE);
+
+    const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kq = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int sp = blockIdx.x, rt = blockIdx.y, b = blockIdx.z;
+    const int rg = wv % RG, pg = wv / RG;
+    const int cnt = tree_count(a.t, b), rows = cnt * a.H, r0 = rt * ROWS;
+    if (r0 >= rows) return;
+    const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
+    const int ntile = (end + TP - 1) / TP;
+    const int t0 = (int)((long)ntile * sp / a.nsplit), t1 = (int)((long)ntile * (sp + 1) / a.nsplit);
+    const int H = a.H, CW = FULL ? TA_CW : a.CW, KL = a.KL;
+    const size_t part = ((size_t)b * a.nrt + rt) * a.nsplit + sp;
+
+    int row[NR];
+    uint64_t anc[NR];
+    {
+        const uint64_t m = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            row[r] = r0 + 16 * (NR * rg + r) + c16;
+            const int n = row[r] < rows ? row[r] / H : 0;
+            anc[r] = ((uint64_t)__shfl((uint32_t)(m >> 32), n, 64) << 32) | __shfl((uint32_t)m, n, 64);
+        }
+    }
+    bf16x8 qb[KS][NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const char *src = reinterpret_cast<const char *>(a.q) + ((size_t)b * a.t.N * H + (row[r] < rows ? row[r] : 0)) * CW * 2;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int u = 4 * ks + kq;
+            uint4 v = {0, 0, 0, 0};
+            if (row[r] < rows && (FULL || u < CW / 8)) v = *reinterpret_cast<const uint4 *>(src + 16 * u);
+            qb[ks][r] = __builtin_bit_cast(bf16x8, v);
+        }
+    }
+
+    // staging: wave wv brings rows 16 wv .. + 15 of the tile
+    const int lrow = lane >> 3;                                  // of eight rows a load
+    const int lu0 = (lane & 7) ^ (lrow >> 1), lu1 = (lane & 7) ^ (4 + (lrow >> 1));   // unit in a group, rows 0-7 and 8-15
+    int pgn[2], pgo[2];   // page and row in it of this lane's rows of the tile to be loaded next, -1: none
+    auto find_rows = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int pos = t * TP + 16 * wv + 8 * i + lrow, at = pos / a.c.page;
+            pgo[i] = pos - at * a.c.page;
+            pgn[i] = -1;
+            if (pos < end && at < a.c.max_pages) pgn[i] = a.c.table[(size_t)b * a.c.max_pages + at];
+        }
+    };
+    auto load_tile = [&](lds_char *dst, int buf) __attribute__((always_inline)) {
+        const char *p[2];
+        uint32_t okb = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const bool ok = pgn[i] >= 0 && pgn[i] < a.c.n_pages;
+            p[i] = ok ? reinterpret_cast<const char *>(a.pages) + ((size_t)pgn[i] * a.c.page + pgo[i]) * (CW * 2)
+                      : reinterpret_cast<const char *>(ta_zeros);
+            p[i] += 16 * (i ? lu1 : lu0);
+            okb |= gather_rows(__ballot(ok)) << (8 * i);
+        }
+        if (lane == 0) s_ok[4 * buf + wv] = (uint16_t)okb;
+#pragma unroll
+        for (int g = 0; g < 9; g++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const char *src = p[i] + 128 * g;
+                if (!FULL && 8 * g + (i ? lu1 : lu0) >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
+                __builtin_amdgcn_global_load_lds((glb_void *)src, (lds_void *)(dst + 2048 * wv + GRP * g + 1024 * i), 16, 0, 0);
+            }
+    };
+
+    f32x4 acc[DT][NR], lacc[1][NR];
+    float M[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        M[r] = -INFINITY;
+        lacc[0][r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d][r] = 0.0f;
+    }
+    // LDS addresses in a block of 16 rows. Score product: row pi, units 4 (ks & 1) + kq of group ks / 2.
+    // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4
+    const int pi = 4 * (c16 & 3) + (c16 >> 2);
+    const int vr = 4 * ((lane >> 2) & 3) + kq;
+    int ka[2], va[4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) ka[i] = 128 * pi + 16 * ((4 * i + kq) ^ ((pi >> 1) & 7)) + 2048 * PB * pg;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        va[i] = 128 * vr + 16 * ((2 * i + ((lane >> 1) & 1)) ^ ((vr >> 1) & 7)) + 8 * (lane & 1) + 2048 * PB * pg;
+
+    // one step: 32 positions (16: HALF) from row 32 hs of the wave's blocks
+    auto scores = [&](lds_cchar *tile, int hs, f32x4 (&S)[SB][NR]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int i = 0; i < SB; i++) {
+                const bf16x8 kf = *(const __attribute__((address_space(3))) bf16x8 *)(tile + ka[ks & 1] + GRP * (ks >> 1) + 4096 * hs + 2048 * i);
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_vec<ASM>(kf, qb[ks][r], S[i][r], ks == 0);
+            }
+        settle_vec<ASM>(S);
+    };
+    // S to weights, as the second product's operand
+    auto softmax = [&](const f32x4 (&S)[SB][NR], bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
+        float al[NR];
+        bool moved = false;
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            float mt = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < SB; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mt = fmaxf(mt, S[i][r][e]);
+            mt *= a.scale2;
+            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const bool up = mt > M[r] + TA_LAZY;
+            const float mn = up ? mt : M[r];
+            al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
+            moved = moved || up;
+            M[r] = mn;
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            bf16x2 w[4];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (i < SB)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i < SB ? i : 0][r][e], a.scale2, -ref));
+                    }
+                w[2 * i] = __builtin_convertvector(f2{p[0], p[1]}, bf16x2);
+                w[2 * i + 1] = __builtin_convertvector(f2{p[2], p[3]}, bf16x2);
+            }
+            pf[r] = bf16x8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
+        }
+        if (__ballot(moved)) {
+            settle_vec<ASM>(lacc);
+#pragma unroll
+            for (int r = 0; r < NR; r++) lacc[0][r] *= al[r];
+            settle<ASM>(acc);
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc_scale<ASM>(acc[d][r], al[r]);
+            settle<ASM>(acc);
+        }
+        // the sum of the weights as they are used (bf16), by the matrix unit
+#pragma unroll
+        for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[0][r]);
+    };
+    auto values = [&](lds_cchar *tile, int hs, const bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            lds_cchar *at = tile + va[d & 3] + GRP * (d >> 2) + 4096 * hs;
+            const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+            s16x4 x1 = {0, 0, 0, 0};
+            if constexpr (!HALF) x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
+            const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
+#pragma unroll
+            for (int r = 0; r < NR; r++) mfma_acc<ASM>(vf, pf[r], acc[d][r]);
+        }
+    };
+    settle<ASM>(acc);
+
+    // whole tiles of committed positions, then the tiles that hold nodes (one or two)
+    const int tm = min(t1, max(t0, len / TP));
+    lds_char *lds = (lds_char *)smem;
+    auto stage_next = [&](lds_char *nxt, int t) __attribute__((always_inline)) {
+        if (t + 1 < t1) {
+            load_tile(nxt, (t + 1) & 1);
+            find_rows(t + 2);
+        }
+    };
+    // The two buffers as parameters that do not alias: else the compiler has every transposed read wait for the
+    // loads in flight.
+    auto whole_tile = [&](lds_cchar *__restrict__ cur, lds_char *__restrict__ nxt, int t) __attribute__((always_inline)) {
+        stage_next(nxt, t);
+        const uint64_t ok = reinterpret_cast<const uint64_t *>(s_ok)[t & 1];
+#pragma unroll
+        for (int hs = 0; hs < NH; hs++) {
+            f32x4 S[SB][NR];
+            bf16x8 pf[NR];
+            scores(cur, hs, S);
+            if (ok != ~0ull) {   // uniform: pages that are none
+#pragma unroll
+                for (int i = 0; i < SB; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!(ok >> (16 * (PB * pg + 2 * hs + i) + 4 * e + kq) & 1))
+#pragma unroll
+                            for (int r = 0; r < NR; r++) S[i][r][e] = -INFINITY;
+            }
+            softmax(S, pf);
+            values(cur, hs, pf);
+        }
+    };
+    if (t0 < t1) {
+        find_rows(t0);
+        load_tile(lds + (t0 & 1) * TA_TILE, t0 & 1);
+        find_rows(t0 + 1);
+    }
+    for (int t = t0; t < tm; t++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        whole_tile(lds + (t & 1) * TA_TILE, lds + (~t & 1) * TA_TILE, t);
+    }
+    for (int t = tm; t < t1; t++) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        stage_next(lds + (~t & 1) * TA_TILE, t);
+        char *tile = smem + (t & 1) * TA_TILE;
+        const uint64_t ok = reinterpret_cast<const uint64_t *>(s_ok)[t & 1];
+        const int s = len - t * TP;   // tile position of the first node
+        uint64_t bad = 0;
+        if (cnt > 1) {
+            // rows of nodes that hold an infinity or a NaN: zeros, and noted, so that the rows that see them
+            // become NaN and no others
+            uint32_t bits = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                char *at = tile + 2048 * wv + 1024 * i + 16 * lane;
+                bool inf = false;
+#pragma unroll
+                for (int g = 0; g < 9; g++) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(at + GRP * g);
+                    inf = inf || not_finite16(w.x) || not_finite16(w.y) || not_finite16(w.z) || not_finite16(w.w);
+                }
+                const uint64_t m = __ballot(inf && 16 * wv + 8 * i + lrow >= s);
+                const bool mine = (m >> (lane & 56) & 0xff) != 0;
+                if (mine)
+#pragma unroll
+                    for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + GRP * g) = uint4{0, 0, 0, 0};
+                bits |= gather_rows(__ballot(mine)) << (8 * i);
+            }
+            if (lane == 0) s_ok[8 + wv] = (uint16_t)bits;
+            __syncthreads();
+            bad = reinterpret_cast<const uint64_t *>(s_ok)[2] >> (16 * PB * pg);
+        }
+        uint64_t see[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            uint64_t w = s >= 64 ? ~0ull : s <= 0 ? 0ull : (1ull << s) - 1;
+            if (s >= 0 && s < 64) w |= anc[r] << s;
+            else if (s < 0 && s > -64) w |= anc[r] >> -s;
+            see[r] = (w & ok) >> (16 * PB * pg);
+        }
+#pragma unroll 1
+        for (int hs = 0; hs < NH; hs++) {
+            f32x4 S[SB][NR];
+            bf16x8 pf[NR];
+            scores(lds + (t & 1) * TA_TILE, hs, S);
+#pragma unroll
+            for (int i = 0; i < SB; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int at = 32 * hs + 16 * i + 4 * e + kq;
+                    const float seen = bad >> at & 1 ? NAN : 0.0f;
+#pragma unroll
+                    for (int r = 0; r < NR; r++) S[i][r][e] = see[r] >> at & 1 ? S[i][r][e] + seen : -INFINITY;
+                }
+            softmax(S, pf);
+            values(lds + (t & 1) * TA_TILE, hs, pf);
+        }
+        if (cnt > 1) __syncthreads();   // the noted rows were read
+    }
+
+    settle<ASM>(acc);
+    settle_vec<ASM>(lacc);
+    float lsum[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) lsum[r] = lacc[0][r][0];
+    if constexpr (PG > 1) {
+        // position groups 1 .. PG - 1 hand their sums to group 0, 16 bytes a lane and tile
+        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);
+        float *xm = reinterpret_cast<float *>(smem + (PG - 1) * RG * NR * DT * 64 * 16);
+        static_assert((PG - 1) * RG * NR * (DT * 64 * 16 + 512) <= 2 * TA_TILE, "exchange fits the tiles");
+        __syncthreads();
+        if (pg > 0) {
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const int at = (((pg - 1) * RG + rg) * NR + r) * 64 + lane;
+                xm[2 * at] = M[r];
+                xm[2 * at + 1] = lsum[r];
+#pragma unroll
+                for (int d = 0; d < DT; d++) xo[(size_t)(((pg - 1) * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] = acc[d][r];
+            }
+        }
+        __syncthreads();
+        if (pg > 0) return;
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+#pragma unroll 1
+            for (int g = 0; g < PG - 1; g++) {
+                const int at = ((g * RG + rg) * NR + r) * 64 + lane;
+                const float m2 = xm[2 * at], l2 = xm[2 * at + 1], mm = fmaxf(M[r], m2);
+                const float w1 = M[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[r] - mm);
+                const float w2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mm);
+                lsum[r] = lsum[r] * w1 + l2 * w2;
+                M[r] = mm;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+                    acc[d][r] = acc[d][r] * w1 + xo[(size_t)((g * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] * w2;
+            }
+    }
+
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        if (row[r] >= rows) continue;
+        const bool split = a.nsplit > 1;
+        const size_t orow = (size_t)b * a.t.N * H + row[r];
+        const size_t prow = part * ROWS + (row[r] - r0);
+        if (split) {
+            if (kq == 0) {
+                a.pm[prow] = M[r];
+                a.pl[prow] = lsum[r];
+            }
+            if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
+        } else if (kq == 0 && a.lse) {
+            a.lse[orow] = lsum[r] == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(lsum[r])) * TA_LN2;
+        }
+        const float inv = split ? 1.0f : lsum[r] == 0.0f ? 0.0f : 1.0f / lsum[r];
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int ch = 16 * d + 4 * kq;
+            const f32x4 v = acc[d][r] * inv;
+            if (ch >= KL) continue;
+            if (split) *reinterpret_cast<f32x4 *>(a.po + prow * KL + ch) = v;
+            else if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * KL + ch) = v;
+            else
+                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * KL + ch) =
+                    uint2{(uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16)};
+        }
+    }
+}
+
 // The ranges of a row merged in order, a wave per row: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s.
 // A range that saw nothing (M_s = -inf) left no sums.
 __global__ __launch_bounds__(TA_NT) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows)
@@ -553,11 +999,12 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     if (f32)
         kern = rows == 16 ? (const void *)tree_attn_kernel<true, 1, 1, 2> : rows == 32 ? (const void *)tree_attn_kernel<true, 1, 2, 2>
                                                                                       : (const void *)tree_attn_kernel<true, 1, 4, 1>;
-    else
-        kern = rows == 16   ? (const void *)tree_attn_kernel<false, 1, 1, 4>
-               : rows == 32 ? (const void *)tree_attn_kernel<false, 1, 2, 2>
-               : rows == 64 ? (const void *)tree_attn_kernel<false, 2, 2, 2>
-                            : (const void *)tree_attn_kernel<false, 2, 4, 1>;
+#define K3_TA(F)                                                                                        \
+    (rows == 16   ? (const void *)tree_attn16_kernel<F, 1, 1, 4>                                               \
+     : rows == 32 ? (const void *)tree_attn16_kernel<F, 1, 2, 2>                                               \
+     : rows == 64 ? (const void *)tree_attn16_kernel<F, 2, 2, 2> : (const void *)tree_attn16_kernel<F, 2, 4, 1>)
+    else kern = CW == TA_CW ? K3_TA(true) : K3_TA(false);
+#undef K3_TA
     K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, TA_LDS));
     void *args[] = {&a};
     K3_HIP(hipLaunchKernel(kern, dim3(a.nsplit, a.nrt, B), dim3(TA_NT), args, TA_LDS, st));
