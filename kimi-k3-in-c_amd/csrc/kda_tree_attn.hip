@@ -68,8 +68,10 @@ struct AttnArgs {
     int o_dt;
     float *lse;
     float scale2;     // scale log2(e)
-    int nsplit, nrt;  // position ranges a sequence, row tiles a sequence
-    float *po, *pm, *pl;   // partials [B][nrt][nsplit][rows of a tile] ( x KL)
+    int nsplit, nrt;  // fp32: position ranges a sequence, row tiles a sequence
+    float *po, *pm, *pl;   // partials of each range [rows of a tile] ( x KL)
+    int B, room;      // bf16: workgroups that the ranges may take
+    int2 *plan;       // [B] first range, ranges a row tile
 };
 
 template <bool F32, int NR, int RG, int PG>
@@ -433,64 +435,49 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // The 16x16x32 MFMAs of the bf16 kernel. With 32 query rows a wave the second product's 256 accumulators fill
 // the accumulation registers: with the builtin the compiler moves them between the register files and
 // spills hundreds, so ASM issues the instruction itself, acc tied to its registers, everything else in
-// ordinary ones. The compiler then knows no MFMA, so the wait states between their writes and other
-// instructions' reads (18 at most), and between other instructions' writes and their reads, are statements
-// that take the registers as operands: nothing that uses them moves past.
+// ordinary ones. The compiler then knows no MFMA; wait() stands where it would have put wait states.
 template <bool ASM>
 __device__ __forceinline__ void mfma_acc(const bf16x8 &a, const bf16x8 &b, f32x4 &c)
 {
-    if constexpr (ASM) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    if constexpr (ASM) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// In ordinary registers, operands straight from LDS.
+// In ordinary registers; both operands come from memory (of a vector instruction's result it would have to wait).
 template <bool ASM>
 __device__ __forceinline__ void mfma_vec(const bf16x8 &a, const bf16x8 &b, f32x4 &c, bool first)
 {
     if constexpr (ASM) {
-        if (first) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
-        else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+        if (first) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+        else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
     } else {
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, first ? f32x4(0.0f) : c, 0, 0, 0);
     }
 }
 
-// c += column sums of b; b, c and the ones may have been written just before, b is settled after it.
+// c += column sums of b; b, c and the ones may have been written just before, b is ready for others after it.
 template <bool ASM>
 __device__ __forceinline__ void mfma_sum(bf16x8 &b, f32x4 &c)
 {
     const bf16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-    if constexpr (ASM) asm("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %1, %0" : "+v"(c), "+v"(b) : "v"(ones));
+    if constexpr (ASM) asm volatile("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %1, %0" : "+v"(c), "+v"(b) : "v"(ones));
     else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b, c, 0, 0, 0);
 }
 
-template <bool ASM, int D, int NR>
-__device__ __forceinline__ void settle(f32x4 (&c)[D][NR])
+// Ten wait states, between MFMAs and other instructions on their results (eight are needed for this one) or
+// between other instructions' results and MFMAs on them; nothing is scheduled across.
+template <bool ASM>
+__device__ __forceinline__ void wait()
 {
-    static_assert(D * NR % 8 == 0, "groups of eight");
     if constexpr (ASM) {
-        f32x4 *x = &c[0][0];
-#pragma unroll
-        for (int i = 0; i < D * NR; i += 8)
-            asm("s_nop 15\n\ts_nop 3" : "+a"(x[i]), "+a"(x[i + 1]), "+a"(x[i + 2]), "+a"(x[i + 3]), "+a"(x[i + 4]),
-                "+a"(x[i + 5]), "+a"(x[i + 6]), "+a"(x[i + 7]));
-    }
-}
-
-template <bool ASM, int B, int NR>
-__device__ __forceinline__ void settle_vec(f32x4 (&c)[B][NR])
-{
-    static_assert(B * NR == 4 || B * NR <= 2, "accumulators");
-    if constexpr (ASM) {
-        f32x4 *x = &c[0][0];
-        if constexpr (B * NR == 4) asm("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
-        else if constexpr (B * NR == 2) asm("s_nop 15\n\ts_nop 3" : "+v"(x[0]), "+v"(x[1]));
-        else asm("s_nop 15\n\ts_nop 3" : "+v"(x[0]));
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 9");
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
 // c *= m, a register at a time through one ordinary register (left to the compiler, all of them are brought
-// over at once and spill). The accumulators are settled before and after.
+// over at once and spill).
 template <bool ASM>
 __device__ __forceinline__ void acc_scale(f32x4 &c, float m)
 {
@@ -520,33 +507,157 @@ __device__ __forceinline__ bool not_finite16(uint32_t w)
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-// bf16 caches. A tile of 64 positions stands in LDS as nine column groups [64 rows][8 units of 16 bytes], so
-// that one load of 64 lanes fills 8 rows of a group and a lane's row, unit and swizzle are the same in all
-// of them: two row addresses a lane and tile, the groups by immediate offset.
-template <bool FULL, int NR, int RG, int PG>
+// Four fp32 to bf16, to nearest even.
+__device__ __forceinline__ uint2 pack4(const f32x4 &v)
+{
+    const bf16x2 x = __builtin_convertvector(f2{v[0], v[1]}, bf16x2), y = __builtin_convertvector(f2{v[2], v[3]}, bf16x2);
+    return uint2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
+}
+
+// Which workgroup takes what. Sequence b's positions are cut, for each of its row tiles, into as many equal
+// ranges as all workgroups of the launch can take with one common quota of steps, the smallest that fits
+// (`room` workgroups), so that sequences of different lengths end together. Ranges are numbered sequence by
+// sequence, range by range, row tile by row tile, and go to the XCDs in runs of neighbours: row tiles that
+// read the same positions share an L2.
+struct Share {
+    int b, rt, split, splits;
+};
+
+// Sequence b's row tiles (of `rows` rows) and steps (of `tp` positions).
+__device__ __forceinline__ void seq_size(const AttnArgs &a, int b, int rows, int tp, int &nrt, int &steps)
+{
+    const int cnt = tree_count(a.t, b);
+    nrt = (cnt * a.H + rows - 1) / rows;
+    steps = cnt ? (paged_len(a.c, a.t.lens, b) + cnt + tp - 1) / tp : 0;
+}
+
+__device__ __forceinline__ int wave_sum(int x)
+{
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
+    return x;
+}
+
+// Every wave works it out for itself, a sequence a lane. With R row tiles in all, T steps over all of them
+// and W workgroups, a quota q needs at least T / q and fewer than T / q + R workgroups, so the smallest
+// one lies in [T / W, T / (W - R)]. False: nothing for this workgroup. Workgroup number 0 writes the plan
+// down for the merge: each sequence's first number and its ranges.
+__device__ __forceinline__ bool find_share(const AttnArgs &a, int rows, int tp, int id, Share &s)
+{
+    const int lane = threadIdx.x & 63;
+    int R = 0, most = 0, nrt0 = 0, steps0 = 0;
+    float T = 0.0f;   // an estimate: the bounds it gives are widened
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        int nrt = 0, steps = 0;
+        if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
+        R += nrt;
+        most = max(most, steps);
+        T += (float)nrt * (float)steps;
+        if (b0 == 0) {
+            nrt0 = nrt;
+            steps0 = steps;
+        }
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        R += __shfl_xor(R, m, 64);
+        T += __shfl_xor(T, m, 64);
+        most = max(most, __shfl_xor(most, m, 64));
+    }
+    if (R == 0) return false;
+    int lo = most, hi = most;   // without room: whole sequences
+    if (R < a.room) {
+        lo = min(most, max(1, (int)(T * 0.999f / (float)a.room)));
+        hi = min(most, (int)(T * 1.001f / (float)(a.room - R)) + 2);
+    }
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        int n = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
+            int nrt = nrt0, steps = steps0;
+            if (b0 > 0) {
+                nrt = steps = 0;
+                if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
+            }
+            n += nrt * ((steps + mid - 1) / mid);
+        }
+        if (wave_sum(n) <= a.room) hi = mid;
+        else lo = mid + 1;
+    }
+    int base = 0;
+    bool found = false;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        int nrt = nrt0, steps = steps0;
+        if (b0 > 0) {
+            nrt = steps = 0;
+            if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
+        }
+        const int sp = (steps + hi - 1) / hi, n = nrt * sp;
+        int end = n;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int x = __shfl_up(end, m, 64);
+            if (lane >= m) end += x;
+        }
+        const int first = base + end - n;
+        if (id == 0 && a.plan && threadIdx.x < 64 && b0 + lane < a.B) a.plan[b0 + lane] = int2{first, sp};
+        const uint64_t in = __ballot(id >= first && id < first + n);
+        if (in && !found) {
+            const int l = __builtin_ctzll(in), at = id - __builtin_amdgcn_readlane(first, l);
+            const int rt = __builtin_amdgcn_readlane(nrt, l);
+            s.b = b0 + l;
+            s.splits = __builtin_amdgcn_readlane(sp, l);
+            s.split = at / rt;
+            s.rt = at - s.split * rt;
+            found = true;
+        }
+        base += __shfl(end, 63, 64);
+    }
+    return found;
+}
+
+// The larger of x and the values of lanes l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float quarter_max(float x)
+{
+    const auto u = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(u[0]), __uint_as_float(u[1]));
+    const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+}
+
+// bf16 caches. A step is 32 positions, staged as nine column groups [32 rows][8 units of 16 bytes] so that one
+// load of 64 lanes fills 8 rows of a group and a lane's row, unit and swizzle are the same in all of
+// them: one row address a lane and step, the groups by immediate offset. Four buffers: while step s is
+// summed and s + 1 scored, s + 2 and s + 3 are on their way.
+//
+// One wave a SIMD has to keep its matrix pipe busy by itself, so the steps overlap: the products of step
+// s + 1's scores are followed by the products of step s's sum with step s + 1's softmax spread between
+// them, two or three vector instructions to a product; the barrier of a step stands before the sum's last
+// eight products, behind which the next scores' first fragments arrive.
+constexpr int TB_TP = 32, TB_GRP = TB_TP * 128, TB_BUF = 9 * TB_GRP, TB_NB = 4;
+constexpr int TB_LDS = TB_NB * TB_BUF + 64;
+static_assert(TB_LDS <= 160 * 1024, "LDS");
+
+template <bool FULL, int NR>
 __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn16_kernel(const AttnArgs a)
 {
-    constexpr int ROWS = 16 * NR * RG, TP = 64, NB = 4, PB = NB / PG;
-    constexpr bool HALF = PB == 1;              // a wave's share of a tile is one block: half of K is zero
-    constexpr int NH = HALF ? 1 : PB / 2;       // steps of 32 positions
-    constexpr int SB = HALF ? 1 : 2;            // blocks a step
-    constexpr int DT = TA_KL / 16, KS = TA_CW / 32;
-    constexpr int GRP = TP * 128;               // bytes a column group
     constexpr bool ASM = NR == 2;
+    constexpr int ROWS = 64 * NR, DT = TA_KL / 16, KS = TA_CW / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    uint16_t *s_ok = reinterpret_cast<uint16_t *>(smem + 2 * TA_TILE);
+    uint8_t *s_ok = reinterpret_cast<uint8_t *>(smem + TB_NB * TB_BUF);   // [buffer][wave] a bit a row; [16 + wave]: not finite
 
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kq = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int sp = blockIdx.x, rt = blockIdx.y, b = blockIdx.z;
-    const int rg = wv % RG, pg = wv / RG;
+    const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);   // the grid is a multiple of 8
+    Share sh;
+    if (!find_share(a, ROWS, TB_TP, id, sh)) return;
+    const int b = __builtin_amdgcn_readfirstlane(sh.b), rt = __builtin_amdgcn_readfirstlane(sh.rt);
+    const int splits = __builtin_amdgcn_readfirstlane(sh.splits), sp = __builtin_amdgcn_readfirstlane(sh.split);
     const int cnt = tree_count(a.t, b), rows = cnt * a.H, r0 = rt * ROWS;
-    if (r0 >= rows) return;
     const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
-    const int ntile = (end + TP - 1) / TP;
-    const int t0 = (int)((long)ntile * sp / a.nsplit), t1 = (int)((long)ntile * (sp + 1) / a.nsplit);
+    const int nstep = (end + TB_TP - 1) / TB_TP;
+    const int s0 = (int)((long)nstep * sp / splits), s1 = (int)((long)nstep * (sp + 1) / splits);
     const int H = a.H, CW = FULL ? TA_CW : a.CW, KL = a.KL;
-    const size_t part = ((size_t)b * a.nrt + rt) * a.nsplit + sp;
 
     int row[NR];
     uint64_t anc[NR];
@@ -554,7 +665,7 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         const uint64_t m = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            row[r] = r0 + 16 * (NR * rg + r) + c16;
+            row[r] = r0 + 16 * (NR * wv + r) + c16;
             const int n = row[r] < rows ? row[r] / H : 0;
             anc[r] = ((uint64_t)__shfl((uint32_t)(m >> 32), n, 64) << 32) | __shfl((uint32_t)m, n, 64);
         }
@@ -572,304 +683,321 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         }
     }
 
-    // staging: wave wv brings rows 16 wv .. + 15 of the tile
-    const int lrow = lane >> 3;                                  // of eight rows a load
-    const int lu0 = (lane & 7) ^ (lrow >> 1), lu1 = (lane & 7) ^ (4 + (lrow >> 1));   // unit in a group, rows 0-7 and 8-15
-    int pgn[2], pgo[2];   // page and row in it of this lane's rows of the tile to be loaded next, -1: none
-    auto find_rows = [&](int t) {
+    // staging: wave wv brings rows 8 wv .. + 7 of a step
+    const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
+    int pgn = -1, pgo = 0;   // page and row in it of this lane's row of the step loaded next
+    auto find_rows = [&](int s) __attribute__((always_inline)) {
+        const int pos = s * TB_TP + prow, at = pos / a.c.page;
+        pgo = pos - at * a.c.page;
+        pgn = -1;
+        if (pos < end && at < a.c.max_pages) pgn = a.c.table[(size_t)b * a.c.max_pages + at];
+    };
+    auto load_step = [&](lds_char *dst, int buf, int page, int in) __attribute__((always_inline)) {
+        const bool ok = page >= 0 && page < a.c.n_pages;
+        const char *p = ok ? reinterpret_cast<const char *>(a.pages) + ((size_t)page * a.c.page + in) * (CW * 2)
+                           : reinterpret_cast<const char *>(ta_zeros);
+        p += 16 * lu;
+        const uint32_t okb = gather_rows(__ballot(ok));
+        if (lane == 0) s_ok[4 * buf + wv] = (uint8_t)okb;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int pos = t * TP + 16 * wv + 8 * i + lrow, at = pos / a.c.page;
-            pgo[i] = pos - at * a.c.page;
-            pgn[i] = -1;
-            if (pos < end && at < a.c.max_pages) pgn[i] = a.c.table[(size_t)b * a.c.max_pages + at];
+        for (int g = 0; g < 9; g++) {
+            const char *src = p + 128 * g;
+            if (!FULL && 8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
+            __builtin_amdgcn_global_load_lds((glb_void *)src, (lds_void *)(dst + TB_GRP * g + 1024 * wv), 16, 0, 0);
         }
     };
-    auto load_tile = [&](lds_char *dst, int buf) __attribute__((always_inline)) {
-        const char *p[2];
-        uint32_t okb = 0;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const bool ok = pgn[i] >= 0 && pgn[i] < a.c.n_pages;
-            p[i] = ok ? reinterpret_cast<const char *>(a.pages) + ((size_t)pgn[i] * a.c.page + pgo[i]) * (CW * 2)
-                      : reinterpret_cast<const char *>(ta_zeros);
-            p[i] += 16 * (i ? lu1 : lu0);
-            okb |= gather_rows(__ballot(ok)) << (8 * i);
-        }
-        if (lane == 0) s_ok[4 * buf + wv] = (uint16_t)okb;
-#pragma unroll
-        for (int g = 0; g < 9; g++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const char *src = p[i] + 128 * g;
-                if (!FULL && 8 * g + (i ? lu1 : lu0) >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
-                __builtin_amdgcn_global_load_lds((glb_void *)src, (lds_void *)(dst + 2048 * wv + GRP * g + 1024 * i), 16, 0, 0);
-            }
-    };
+    auto buf_of = [](int s) { return s & (TB_NB - 1); };
+    lds_char *lds = (lds_char *)smem;
 
-    f32x4 acc[DT][NR], lacc[1][NR];
+    f32x4 acc[DT][NR], lacc[NR];
     float M[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         M[r] = -INFINITY;
-        lacc[0][r] = 0.0f;
+        lacc[r] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) acc[d][r] = 0.0f;
     }
+    wait<ASM>();
     // LDS addresses in a block of 16 rows. Score product: row pi, units 4 (ks & 1) + kq of group ks / 2.
-    // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4
-    const int pi = 4 * (c16 & 3) + (c16 >> 2);
-    const int vr = 4 * ((lane >> 2) & 3) + kq;
+    // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4. Unit u
+    // of row r stands at u ^ ((r / 2) & 6)
+    const int pi = 4 * (c16 & 3) + (c16 >> 2), vr = 4 * ((lane >> 2) & 3) + kq;
     int ka[2], va[4];
 #pragma unroll
-    for (int i = 0; i < 2; i++) ka[i] = 128 * pi + 16 * ((4 * i + kq) ^ ((pi >> 1) & 7)) + 2048 * PB * pg;
+    for (int i = 0; i < 2; i++) ka[i] = 128 * pi + 16 * ((4 * i + kq) ^ ((pi >> 1) & 6));
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        va[i] = 128 * vr + 16 * ((2 * i + ((lane >> 1) & 1)) ^ ((vr >> 1) & 7)) + 8 * (lane & 1) + 2048 * PB * pg;
+    for (int i = 0; i < 4; i++) va[i] = 128 * vr + 16 * ((2 * i + ((lane >> 1) & 1)) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
 
-    // one step: 32 positions (16: HALF) from row 32 hs of the wave's blocks
-    auto scores = [&](lds_cchar *tile, int hs, f32x4 (&S)[SB][NR]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-            for (int i = 0; i < SB; i++) {
-                const bf16x8 kf = *(const __attribute__((address_space(3))) bf16x8 *)(tile + ka[ks & 1] + GRP * (ks >> 1) + 4096 * hs + 2048 * i);
-#pragma unroll
-                for (int r = 0; r < NR; r++) mfma_vec<ASM>(kf, qb[ks][r], S[i][r], ks == 0);
-            }
-        settle_vec<ASM>(S);
+    constexpr int KF = 4, NF = 2 * KS;   // score fragments in flight, and of a step: fragment 2 ks + block
+    auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {
+        return *(const __attribute__((address_space(3))) bf16x8 *)(buf + ka[(f >> 1) & 1] + TB_GRP * (f >> 2) + 2048 * (f & 1));
     };
-    // S to weights, as the second product's operand
-    auto softmax = [&](const f32x4 (&S)[SB][NR], bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
-        float al[NR];
-        bool moved = false;
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            float mt = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < SB; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mt = fmaxf(mt, S[i][r][e]);
-            mt *= a.scale2;
-            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const bool up = mt > M[r] + TA_LAZY;
-            const float mn = up ? mt : M[r];
-            al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
-            moved = moved || up;
-            M[r] = mn;
-            const float ref = mn == -INFINITY ? 0.0f : mn;
-            bf16x2 w[4];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float p[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (i < SB)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i < SB ? i : 0][r][e], a.scale2, -ref));
-                    }
-                w[2 * i] = __builtin_convertvector(f2{p[0], p[1]}, bf16x2);
-                w[2 * i + 1] = __builtin_convertvector(f2{p[2], p[3]}, bf16x2);
-            }
-            pf[r] = bf16x8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
-        }
-        if (__ballot(moved)) {
-            settle_vec<ASM>(lacc);
-#pragma unroll
-            for (int r = 0; r < NR; r++) lacc[0][r] *= al[r];
-            settle<ASM>(acc);
-#pragma unroll
-            for (int r = 0; r < NR; r++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) acc_scale<ASM>(acc[d][r], al[r]);
-            settle<ASM>(acc);
-        }
-        // the sum of the weights as they are used (bf16), by the matrix unit
-#pragma unroll
-        for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[0][r]);
+    auto vread = [&](lds_cchar *buf, int d) __attribute__((always_inline)) {
+        lds_cchar *at = buf + va[d & 3] + TB_GRP * (d >> 2);
+        const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
+        const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
+        return __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
     };
-    auto values = [&](lds_cchar *tile, int hs, const bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
+    // scores of a step, its first KF fragments already read
+    auto scores = [&](lds_cchar *buf, bf16x8 (&kf)[KF], f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            lds_cchar *at = tile + va[d & 3] + GRP * (d >> 2) + 4096 * hs;
-            const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
-            s16x4 x1 = {0, 0, 0, 0};
-            if constexpr (!HALF) x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
-            const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
-            const bf16x8 vf = __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
+        for (int f = 0; f < NF; f++) {
+            const bf16x8 x = kf[f % KF];
 #pragma unroll
-            for (int r = 0; r < NR; r++) mfma_acc<ASM>(vf, pf[r], acc[d][r]);
+            for (int r = 0; r < NR; r++) mfma_vec<ASM>(x, qb[f >> 1][r], S[f & 1][r], f < 2);
+            if (f + KF < NF) kf[f % KF] = kread(buf, f + KF);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    settle<ASM>(acc);
-
-    // whole tiles of committed positions, then the tiles that hold nodes (one or two)
-    const int tm = min(t1, max(t0, len / TP));
-    lds_char *lds = (lds_char *)smem;
-    auto stage_next = [&](lds_char *nxt, int t) __attribute__((always_inline)) {
-        if (t + 1 < t1) {
-            load_tile(nxt, (t + 1) & 1);
-            find_rows(t + 2);
-        }
+    // the softmax of a step in 28 pieces: S to weights in the second product's operand, M and the factor al
+    // that the sums before it are to be scaled by
+    struct Soft {
+        float mt[NR], ref[NR], al[NR];
+        bool moved;
     };
-    // The two buffers as parameters that do not alias: else the compiler has every transposed read wait for the
-    // loads in flight.
-    auto whole_tile = [&](lds_cchar *__restrict__ cur, lds_char *__restrict__ nxt, int t) __attribute__((always_inline)) {
-        stage_next(nxt, t);
-        const uint64_t ok = reinterpret_cast<const uint64_t *>(s_ok)[t & 1];
+    auto soft_piece = [&](int i, f32x4 (&S)[2][NR], Soft &x, bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
+        if (i < NR) {
+            const f32x4 u = S[0][i], v = S[1][i];
+            x.mt[i] = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+        } else if (i == 2) {
 #pragma unroll
-        for (int hs = 0; hs < NH; hs++) {
-            f32x4 S[SB][NR];
-            bf16x8 pf[NR];
-            scores(cur, hs, S);
-            if (ok != ~0ull) {   // uniform: pages that are none
-#pragma unroll
-                for (int i = 0; i < SB; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (!(ok >> (16 * (PB * pg + 2 * hs + i) + 4 * e + kq) & 1))
-#pragma unroll
-                            for (int r = 0; r < NR; r++) S[i][r][e] = -INFINITY;
-            }
-            softmax(S, pf);
-            values(cur, hs, pf);
-        }
-    };
-    if (t0 < t1) {
-        find_rows(t0);
-        load_tile(lds + (t0 & 1) * TA_TILE, t0 & 1);
-        find_rows(t0 + 1);
-    }
-    for (int t = t0; t < tm; t++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        whole_tile(lds + (t & 1) * TA_TILE, lds + (~t & 1) * TA_TILE, t);
-    }
-    for (int t = tm; t < t1; t++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        stage_next(lds + (~t & 1) * TA_TILE, t);
-        char *tile = smem + (t & 1) * TA_TILE;
-        const uint64_t ok = reinterpret_cast<const uint64_t *>(s_ok)[t & 1];
-        const int s = len - t * TP;   // tile position of the first node
-        uint64_t bad = 0;
-        if (cnt > 1) {
-            // rows of nodes that hold an infinity or a NaN: zeros, and noted, so that the rows that see them
-            // become NaN and no others
-            uint32_t bits = 0;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                char *at = tile + 2048 * wv + 1024 * i + 16 * lane;
-                bool inf = false;
-#pragma unroll
-                for (int g = 0; g < 9; g++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(at + GRP * g);
-                    inf = inf || not_finite16(w.x) || not_finite16(w.y) || not_finite16(w.z) || not_finite16(w.w);
-                }
-                const uint64_t m = __ballot(inf && 16 * wv + 8 * i + lrow >= s);
-                const bool mine = (m >> (lane & 56) & 0xff) != 0;
-                if (mine)
-#pragma unroll
-                    for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + GRP * g) = uint4{0, 0, 0, 0};
-                bits |= gather_rows(__ballot(mine)) << (8 * i);
-            }
-            if (lane == 0) s_ok[8 + wv] = (uint16_t)bits;
-            __syncthreads();
-            bad = reinterpret_cast<const uint64_t *>(s_ok)[2] >> (16 * PB * pg);
-        }
-        uint64_t see[NR];
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            uint64_t w = s >= 64 ? ~0ull : s <= 0 ? 0ull : (1ull << s) - 1;
-            if (s >= 0 && s < 64) w |= anc[r] << s;
-            else if (s < 0 && s > -64) w |= anc[r] >> -s;
-            see[r] = (w & ok) >> (16 * PB * pg);
-        }
-#pragma unroll 1
-        for (int hs = 0; hs < NH; hs++) {
-            f32x4 S[SB][NR];
-            bf16x8 pf[NR];
-            scores(lds + (t & 1) * TA_TILE, hs, S);
-#pragma unroll
-            for (int i = 0; i < SB; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int at = 32 * hs + 16 * i + 4 * e + kq;
-                    const float seen = bad >> at & 1 ? NAN : 0.0f;
-#pragma unroll
-                    for (int r = 0; r < NR; r++) S[i][r][e] = see[r] >> at & 1 ? S[i][r][e] + seen : -INFINITY;
-                }
-            softmax(S, pf);
-            values(lds + (t & 1) * TA_TILE, hs, pf);
-        }
-        if (cnt > 1) __syncthreads();   // the noted rows were read
-    }
-
-    settle<ASM>(acc);
-    settle_vec<ASM>(lacc);
-    float lsum[NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) lsum[r] = lacc[0][r][0];
-    if constexpr (PG > 1) {
-        // position groups 1 .. PG - 1 hand their sums to group 0, 16 bytes a lane and tile
-        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);
-        float *xm = reinterpret_cast<float *>(smem + (PG - 1) * RG * NR * DT * 64 * 16);
-        static_assert((PG - 1) * RG * NR * (DT * 64 * 16 + 512) <= 2 * TA_TILE, "exchange fits the tiles");
-        __syncthreads();
-        if (pg > 0) {
+            for (int r = 0; r < NR; r++) x.mt[r] = quarter_max(x.mt[r]) * a.scale2;
+        } else if (i == 3) {
+            x.moved = false;
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const int at = (((pg - 1) * RG + rg) * NR + r) * 64 + lane;
-                xm[2 * at] = M[r];
-                xm[2 * at + 1] = lsum[r];
-#pragma unroll
-                for (int d = 0; d < DT; d++) xo[(size_t)(((pg - 1) * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] = acc[d][r];
+                const bool up = x.mt[r] > M[r] + TA_LAZY;
+                const float mn = up ? x.mt[r] : M[r];
+                x.al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
+                x.moved = x.moved || up;
+                M[r] = mn;
+                x.ref[r] = mn == -INFINITY ? 0.0f : mn;
             }
+        } else if (i >= 4 && i < 4 + 8 * NR) {
+            const int k = i - 4, r = k >> 3, e = k & 7;
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e >> 2][r][e & 3], a.scale2, -x.ref[r]));
+            asm volatile("" : "+v"(p));   // here, not where it is used
+            S[e >> 2][r][e & 3] = p;
+        } else if (i >= 20 && i < 20 + 4 * NR) {
+            const int k = i - 20, r = k >> 2, w = k & 3;
+            const bf16x2 y = __builtin_convertvector(f2{S[w >> 1][r][2 * (w & 1)], S[w >> 1][r][2 * (w & 1) + 1]}, bf16x2);
+            pf[r][2 * w] = y[0];
+            pf[r][2 * w + 1] = y[1];
         }
-        __syncthreads();
-        if (pg > 0) return;
+    };
+    auto rescale = [&](const Soft &x) __attribute__((always_inline)) {
+        if (!__ballot(x.moved)) return;
+        wait<ASM>();
+#pragma unroll
+        for (int r = 0; r < NR; r++) lacc[r] *= x.al[r];
 #pragma unroll
         for (int r = 0; r < NR; r++)
-#pragma unroll 1
-            for (int g = 0; g < PG - 1; g++) {
-                const int at = ((g * RG + rg) * NR + r) * 64 + lane;
-                const float m2 = xm[2 * at], l2 = xm[2 * at + 1], mm = fmaxf(M[r], m2);
-                const float w1 = M[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[r] - mm);
-                const float w2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mm);
-                lsum[r] = lsum[r] * w1 + l2 * w2;
-                M[r] = mm;
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-                    acc[d][r] = acc[d][r] * w1 + xo[(size_t)((g * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] * w2;
+            for (int d = 0; d < DT; d++) acc_scale<ASM>(acc[d][r], x.al[r]);
+        wait<ASM>();
+    };
+    constexpr int VF = 4;   // sum fragments in flight
+    auto publish = [](int left) __attribute__((always_inline)) {   // this wave's loads but the last `left`, then every wave's
+        if (left) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto mask_pages = [&](int s, f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)]);
+        if (ok == 0xffffffffu) return;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (!(ok >> (16 * i + 4 * e + kq) & 1))
+#pragma unroll
+                    for (int r = 0; r < NR; r++) S[i][r][e] = -INFINITY;
+    };
+
+    // steps s0 .. s0 + 2 on their way, the page of s0 + 3 looked up
+    const int sm = min(s1, max(s0, len / TB_TP));   // whole steps of committed positions end here
+    {
+        int pg[3], in[3];
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+            find_rows(s0 + i);
+            pg[i] = pgn;
+            in[i] = pgo;
+        }
+        find_rows(s0 + 3);
+#pragma unroll
+        for (int i = 0; i < 3; i++) load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i), pg[i], in[i]);
+    }
+    if (s0 < sm) {
+        f32x4 S[2][NR];
+        bf16x8 kf[KF], pf[NR];
+        Soft x;
+        publish(9);
+        {
+            lds_cchar *cur = lds + buf_of(s0) * TB_BUF;
+#pragma unroll
+            for (int f = 0; f < KF; f++) kf[f] = kread(cur, f);
+            scores(cur, kf, S);
+            wait<ASM>();
+            mask_pages(s0, S);
+#pragma unroll
+            for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
+            cur = lds + buf_of(s0 + 1) * TB_BUF;
+            if (s0 + 1 < sm)
+#pragma unroll
+                for (int f = 0; f < KF; f++) kf[f] = kread(cur, f);
+        }
+        // Step s's sum and step s + 1's scores. The buffers as parameters that do not alias: else the compiler
+        // has every transposed read wait for the loads in flight.
+        auto step = [&](lds_cchar *__restrict__ cur, lds_cchar *__restrict__ nxt, lds_cchar *__restrict__ nx2,
+                        lds_char *__restrict__ fill, int s) __attribute__((always_inline)) {
+            const int page = pgn, in = pgo;
+            find_rows(s + 4);
+            load_step(fill, buf_of(s + 3), page, in);
+            scores(nxt, kf, S);
+            bf16x8 vf[VF], pn[NR];
+#pragma unroll
+            for (int d = 0; d < VF; d++) vf[d] = vread(cur, d);
+#pragma unroll
+            for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
+            wait<ASM>();
+            mask_pages(s + 1, S);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const bf16x8 v = vf[d % VF];
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
+                if (d + VF < DT) vf[d % VF] = vread(cur, d + VF);
+                if (d < 28) soft_piece(d, S, x, pn);
+                if (d == DT - VF - 1) {
+                    // every fragment of step s is in registers: its buffer is free behind the barrier
+                    publish(9);
+#pragma unroll
+                    for (int f = 0; f < KF; f++) kf[f] = kread(nx2, f);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            wait<ASM>();   // also for what the compiler moves at the loop's end
+            rescale(x);
+#pragma unroll
+            for (int r = 0; r < NR; r++) pf[r] = pn[r];
+        };
+        rescale(x);
+        for (int s = s0; s + 1 < sm; s++)
+            step(lds + buf_of(s) * TB_BUF, lds + buf_of(s + 1) * TB_BUF, lds + buf_of(s + 2) * TB_BUF, lds + buf_of(s + 3) * TB_BUF, s);
+        {
+            lds_cchar *cur = lds + buf_of(sm - 1) * TB_BUF;
+            const int page = pgn, in = pgo;
+            publish(0);
+            load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2), page, in);
+#pragma unroll
+            for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const bf16x8 v = vread(cur, d);
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
+            }
+            wait<ASM>();
+        }
+    }
+    // the steps that hold nodes: at most three, on their way by now
+    for (int s = sm; s < s1; s++) {
+        publish(0);
+        char *at = smem + buf_of(s) * TB_BUF + 1024 * wv + 16 * lane;
+        lds_cchar *cur = lds + buf_of(s) * TB_BUF;
+        const uint32_t ok = reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)];
+        const int n0 = len - s * TB_TP;   // place of the first node in the step
+        uint32_t bad = 0;
+        if (cnt > 1) {
+            // rows of nodes that hold an infinity or a NaN: zeros, and noted, so that the query rows that see
+            // them become NaN and no others
+            bool inf = false;
+#pragma unroll
+            for (int g = 0; g < 9; g++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(at + TB_GRP * g);
+                inf = inf || not_finite16(w.x) || not_finite16(w.y) || not_finite16(w.z) || not_finite16(w.w);
+            }
+            const uint64_t m = __ballot(inf && prow >= n0);
+            const bool mine = (m >> (lane & 56) & 0xff) != 0;
+            if (mine)
+#pragma unroll
+                for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + TB_GRP * g) = uint4{0, 0, 0, 0};
+            const uint32_t bits = gather_rows(__ballot(mine));
+            if (lane == 0) s_ok[16 + wv] = (uint8_t)bits;
+            __syncthreads();
+            bad = reinterpret_cast<const uint32_t *>(s_ok)[4];
+        }
+        f32x4 S[2][NR];
+        bf16x8 kf[KF], pf[NR];
+        Soft x;
+#pragma unroll
+        for (int f = 0; f < KF; f++) kf[f] = kread(cur, f);
+        scores(cur, kf, S);
+        wait<ASM>();
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
+            if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc[r] << n0);
+            else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc[r] >> -n0);
+            w &= ok;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int bit = 16 * i + 4 * e + kq;
+                    const float seen = bad >> bit & 1 ? NAN : 0.0f;
+                    S[i][r][e] = w >> bit & 1 ? S[i][r][e] + seen : -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
+        rescale(x);
+#pragma unroll
+        for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const bf16x8 v = vread(cur, d);
+#pragma unroll
+            for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
+        }
+        wait<ASM>();
     }
 
+    const bool split = splits > 1;
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         if (row[r] >= rows) continue;
-        const bool split = a.nsplit > 1;
-        const size_t orow = (size_t)b * a.t.N * H + row[r];
-        const size_t prow = part * ROWS + (row[r] - r0);
+        const float l = lacc[r][0];
+        const size_t orow = (size_t)b * a.t.N * H + row[r], prow = (size_t)id * ROWS + (row[r] - r0);
         if (split) {
             if (kq == 0) {
                 a.pm[prow] = M[r];
-                a.pl[prow] = lsum[r];
+                a.pl[prow] = l;
             }
             if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
-        } else if (kq == 0 && a.lse) {
-            a.lse[orow] = lsum[r] == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(lsum[r])) * TA_LN2;
-        }
-        const float inv = split ? 1.0f : lsum[r] == 0.0f ? 0.0f : 1.0f / lsum[r];
+            float *dst = a.po + prow * KL + 4 * kq;
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const int ch = 16 * d + 4 * kq;
-            const f32x4 v = acc[d][r] * inv;
-            if (ch >= KL) continue;
-            if (split) *reinterpret_cast<f32x4 *>(a.po + prow * KL + ch) = v;
-            else if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * KL + ch) = v;
-            else
-                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * KL + ch) =
-                    uint2{(uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16)};
+            for (int d = 0; d < DT; d++)
+                if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r];
+        } else {
+            if (kq == 0 && a.lse) a.lse[orow] = l == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(l)) * TA_LN2;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (a.o_dt == K3HIP_F32) {
+                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * kq;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+                    if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r] * inv;
+            } else {
+                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * kq;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+                    if (16 * d + 4 * kq < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d][r] * inv);
+            }
         }
     }
 }
@@ -879,29 +1007,36 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 __global__ __launch_bounds__(TA_NT) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows)
 {
     const int b = blockIdx.y, lane = threadIdx.x & 63, row = blockIdx.x * (TA_NT / 64) + (threadIdx.x >> 6);
-    if (row >= tree_count(a.t, b) * a.H) return;
+    const int rows = tree_count(a.t, b) * a.H;
+    if (row >= rows) return;
     const int rt = row / tile_rows;
-    const size_t p0 = ((size_t)b * a.nrt + rt) * a.nsplit * tile_rows + row % tile_rows;
+    int first = (b * a.nrt + rt) * a.nsplit, n = a.nsplit, step = 1;
+    if (a.plan) {
+        const int2 p = a.plan[b];
+        n = p.y;
+        if (n <= 1) return;   // written by its only workgroup
+        first = p.x + rt;
+        step = (rows + tile_rows - 1) / tile_rows;
+    }
+    const size_t p0 = (size_t)first * tile_rows + row % tile_rows, pd = (size_t)step * tile_rows;
     float M = -INFINITY, l = 0.0f;
-    for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, a.pm[p0 + (size_t)s * tile_rows]);
+    for (int s = 0; s < n; s++) M = fmaxf(M, a.pm[p0 + s * pd]);
     for (int c0 = 0; c0 < a.KL; c0 += 256) {
         const int c = c0 + 4 * lane;
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         l = 0.0f;
-        for (int s = 0; s < a.nsplit; s++) {
-            const float m = a.pm[p0 + (size_t)s * tile_rows];
+        for (int s = 0; s < n; s++) {
+            const float m = a.pm[p0 + s * pd];
             if (m == -INFINITY) continue;
             const float w = __builtin_amdgcn_exp2f(m - M);
-            l += w * a.pl[p0 + (size_t)s * tile_rows];
-            if (c < a.KL) v += w * *reinterpret_cast<const f32x4 *>(a.po + (p0 + (size_t)s * tile_rows) * a.KL + c);
+            l += w * a.pl[p0 + s * pd];
+            if (c < a.KL) v += w * *reinterpret_cast<const f32x4 *>(a.po + (p0 + s * pd) * a.KL + c);
         }
         if (c < a.KL) {
             const size_t at = ((size_t)b * a.t.N * a.H + row) * a.KL + c;
             v *= l == 0.0f ? 0.0f : 1.0f / l;
             if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + at) = v;
-            else
-                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + at) =
-                    uint2{(uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16)};
+            else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + at) = pack4(v);
         }
     }
     if (a.lse && lane == 0)
@@ -912,7 +1047,7 @@ __global__ __launch_bounds__(TA_NT) void tree_attn_merge_kernel(const AttnArgs a
 int ta_rows(bool f32, long rows)
 {
     if (f32) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    return rows <= 64 ? 64 : 128;
 }
 
 int ta_split(int B, int nrt, int tiles)
@@ -923,11 +1058,21 @@ int ta_split(int B, int nrt, int tiles)
     return (int)std::max(1L, std::min({(long)tiles, ncu / wg, 64L}));
 }
 
-size_t ta_ws_bytes(int B, int rows, int nrt, int nsplit, int KL)
+// bf16: a range a CU, two where the row tiles alone are more.
+int ta_room(int B, int nrt)
 {
-    if (nsplit <= 1) return 0;
-    const size_t r = (size_t)B * nrt * nsplit * rows;
-    return ((r * KL * 4 + 255) & ~(size_t)255) + 2 * ((r * 4 + 255) & ~(size_t)255);
+    int ncu = 256;
+    (void)cu_count(ncu);
+    return (long)B * nrt <= ncu ? ncu : 2 * ncu;
+}
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Partials of `ranges` ranges of `rows` rows, and the plan of B sequences.
+size_t ta_ws_bytes(long ranges, int rows, int KL, int B)
+{
+    const size_t r = (size_t)ranges * rows;
+    return up256(r * KL * 4) + 2 * up256(r * 4) + up256((size_t)B * sizeof(int2));
 }
 
 }  // namespace
@@ -939,12 +1084,10 @@ using namespace k3kda;
 extern "C" size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora)
 {
     if (B <= 0 || N <= 0 || N > TREE_MAX || H <= 0 || kv_lora <= 0 || kv_lora > TA_KL) return 0;
-    size_t most = 0;
-    for (int f32 = 0; f32 < 2; f32++) {
-        const int rows = ta_rows(f32, (long)N * H), nrt = (int)(((long)N * H + rows - 1) / rows);
-        most = std::max(most, ta_ws_bytes(B, rows, nrt, ta_split(B, nrt, 1 << 20), kv_lora));
-    }
-    return std::max<size_t>(most, 256);
+    const int r4 = ta_rows(true, (long)N * H), n4 = (int)(((long)N * H + r4 - 1) / r4);
+    const int r2 = ta_rows(false, (long)N * H), n2 = (int)(((long)N * H + r2 - 1) / r2);
+    return std::max(ta_ws_bytes((long)B * n4 * ta_split(B, n4, 1 << 20), r4, kv_lora, B),
+                    ta_ws_bytes(ta_room(B, n2), r2, kv_lora, B));
 }
 
 extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int rope, float scale, const void *q,
@@ -979,37 +1122,54 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     a.scale2 = scale * TA_LOG2E;
     const int rows = ta_rows(f32, (long)N * H);
     a.nrt = (int)(((long)N * H + rows - 1) / rows);
-    const long tiles = ((long)max_pages * page + N + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
-    a.nsplit = ta_split(B, a.nrt, (int)tiles);
-    const size_t need = ta_ws_bytes(B, rows, a.nrt, a.nsplit, kv_lora);
+    a.B = B;
+    const long tp = f32 ? 32 : TB_TP, tiles = ((long)max_pages * page + N + tp - 1) / tp;
+    long ranges;
+    bool split;
+    if (f32) {
+        a.nsplit = ta_split(B, a.nrt, (int)tiles);
+        ranges = (long)B * a.nrt * a.nsplit;
+        split = a.nsplit > 1;
+    } else {
+        a.room = ta_room(B, a.nrt);
+        ranges = a.room;
+        split = tiles > 1 && (long)B * a.nrt < a.room;
+        if (!split) a.room = 0;
+    }
     StreamBuf buf;
-    if (need) {
+    if (split) {
+        const size_t need = ta_ws_bytes(ranges, rows, kv_lora, B);
         if (!workspace) {
             if (int rc = stream_alloc(buf, need, st)) return rc;
             workspace = buf.p;
         } else if (workspace_bytes < need || ((uintptr_t)workspace & 15)) {
             K3_FAIL(K3HIP_EINVAL, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
         }
-        const size_t r = (size_t)B * a.nrt * a.nsplit * rows;
+        const size_t r = (size_t)ranges * rows;
         a.po = (float *)workspace;
-        a.pm = (float *)((char *)workspace + ((r * kv_lora * 4 + 255) & ~(size_t)255));
-        a.pl = (float *)((char *)a.pm + ((r * 4 + 255) & ~(size_t)255));
+        a.pm = (float *)((char *)workspace + up256(r * kv_lora * 4));
+        a.pl = (float *)((char *)a.pm + up256(r * 4));
+        if (!f32) a.plan = (int2 *)((char *)a.pl + up256(r * 4));
     }
     const void *kern;
-    if (f32)
+    dim3 grid;
+    size_t lds;
+    if (f32) {
         kern = rows == 16 ? (const void *)tree_attn_kernel<true, 1, 1, 2> : rows == 32 ? (const void *)tree_attn_kernel<true, 1, 2, 2>
                                                                                       : (const void *)tree_attn_kernel<true, 1, 4, 1>;
-#define K3_TA(F)                                                                                        \
-    (rows == 16   ? (const void *)tree_attn16_kernel<F, 1, 1, 4>                                               \
-     : rows == 32 ? (const void *)tree_attn16_kernel<F, 1, 2, 2>                                               \
-     : rows == 64 ? (const void *)tree_attn16_kernel<F, 2, 2, 2> : (const void *)tree_attn16_kernel<F, 2, 4, 1>)
-    else kern = CW == TA_CW ? K3_TA(true) : K3_TA(false);
-#undef K3_TA
-    K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, TA_LDS));
+        grid = dim3(a.nsplit, a.nrt, B);
+        lds = TA_LDS;
+    } else {
+        kern = CW == TA_CW ? (rows == 64 ? (const void *)tree_attn16_kernel<true, 1> : (const void *)tree_attn16_kernel<true, 2>)
+                           : (rows == 64 ? (const void *)tree_attn16_kernel<false, 1> : (const void *)tree_attn16_kernel<false, 2>);
+        grid = dim3((unsigned)((std::max((long)a.room, (long)B * a.nrt) + 7) & ~7L));   // a multiple of the XCDs
+        lds = TB_LDS;
+    }
+    K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *args[] = {&a};
-    K3_HIP(hipLaunchKernel(kern, dim3(a.nsplit, a.nrt, B), dim3(TA_NT), args, TA_LDS, st));
+    K3_HIP(hipLaunchKernel(kern, grid, dim3(TA_NT), args, lds, st));
     K3_LAUNCHED();
-    if (a.nsplit > 1) {
+    if (split) {
         const int per = TA_NT / 64;
         hipLaunchKernelGGL(tree_attn_merge_kernel, dim3((unsigned)(((long)N * H + per - 1) / per), (unsigned)B), dim3(TA_NT),
                            0, st, a, rows);
