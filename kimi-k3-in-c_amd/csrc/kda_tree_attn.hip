@@ -686,25 +686,30 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     // staging: wave wv brings rows 8 wv .. + 7 of a step
     const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
     int pgn = -1, pgo = 0;   // page and row in it of this lane's row of the step loaded next
-    auto find_rows = [&](int s) __attribute__((always_inline)) {
-        const int pos = s * TB_TP + prow, at = pos / a.c.page;
-        pgo = pos - at * a.c.page;
-        pgn = -1;
-        if (pos < end && at < a.c.max_pages) pgn = a.c.table[(size_t)b * a.c.max_pages + at];
+    auto find_rows = [&](int s) __attribute__((always_inline)) {   // no branch: it stands between products
+        const uint32_t pos = (uint32_t)(s * TB_TP + prow), at = pos / (uint32_t)a.c.page;
+        const bool in = (int)pos < end && (int)at < a.c.max_pages;
+        pgo = (int)(pos - at * (uint32_t)a.c.page);
+        const int n = a.c.table[(size_t)b * a.c.max_pages + (in ? at : 0u)];
+        pgn = in ? n : -1;
     };
-    auto load_step = [&](lds_char *dst, int buf, int page, int in) __attribute__((always_inline)) {
+    const char *ldp = nullptr;   // this lane's row of the step being loaded
+    auto load_row = [&](int buf, int page, int in) __attribute__((always_inline)) {
         const bool ok = page >= 0 && page < a.c.n_pages;
-        const char *p = ok ? reinterpret_cast<const char *>(a.pages) + ((size_t)page * a.c.page + in) * (CW * 2)
-                           : reinterpret_cast<const char *>(ta_zeros);
-        p += 16 * lu;
+        const char *p = reinterpret_cast<const char *>(a.pages) + ((size_t)(ok ? page : 0) * a.c.page + in) * (CW * 2);
+        ldp = (ok ? p : reinterpret_cast<const char *>(ta_zeros)) + 16 * lu;
         const uint32_t okb = gather_rows(__ballot(ok));
         if (lane == 0) s_ok[4 * buf + wv] = (uint8_t)okb;
+    };
+    auto load_group = [&](lds_char *dst, int g) __attribute__((always_inline)) {
+        const char *src = ldp + 128 * g;
+        if (!FULL && 8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
+        __builtin_amdgcn_global_load_lds((glb_void *)src, (lds_void *)(dst + TB_GRP * g + 1024 * wv), 16, 0, 0);
+    };
+    auto load_step = [&](lds_char *dst, int buf, int page, int in) __attribute__((always_inline)) {
+        load_row(buf, page, in);
 #pragma unroll
-        for (int g = 0; g < 9; g++) {
-            const char *src = p + 128 * g;
-            if (!FULL && 8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
-            __builtin_amdgcn_global_load_lds((glb_void *)src, (lds_void *)(dst + TB_GRP * g + 1024 * wv), 16, 0, 0);
-        }
+        for (int g = 0; g < 9; g++) load_group(dst, g);
     };
     auto buf_of = [](int s) { return s & (TB_NB - 1); };
     lds_char *lds = (lds_char *)smem;
@@ -729,7 +734,8 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 #pragma unroll
     for (int i = 0; i < 4; i++) va[i] = 128 * vr + 16 * ((2 * i + ((lane >> 1) & 1)) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
 
-    constexpr int KF = 4, NF = 2 * KS;   // score fragments in flight, and of a step: fragment 2 ks + block
+    // fragments read ahead, and score fragments of a step (fragment 2 ks + block)
+    constexpr int AH = 8, NF = 2 * KS;
     auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {
         return *(const __attribute__((address_space(3))) bf16x8 *)(buf + ka[(f >> 1) & 1] + TB_GRP * (f >> 2) + 2048 * (f & 1));
     };
@@ -740,14 +746,31 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
         return __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
     };
-    // scores of a step, its first KF fragments already read
-    auto scores = [&](lds_cchar *buf, bf16x8 (&kf)[KF], f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
+    // Scores of a step, its first AH fragments already read; the last AH products read the first fragments of
+    // the sum from `sum`. between(f): work that goes between the products.
+    auto scores = [&](lds_cchar *buf, lds_cchar *sum, bf16x8 (&kf)[AH], bf16x8 (&vf)[AH], f32x4 (&S)[2][NR], auto between)
+                      __attribute__((always_inline)) {
 #pragma unroll
         for (int f = 0; f < NF; f++) {
-            const bf16x8 x = kf[f % KF];
+            const bf16x8 x = kf[f % AH];
 #pragma unroll
             for (int r = 0; r < NR; r++) mfma_vec<ASM>(x, qb[f >> 1][r], S[f & 1][r], f < 2);
-            if (f + KF < NF) kf[f % KF] = kread(buf, f + KF);
+            if (f + AH < NF) kf[f % AH] = kread(buf, f + AH);
+            else vf[f + AH - NF] = vread(sum, f + AH - NF);
+            between(f);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto nothing = [](int) __attribute__((always_inline)) {};
+    // The sum of a step, its first AH fragments already read; between(d) before the next fragment but AH is read.
+    auto values = [&](lds_cchar *buf, bf16x8 (&vf)[AH], const bf16x8 (&pf)[NR], auto between) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const bf16x8 v = vf[d % AH];
+#pragma unroll
+            for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
+            if (d + AH < DT) vf[d % AH] = vread(buf, d + AH);
+            between(d);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -798,7 +821,6 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
             for (int d = 0; d < DT; d++) acc_scale<ASM>(acc[d][r], x.al[r]);
         wait<ASM>();
     };
-    constexpr int VF = 4;   // sum fragments in flight
     auto publish = [](int left) __attribute__((always_inline)) {   // this wave's loads but the last `left`, then every wave's
         if (left) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -834,74 +856,64 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     }
     if (s0 < sm) {
         f32x4 S[2][NR];
-        bf16x8 kf[KF], pf[NR];
+        bf16x8 kf[AH], vf[AH], pf[NR];
         Soft x;
         publish(9);
         {
             lds_cchar *cur = lds + buf_of(s0) * TB_BUF;
 #pragma unroll
-            for (int f = 0; f < KF; f++) kf[f] = kread(cur, f);
-            scores(cur, kf, S);
+            for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
+            scores(cur, cur, kf, vf, S, nothing);
             wait<ASM>();
             mask_pages(s0, S);
 #pragma unroll
             for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
             cur = lds + buf_of(s0 + 1) * TB_BUF;
-            if (s0 + 1 < sm)
 #pragma unroll
-                for (int f = 0; f < KF; f++) kf[f] = kread(cur, f);
+            for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
         }
+        rescale(x);
         // Step s's sum and step s + 1's scores. The buffers as parameters that do not alias: else the compiler
         // has every transposed read wait for the loads in flight.
         auto step = [&](lds_cchar *__restrict__ cur, lds_cchar *__restrict__ nxt, lds_cchar *__restrict__ nx2,
                         lds_char *__restrict__ fill, int s) __attribute__((always_inline)) {
-            const int page = pgn, in = pgo;
-            find_rows(s + 4);
-            load_step(fill, buf_of(s + 3), page, in);
-            scores(nxt, kf, S);
-            bf16x8 vf[VF], pn[NR];
-#pragma unroll
-            for (int d = 0; d < VF; d++) vf[d] = vread(cur, d);
+            scores(nxt, cur, kf, vf, S, [&](int f) __attribute__((always_inline)) {
+                if (f == 2) load_row(buf_of(s + 3), pgn, pgo);
+                if (f == 4) find_rows(s + 4);
+                if (f >= 8 && f < 26 && f % 2 == 0) load_group(fill, (f - 8) / 2);
+            });
+            bf16x8 pn[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
             wait<ASM>();
             mask_pages(s + 1, S);
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const bf16x8 v = vf[d % VF];
-#pragma unroll
-                for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
-                if (d + VF < DT) vf[d % VF] = vread(cur, d + VF);
+            values(cur, vf, pf, [&](int d) __attribute__((always_inline)) {
                 if (d < 28) soft_piece(d, S, x, pn);
-                if (d == DT - VF - 1) {
+                if (d == 28) {
                     // every fragment of step s is in registers: its buffer is free behind the barrier
                     publish(9);
 #pragma unroll
-                    for (int f = 0; f < KF; f++) kf[f] = kread(nx2, f);
+                    for (int f = 0; f < 4; f++) kf[f] = kread(nx2, f);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                if (d > 28) kf[d - 25] = kread(nx2, d - 25);
+                if (d == 31) kf[7] = kread(nx2, 7);
+            });
             wait<ASM>();   // also for what the compiler moves at the loop's end
             rescale(x);
 #pragma unroll
             for (int r = 0; r < NR; r++) pf[r] = pn[r];
         };
-        rescale(x);
         for (int s = s0; s + 1 < sm; s++)
             step(lds + buf_of(s) * TB_BUF, lds + buf_of(s + 1) * TB_BUF, lds + buf_of(s + 2) * TB_BUF, lds + buf_of(s + 3) * TB_BUF, s);
         {
             lds_cchar *cur = lds + buf_of(sm - 1) * TB_BUF;
-            const int page = pgn, in = pgo;
             publish(0);
-            load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2), page, in);
+            load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2), pgn, pgo);
+#pragma unroll
+            for (int d = 0; d < AH; d++) vf[d] = vread(cur, d);
 #pragma unroll
             for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const bf16x8 v = vread(cur, d);
-#pragma unroll
-                for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
-            }
+            values(cur, vf, pf, nothing);
             wait<ASM>();
         }
     }
@@ -933,11 +945,11 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
             bad = reinterpret_cast<const uint32_t *>(s_ok)[4];
         }
         f32x4 S[2][NR];
-        bf16x8 kf[KF], pf[NR];
+        bf16x8 kf[AH], vf[AH], pf[NR];
         Soft x;
 #pragma unroll
-        for (int f = 0; f < KF; f++) kf[f] = kread(cur, f);
-        scores(cur, kf, S);
+        for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
+        scores(cur, cur, kf, vf, S, nothing);
         wait<ASM>();
 #pragma unroll
         for (int r = 0; r < NR; r++) {
@@ -959,12 +971,7 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         rescale(x);
 #pragma unroll
         for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const bf16x8 v = vread(cur, d);
-#pragma unroll
-            for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
-        }
+        values(cur, vf, pf, nothing);
         wait<ASM>();
     }
 
