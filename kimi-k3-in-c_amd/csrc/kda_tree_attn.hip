@@ -56,8 +56,8 @@ constexpr int TA_LDS = 2 * TA_TILE + 64;       // two tiles, their rows' validit
 constexpr float TA_LOG2E = 1.4426950408889634f, TA_LN2 = 0.6931471805599453f;
 constexpr float TA_LAZY = 8.0f;                // log2 of the largest weight before a rescale
 
-// What rows without a page and channels past CW are staged from.
-__device__ const uint4 ta_zeros[TA_CW * 4 / 16] = {};
+// What rows without a page and channels past CW are staged from: eight rows of bf16.
+__device__ const uint4 ta_zeros[8 * TA_CW * 2 / 16] = {};
 
 struct AttnArgs {
     TreeSeqs t;
@@ -70,8 +70,10 @@ struct AttnArgs {
     float scale2;     // scale log2(e)
     int nsplit, nrt;  // fp32: position ranges a sequence, row tiles a sequence
     float *po, *pm, *pl;   // partials of each range [rows of a tile] ( x KL)
-    int B, room;      // bf16: workgroups that the ranges may take
-    int2 *plan;       // [B] first range, ranges a row tile
+    int B;
+    uint32_t page_bytes;
+    int tcol, trow;   // bf16: a step in table columns and rows
+    int4 *plan;       // bf16: [B] first and last slot, workgroups a slot
 };
 
 template <bool F32, int NR, int RG, int PG>
@@ -514,13 +516,13 @@ __device__ __forceinline__ uint2 pack4(const f32x4 &v)
     return uint2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
 }
 
-// Which workgroup takes what. Sequence b's positions are cut, for each of its row tiles, into as many equal
-// ranges as all workgroups of the launch can take with one common quota of steps, the smallest that fits
-// (`room` workgroups), so that sequences of different lengths end together. Ranges are numbered sequence by
-// sequence, range by range, row tile by row tile, and go to the XCDs in runs of neighbours: row tiles that
-// read the same positions share an L2.
-struct Share {
-    int b, rt, split, splits;
+// Which workgroup takes what. All sequences' steps stand on one axis, cut into equal slots; a slot takes the n
+// workgroups that the most row tiles of a sequence need, one each, so the workgroups of a slot walk the same
+// positions (and stand on one XCD, where they share its L2), and sequences of different lengths cost no
+// one a wait. A slot that ends inside a sequence leaves that sequence's sums as a part, merged after.
+struct Slots {
+    int n, count;   // workgroups a slot, slots
+    int steps;      // of all sequences (the host checks that this fits an int)
 };
 
 // Sequence b's row tiles (of `rows` rows) and steps (of `tp` positions).
@@ -531,28 +533,21 @@ __device__ __forceinline__ void seq_size(const AttnArgs &a, int b, int rows, int
     steps = cnt ? (paged_len(a.c, a.t.lens, b) + cnt + tp - 1) / tp : 0;
 }
 
-__device__ __forceinline__ int wave_sum(int x)
-{
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
-    return x;
-}
+__device__ __forceinline__ int slot_start(const Slots &s, int k) { return (int)((uint64_t)s.steps * (uint32_t)k / (uint32_t)s.count); }
+__device__ __forceinline__ int slot_of(const Slots &s, int step) { return (int)(((uint64_t)(step + 1) * (uint32_t)s.count - 1) / (uint32_t)s.steps); }
 
-// Every wave works it out for itself, a sequence a lane. With R row tiles in all, T steps over all of them
-// and W workgroups, a quota q needs at least T / q and fewer than T / q + R workgroups, so the smallest
-// one lies in [T / W, T / (W - R)]. False: nothing for this workgroup. Workgroup number 0 writes the plan
-// down for the merge: each sequence's first number and its ranges.
-__device__ __forceinline__ bool find_share(const AttnArgs &a, int rows, int tp, int id, Share &s)
+// The slots, and the sequence b that step `slot_start` of workgroup id's slot lies in, with the step that
+// sequence begins at; every wave works it out for itself, a sequence a lane. Workgroup 0 writes down for the
+// merge which slots each sequence begins and ends in.
+__device__ __forceinline__ bool find_slot(const AttnArgs &a, int rows, int tp, int id, int most, Slots &s, int &b, int &begin)
 {
     const int lane = threadIdx.x & 63;
-    int R = 0, most = 0, nrt0 = 0, steps0 = 0;
-    float T = 0.0f;   // an estimate: the bounds it gives are widened
+    int n = 0, nrt0 = 0, steps0 = 0, T = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int nrt = 0, steps = 0;
         if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
-        R += nrt;
-        most = max(most, steps);
-        T += (float)nrt * (float)steps;
+        n = max(n, nrt);
+        T += steps;
         if (b0 == 0) {
             nrt0 = nrt;
             steps0 = steps;
@@ -560,60 +555,52 @@ __device__ __forceinline__ bool find_share(const AttnArgs &a, int rows, int tp, 
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
-        R += __shfl_xor(R, m, 64);
+        n = max(n, __shfl_xor(n, m, 64));
         T += __shfl_xor(T, m, 64);
-        most = max(most, __shfl_xor(most, m, 64));
     }
-    if (R == 0) return false;
-    int lo = most, hi = most;   // without room: whole sequences
-    if (R < a.room) {
-        lo = min(most, max(1, (int)(T * 0.999f / (float)a.room)));
-        hi = min(most, (int)(T * 1.001f / (float)(a.room - R)) + 2);
-    }
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        int n = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64) {
-            int nrt = nrt0, steps = steps0;
-            if (b0 > 0) {
-                nrt = steps = 0;
-                if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
-            }
-            n += nrt * ((steps + mid - 1) / mid);
-        }
-        if (wave_sum(n) <= a.room) hi = mid;
-        else lo = mid + 1;
-    }
+    n = __builtin_amdgcn_readfirstlane(n);
+    if (n == 0) return false;
+    s.n = n;
+    s.steps = __builtin_amdgcn_readfirstlane(T);
+    s.count = min(max(1, most / n), s.steps);
+    const int k = id / n;
+    if (k >= s.count) return false;
+    const int from = slot_start(s, k);
     int base = 0;
     bool found = false;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int nrt = nrt0, steps = steps0;
         if (b0 > 0) {
-            nrt = steps = 0;
+            steps = 0;
             if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
         }
-        const int sp = (steps + hi - 1) / hi, n = nrt * sp;
-        int end = n;
+        int end = steps;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
             const int x = __shfl_up(end, m, 64);
             if (lane >= m) end += x;
         }
-        const int first = base + end - n;
-        if (id == 0 && a.plan && threadIdx.x < 64 && b0 + lane < a.B) a.plan[b0 + lane] = int2{first, sp};
-        const uint64_t in = __ballot(id >= first && id < first + n);
+        const int first = base + end - steps;
+        if (id == 0 && threadIdx.x < 64 && b0 + lane < a.B && steps)
+            a.plan[b0 + lane] = int4{slot_of(s, first), slot_of(s, first + steps - 1), n, 0};
+        const uint64_t in = __ballot(from >= first && from < first + steps);
         if (in && !found) {
-            const int l = __builtin_ctzll(in), at = id - __builtin_amdgcn_readlane(first, l);
-            const int rt = __builtin_amdgcn_readlane(nrt, l);
-            s.b = b0 + l;
-            s.splits = __builtin_amdgcn_readlane(sp, l);
-            s.split = at / rt;
-            s.rt = at - s.split * rt;
+            const int l = __builtin_ctzll(in);
+            b = b0 + l;
+            begin = __builtin_amdgcn_readlane(first, l);
             found = true;
+            if (id != 0) break;
         }
-        base += __shfl(end, 63, 64);
+        base += __builtin_amdgcn_readlane(end, 63);
     }
-    return found;
+    return true;
+}
+
+// x, worked out anew from here on: what the compiler would else keep in registers over the whole loop.
+__device__ __forceinline__ int opaque(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // The larger of x and the values of lanes l ^ 16, l ^ 32, l ^ 48.
@@ -635,79 +622,112 @@ __device__ __forceinline__ float quarter_max(float x)
 // them, two or three vector instructions to a product; the barrier of a step stands before the sum's last
 // eight products, behind which the next scores' first fragments arrive.
 constexpr int TB_TP = 32, TB_GRP = TB_TP * 128, TB_BUF = 9 * TB_GRP, TB_NB = 4;
-constexpr int TB_LDS = TB_NB * TB_BUF + 64;
+constexpr int TB_LDS = TB_NB * TB_BUF + 64 + TREE_MAX * 8;
 static_assert(TB_LDS <= 160 * 1024, "LDS");
 
-template <bool FULL, int NR>
+template <bool FAST, int NR>
 __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn16_kernel(const AttnArgs a)
 {
     constexpr bool ASM = NR == 2;
     constexpr int ROWS = 64 * NR, DT = TA_KL / 16, KS = TA_CW / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint8_t *s_ok = reinterpret_cast<uint8_t *>(smem + TB_NB * TB_BUF);   // [buffer][wave] a bit a row; [16 + wave]: not finite
+    uint64_t *s_anc = reinterpret_cast<uint64_t *>(smem + TB_NB * TB_BUF + 64);   // [node] its ancestors
 
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kq = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);   // the grid is a multiple of 8
-    Share sh;
-    if (!find_share(a, ROWS, TB_TP, id, sh)) return;
-    const int b = __builtin_amdgcn_readfirstlane(sh.b), rt = __builtin_amdgcn_readfirstlane(sh.rt);
-    const int splits = __builtin_amdgcn_readfirstlane(sh.splits), sp = __builtin_amdgcn_readfirstlane(sh.split);
-    const int cnt = tree_count(a.t, b), rows = cnt * a.H, r0 = rt * ROWS;
+    const int H = a.H, CW = FAST ? TA_CW : a.CW, KL = a.KL;
+    Slots sl;
+    int seq = 0, begin = 0;
+    if (!find_slot(a, ROWS, TB_TP, id, gridDim.x, sl, seq, begin)) return;
+    const int slot = id / sl.n, rt = id - slot * sl.n;
+    const int to = slot_start(sl, slot + 1);
+    int from = slot_start(sl, slot);
+    for (int b = seq; from < to; b++) {
+    const int cnt = tree_count(a.t, b), rows = cnt * H, r0 = rt * ROWS;
     const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
-    const int nstep = (end + TB_TP - 1) / TB_TP;
-    const int s0 = (int)((long)nstep * sp / splits), s1 = (int)((long)nstep * (sp + 1) / splits);
-    const int H = a.H, CW = FULL ? TA_CW : a.CW, KL = a.KL;
+    const int nstep = cnt ? (end + TB_TP - 1) / TB_TP : 0;
+    const int s0 = from - begin, s1 = min(nstep, to - begin);
+    const bool split = s0 > 0 || s1 < nstep;
+    begin += nstep;
+    from = min(begin, to);
+    if (s0 >= s1 || r0 >= rows) continue;
+    __syncthreads();   // the staged steps of the sequence before
 
-    int row[NR];
-    uint64_t anc[NR];
-    {
-        const uint64_t m = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            row[r] = r0 + 16 * (NR * wv + r) + c16;
-            const int n = row[r] < rows ? row[r] / H : 0;
-            anc[r] = ((uint64_t)__shfl((uint32_t)(m >> 32), n, 64) << 32) | __shfl((uint32_t)m, n, 64);
-        }
-    }
+    if (tid < 64) s_anc[lane] = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
+    // this lane's query rows: column c16 of each of the wave's NR row tiles
+    auto row_of = [&](int r) __attribute__((always_inline)) { return r0 + 16 * (NR * wv + r) + (opaque(tid) & 15); };
     bf16x8 qb[KS][NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const char *src = reinterpret_cast<const char *>(a.q) + ((size_t)b * a.t.N * H + (row[r] < rows ? row[r] : 0)) * CW * 2;
+        const int row = row_of(r);
+        const char *src = reinterpret_cast<const char *>(a.q) + ((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW * 2;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             const int u = 4 * ks + kq;
             uint4 v = {0, 0, 0, 0};
-            if (row[r] < rows && (FULL || u < CW / 8)) v = *reinterpret_cast<const uint4 *>(src + 16 * u);
+            if (row < rows && (FAST || u < CW / 8)) v = *reinterpret_cast<const uint4 *>(src + 16 * u);
             qb[ks][r] = __builtin_bit_cast(bf16x8, v);
         }
     }
 
     // staging: wave wv brings rows 8 wv .. + 7 of a step
     const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
-    int pgn = -1, pgo = 0;   // page and row in it of this lane's row of the step loaded next
-    auto find_rows = [&](int s) __attribute__((always_inline)) {   // no branch: it stands between products
-        const uint32_t pos = (uint32_t)(s * TB_TP + prow), at = pos / (uint32_t)a.c.page;
-        const bool in = (int)pos < end && (int)at < a.c.max_pages;
-        pgo = (int)(pos - at * (uint32_t)a.c.page);
-        const int n = a.c.table[(size_t)b * a.c.max_pages + (in ? at : 0u)];
+    // The page number `pgn` (-1: none) and row in it of the step loaded next; (ncol, nrow) the table column and
+    // row of the one after it, which end at (ecol, erow). A step is tcol columns, trow rows. FAST: of the
+    // wave's first row, its eight lie in one page; else of each lane's.
+    const int ecol = min(end / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? end - ecol * a.c.page : 0;
+    const int frow = s0 * TB_TP + (FAST ? 8 * wv : prow);
+    int pgn = -1, pgo = 0, ncol = frow / a.c.page, nrow = frow - ncol * a.c.page;
+    const int *table = a.c.table + (size_t)b * a.c.max_pages;
+    auto find_rows = [&]() __attribute__((always_inline)) {   // no branch: it stands between products
+        const bool in = (ncol < ecol) | ((ncol == ecol) & (nrow < erow));
+        int at = in ? ncol : 0;
+        if constexpr (FAST) asm volatile("" : "+v"(at));   // a vector load: a scalar one shares the counter of the LDS reads
+        const int n = table[at];
         pgn = in ? n : -1;
+        pgo = nrow;
+        nrow += a.trow;
+        ncol += a.tcol + (nrow >= a.c.page);
+        nrow -= nrow >= a.c.page ? a.c.page : 0;
     };
-    const char *ldp = nullptr;   // this lane's row of the step being loaded
-    auto load_row = [&](int buf, int page, int in) __attribute__((always_inline)) {
-        const bool ok = page >= 0 && page < a.c.n_pages;
-        const char *p = reinterpret_cast<const char *>(a.pages) + ((size_t)(ok ? page : 0) * a.c.page + in) * (CW * 2);
-        ldp = (ok ? p : reinterpret_cast<const char *>(ta_zeros)) + 16 * lu;
-        const uint32_t okb = gather_rows(__ballot(ok));
-        if (lane == 0) s_ok[4 * buf + wv] = (uint8_t)okb;
+    // Loads of a step into LDS. FAST: buffer loads from the page's start (of zeros, where there is none; rows
+    // behind the last node are zeroed where they are used). The others go by global loads, a lane's row where
+    // it is, which the compiler takes for LDS accesses too: it then waits for all LDS reads after each.
+    const int fast_off = lrow * (TA_CW * 2) + 16 * lu;
+    int ldo = 0, ldn = 0;
+    const char *ldp = nullptr;
+    auto load_row = [&](int buf) __attribute__((always_inline)) {
+        uint32_t okb;
+        if constexpr (FAST) {
+            const int page = __builtin_amdgcn_readfirstlane(pgn);
+            const bool ok = page >= 0 && page < a.c.n_pages;
+            const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)page * a.page_bytes;
+            ldp = ok ? p : reinterpret_cast<const char *>(ta_zeros);
+            ldn = ok ? (int)a.page_bytes : 8 * TA_CW * 2;
+            ldo = ok ? pgo * (TA_CW * 2) : 0;
+            okb = ok ? 0xff : 0;
+        } else {
+            const bool ok = pgn >= 0 && pgn < a.c.n_pages;
+            const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)pgn * a.page_bytes + (uint32_t)pgo * (uint32_t)(CW * 2);
+            ldp = (ok ? p : reinterpret_cast<const char *>(ta_zeros)) + 16 * lu;
+            okb = gather_rows(__ballot(ok));
+        }
+        s_ok[4 * buf + wv] = (uint8_t)okb;   // every lane the same
     };
     auto load_group = [&](lds_char *dst, int g) __attribute__((always_inline)) {
-        const char *src = ldp + 128 * g;
-        if (!FULL && 8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
-        __builtin_amdgcn_global_load_lds((glb_void *)src, (lds_void *)(dst + TB_GRP * g + 1024 * wv), 16, 0, 0);
+        lds_void *to = (lds_void *)(dst + TB_GRP * g + 1024 * wv);
+        if constexpr (FAST) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void *)ldp, (short)0, ldn, 0x00020000), to, 16, fast_off, ldo + 128 * g, 0, 0);
+        } else {
+            const char *src = ldp + 128 * g;
+            if (8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
+            __builtin_amdgcn_global_load_lds((glb_void *)src, to, 16, 0, 0);
+        }
     };
-    auto load_step = [&](lds_char *dst, int buf, int page, int in) __attribute__((always_inline)) {
-        load_row(buf, page, in);
+    auto load_step = [&](lds_char *dst, int buf) __attribute__((always_inline)) {
+        load_row(buf);
 #pragma unroll
         for (int g = 0; g < 9; g++) load_group(dst, g);
     };
@@ -726,21 +746,26 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     wait<ASM>();
     // LDS addresses in a block of 16 rows. Score product: row pi, units 4 (ks & 1) + kq of group ks / 2.
     // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4. Unit u
-    // of row r stands at u ^ ((r / 2) & 6)
+    // of row r stands at u ^ ((r / 2) & 6), so the other units are the first ones with a bit or two turned. The
+    // fragments go in an order that changes the unit seldom, and each address is worked out when it does.
     const int pi = 4 * (c16 & 3) + (c16 >> 2), vr = 4 * ((lane >> 2) & 3) + kq;
-    int ka[2], va[4];
-#pragma unroll
-    for (int i = 0; i < 2; i++) ka[i] = 128 * pi + 16 * ((4 * i + kq) ^ ((pi >> 1) & 6));
-#pragma unroll
-    for (int i = 0; i < 4; i++) va[i] = 128 * vr + 16 * ((2 * i + ((lane >> 1) & 1)) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
+    const int ka = 128 * pi + 16 * (kq ^ ((pi >> 1) & 6));
+    const int va = 128 * vr + 16 * (((lane >> 1) & 1) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
 
     // fragments read ahead, and score fragments of a step (fragment 2 ks + block)
     constexpr int AH = 8, NF = 2 * KS;
+    // fragment f of the scores: block f % 2 of K-step ks_of(f); of the sum: latent tile d_of(i)
+    auto ks_of = [](int f) { return f < KS ? 2 * (f >> 1) : 2 * ((f - KS) >> 1) + 1; };
+    auto d_of = [](int i) { return 4 * (i & 7) + (i >> 3); };
+    static_assert(KS % 2 == 0 && DT == 32, "fragment orders");
+    int kat = 0, vat = 0;
     auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {
-        return *(const __attribute__((address_space(3))) bf16x8 *)(buf + ka[(f >> 1) & 1] + TB_GRP * (f >> 2) + 2048 * (f & 1));
+        if (f == 0 || f == KS) kat = opaque(ka) ^ (f == KS ? 64 : 0);
+        return *(const __attribute__((address_space(3))) bf16x8 *)(buf + kat + TB_GRP * (ks_of(f) >> 1) + 2048 * (f & 1));
     };
-    auto vread = [&](lds_cchar *buf, int d) __attribute__((always_inline)) {
-        lds_cchar *at = buf + va[d & 3] + TB_GRP * (d >> 2);
+    auto vread = [&](lds_cchar *buf, int i) __attribute__((always_inline)) {
+        if (i % 8 == 0) vat = opaque(va) ^ (4 * i);
+        lds_cchar *at = buf + vat + TB_GRP * (d_of(i) >> 2);
         const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
         const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
         const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
@@ -754,7 +779,7 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         for (int f = 0; f < NF; f++) {
             const bf16x8 x = kf[f % AH];
 #pragma unroll
-            for (int r = 0; r < NR; r++) mfma_vec<ASM>(x, qb[f >> 1][r], S[f & 1][r], f < 2);
+            for (int r = 0; r < NR; r++) mfma_vec<ASM>(x, qb[ks_of(f)][r], S[f & 1][r], f < 2);
             if (f + AH < NF) kf[f % AH] = kread(buf, f + AH);
             else vf[f + AH - NF] = vread(sum, f + AH - NF);
             between(f);
@@ -768,7 +793,7 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         for (int d = 0; d < DT; d++) {
             const bf16x8 v = vf[d % AH];
 #pragma unroll
-            for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d][r]);
+            for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d_of(d)][r]);
             if (d + AH < DT) vf[d % AH] = vread(buf, d + AH);
             between(d);
             __builtin_amdgcn_sched_barrier(0);
@@ -828,8 +853,9 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    auto mask_pages = [&](int s, f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)]);
+    auto pages_of = [&](int s) __attribute__((always_inline)) { return reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)]; };
+    auto mask_pages = [&](uint32_t held, f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(held);
         if (ok == 0xffffffffu) return;
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -842,17 +868,17 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 
     // steps s0 .. s0 + 2 on their way, the page of s0 + 3 looked up
     const int sm = min(s1, max(s0, len / TB_TP));   // whole steps of committed positions end here
-    {
-        int pg[3], in[3];
+    find_rows();
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-            find_rows(s0 + i);
-            pg[i] = pgn;
-            in[i] = pgo;
-        }
-        find_rows(s0 + 3);
-#pragma unroll
-        for (int i = 0; i < 3; i++) load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i), pg[i], in[i]);
+    for (int i = 0; i < 3; i++) {
+        const int n = pgn, o = pgo;
+        find_rows();   // the next lookup before this step's loads, so that waiting for it waits for none of them
+        const int n1 = pgn, o1 = pgo;
+        pgn = n;
+        pgo = o;
+        load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i));
+        pgn = n1;
+        pgo = o1;
     }
     if (s0 < sm) {
         f32x4 S[2][NR];
@@ -865,7 +891,7 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
             for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
             scores(cur, cur, kf, vf, S, nothing);
             wait<ASM>();
-            mask_pages(s0, S);
+            mask_pages(pages_of(s0), S);
 #pragma unroll
             for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
             cur = lds + buf_of(s0 + 1) * TB_BUF;
@@ -877,16 +903,18 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         // has every transposed read wait for the loads in flight.
         auto step = [&](lds_cchar *__restrict__ cur, lds_cchar *__restrict__ nxt, lds_cchar *__restrict__ nx2,
                         lds_char *__restrict__ fill, int s) __attribute__((always_inline)) {
+            uint32_t held = 0;
             scores(nxt, cur, kf, vf, S, [&](int f) __attribute__((always_inline)) {
-                if (f == 2) load_row(buf_of(s + 3), pgn, pgo);
-                if (f == 4) find_rows(s + 4);
+                if (f == 6) held = pages_of(s + 1);
+                if (f == 2) load_row(buf_of(s + 3));
+                if (f == 4) find_rows();
                 if (f >= 8 && f < 26 && f % 2 == 0) load_group(fill, (f - 8) / 2);
             });
             bf16x8 pn[NR];
 #pragma unroll
-            for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
-            wait<ASM>();
-            mask_pages(s + 1, S);
+            for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);   // with its wait states, S is there
+            __builtin_amdgcn_sched_barrier(0);
+            mask_pages(held, S);
             values(cur, vf, pf, [&](int d) __attribute__((always_inline)) {
                 if (d < 28) soft_piece(d, S, x, pn);
                 if (d == 28) {
@@ -898,17 +926,17 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
                 if (d > 28) kf[d - 25] = kread(nx2, d - 25);
                 if (d == 31) kf[7] = kread(nx2, 7);
             });
-            wait<ASM>();   // also for what the compiler moves at the loop's end
             rescale(x);
 #pragma unroll
             for (int r = 0; r < NR; r++) pf[r] = pn[r];
         };
         for (int s = s0; s + 1 < sm; s++)
             step(lds + buf_of(s) * TB_BUF, lds + buf_of(s + 1) * TB_BUF, lds + buf_of(s + 2) * TB_BUF, lds + buf_of(s + 3) * TB_BUF, s);
+        wait<ASM>();
         {
             lds_cchar *cur = lds + buf_of(sm - 1) * TB_BUF;
             publish(0);
-            load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2), pgn, pgo);
+            load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2));
 #pragma unroll
             for (int d = 0; d < AH; d++) vf[d] = vread(cur, d);
 #pragma unroll
@@ -920,30 +948,30 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     // the steps that hold nodes: at most three, on their way by now
     for (int s = sm; s < s1; s++) {
         publish(0);
-        char *at = smem + buf_of(s) * TB_BUF + 1024 * wv + 16 * lane;
+        const int ln = opaque(tid) & 63, pr = 8 * wv + (ln >> 3), q4 = ln >> 4;
+        char *at = smem + buf_of(s) * TB_BUF + 1024 * wv + 16 * ln;
         lds_cchar *cur = lds + buf_of(s) * TB_BUF;
         const uint32_t ok = reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)];
         const int n0 = len - s * TB_TP;   // place of the first node in the step
-        uint32_t bad = 0;
+        // Zeros in the rows behind the last node, and in rows of nodes that hold an infinity or a NaN, which are
+        // noted, so that the query rows that see them become NaN and no others
+        bool inf = false;
         if (cnt > 1) {
-            // rows of nodes that hold an infinity or a NaN: zeros, and noted, so that the query rows that see
-            // them become NaN and no others
-            bool inf = false;
 #pragma unroll
             for (int g = 0; g < 9; g++) {
                 const uint4 w = *reinterpret_cast<const uint4 *>(at + TB_GRP * g);
                 inf = inf || not_finite16(w.x) || not_finite16(w.y) || not_finite16(w.z) || not_finite16(w.w);
             }
-            const uint64_t m = __ballot(inf && prow >= n0);
-            const bool mine = (m >> (lane & 56) & 0xff) != 0;
-            if (mine)
-#pragma unroll
-                for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + TB_GRP * g) = uint4{0, 0, 0, 0};
-            const uint32_t bits = gather_rows(__ballot(mine));
-            if (lane == 0) s_ok[16 + wv] = (uint8_t)bits;
-            __syncthreads();
-            bad = reinterpret_cast<const uint32_t *>(s_ok)[4];
         }
+        const bool behind = s * TB_TP + pr >= end;
+        const uint64_t m = __ballot(inf && pr >= n0);
+        const bool mine = (m >> (ln & 56) & 0xff) != 0 && !behind;
+        if (mine || behind)
+#pragma unroll
+            for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + TB_GRP * g) = uint4{0, 0, 0, 0};
+        s_ok[16 + wv] = (uint8_t)gather_rows(__ballot(mine));
+        __syncthreads();
+        const uint32_t bad = reinterpret_cast<const uint32_t *>(s_ok)[4];
         f32x4 S[2][NR];
         bf16x8 kf[AH], vf[AH], pf[NR];
         Soft x;
@@ -953,15 +981,17 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         wait<ASM>();
 #pragma unroll
         for (int r = 0; r < NR; r++) {
+            const int row = row_of(r);
+            const uint64_t anc = s_anc[row < rows ? row / H : 0];
             uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
-            if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc[r] << n0);
-            else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc[r] >> -n0);
+            if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc << n0);
+            else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc >> -n0);
             w &= ok;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int bit = 16 * i + 4 * e + kq;
+                    const int bit = 16 * i + 4 * e + q4;
                     const float seen = bad >> bit & 1 ? NAN : 0.0f;
                     S[i][r][e] = w >> bit & 1 ? S[i][r][e] + seen : -INFINITY;
                 }
@@ -975,37 +1005,39 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         wait<ASM>();
     }
 
-    const bool split = splits > 1;
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        if (row[r] >= rows) continue;
+        const int row = row_of(r);
+        if (row >= rows) continue;
         const float l = lacc[r][0];
-        const size_t orow = (size_t)b * a.t.N * H + row[r], prow = (size_t)id * ROWS + (row[r] - r0);
+        const int q4 = (opaque(tid) & 63) >> 4;
+        const size_t orow = (size_t)b * a.t.N * H + row, prow = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
         if (split) {
-            if (kq == 0) {
+            if (q4 == 0) {
                 a.pm[prow] = M[r];
                 a.pl[prow] = l;
             }
             if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
-            float *dst = a.po + prow * KL + 4 * kq;
+            float *dst = a.po + prow * KL + 4 * q4;
 #pragma unroll
             for (int d = 0; d < DT; d++)
-                if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r];
+                if (16 * d + 4 * q4 < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r];
         } else {
-            if (kq == 0 && a.lse) a.lse[orow] = l == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(l)) * TA_LN2;
+            if (q4 == 0 && a.lse) a.lse[orow] = l == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(l)) * TA_LN2;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             if (a.o_dt == K3HIP_F32) {
-                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * kq;
+                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * q4;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r] * inv;
+                    if (16 * d + 4 * q4 < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r] * inv;
             } else {
-                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * kq;
+                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * q4;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + 4 * kq < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d][r] * inv);
+                    if (16 * d + 4 * q4 < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d][r] * inv);
             }
         }
+    }
     }
 }
 
@@ -1016,28 +1048,30 @@ __global__ __launch_bounds__(TA_NT) void tree_attn_merge_kernel(const AttnArgs a
     const int b = blockIdx.y, lane = threadIdx.x & 63, row = blockIdx.x * (TA_NT / 64) + (threadIdx.x >> 6);
     const int rows = tree_count(a.t, b) * a.H;
     if (row >= rows) return;
-    const int rt = row / tile_rows;
-    int first = (b * a.nrt + rt) * a.nsplit, n = a.nsplit, step = 1;
+    const int rt = row / tile_rows, in = row % tile_rows;
+    int n = a.nsplit;
+    int4 p = {0, 0, 0, 0};
     if (a.plan) {
-        const int2 p = a.plan[b];
-        n = p.y;
+        p = a.plan[b];
+        n = p.y - p.x + 1;
         if (n <= 1) return;   // written by its only workgroup
-        first = p.x + rt;
-        step = (rows + tile_rows - 1) / tile_rows;
     }
-    const size_t p0 = (size_t)first * tile_rows + row % tile_rows, pd = (size_t)step * tile_rows;
+    // part s: fp32 in order; bf16 the first slot's second part, then the others' first
+    auto at = [&](int s) -> size_t {
+        return (a.plan ? 2 * ((size_t)(p.x + s) * p.z + rt) + (s == 0) : ((size_t)b * a.nrt + rt) * n + s) * tile_rows + in;
+    };
     float M = -INFINITY, l = 0.0f;
-    for (int s = 0; s < n; s++) M = fmaxf(M, a.pm[p0 + s * pd]);
+    for (int s = 0; s < n; s++) M = fmaxf(M, a.pm[at(s)]);
     for (int c0 = 0; c0 < a.KL; c0 += 256) {
         const int c = c0 + 4 * lane;
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         l = 0.0f;
         for (int s = 0; s < n; s++) {
-            const float m = a.pm[p0 + s * pd];
+            const float m = a.pm[at(s)];
             if (m == -INFINITY) continue;
             const float w = __builtin_amdgcn_exp2f(m - M);
-            l += w * a.pl[p0 + s * pd];
-            if (c < a.KL) v += w * *reinterpret_cast<const f32x4 *>(a.po + (p0 + s * pd) * a.KL + c);
+            l += w * a.pl[at(s)];
+            if (c < a.KL) v += w * *reinterpret_cast<const f32x4 *>(a.po + at(s) * a.KL + c);
         }
         if (c < a.KL) {
             const size_t at = ((size_t)b * a.t.N * a.H + row) * a.KL + c;
@@ -1065,21 +1099,32 @@ int ta_split(int B, int nrt, int tiles)
     return (int)std::max(1L, std::min({(long)tiles, ncu / wg, 64L}));
 }
 
-// bf16: a range a CU, two where the row tiles alone are more.
-int ta_room(int B, int nrt)
+// bf16: the workgroups of a launch, the least multiple of the CUs whose slots of n leave no more than a
+// tenth of them without work.
+long ta_grid(int n)
 {
     int ncu = 256;
     (void)cu_count(ncu);
-    return (long)B * nrt <= ncu ? ncu : 2 * ncu;
+    long best = 0;
+    double most = 0.0;
+    for (long k = (n + ncu - 1) / ncu, k0 = k; k < k0 + 4; k++) {
+        const double used = (double)(ncu * k / n * n) / (double)(ncu * k);
+        if (used > most + 0.01) {
+            most = used;
+            best = ncu * k;
+        }
+        if (used >= 0.9) break;
+    }
+    return (best + 7) & ~7L;   // a multiple of the XCDs
 }
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Partials of `ranges` ranges of `rows` rows, and the plan of B sequences.
-size_t ta_ws_bytes(long ranges, int rows, int KL, int B)
+// `parts` partial sums of `rows` rows, and the plan of B sequences.
+size_t ta_ws_bytes(long parts, int rows, int KL, int B)
 {
-    const size_t r = (size_t)ranges * rows;
-    return up256(r * KL * 4) + 2 * up256(r * 4) + up256((size_t)B * sizeof(int2));
+    const size_t r = (size_t)parts * rows;
+    return up256(r * KL * 4) + 2 * up256(r * 4) + up256((size_t)B * sizeof(int4));
 }
 
 }  // namespace
@@ -1094,7 +1139,7 @@ extern "C" size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora)
     const int r4 = ta_rows(true, (long)N * H), n4 = (int)(((long)N * H + r4 - 1) / r4);
     const int r2 = ta_rows(false, (long)N * H), n2 = (int)(((long)N * H + r2 - 1) / r2);
     return std::max(ta_ws_bytes((long)B * n4 * ta_split(B, n4, 1 << 20), r4, kv_lora, B),
-                    ta_ws_bytes(ta_room(B, n2), r2, kv_lora, B));
+                    ta_ws_bytes(2 * ta_grid(n2), r2, kv_lora, B));
 }
 
 extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int rope, float scale, const void *q,
@@ -1114,6 +1159,9 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
         K3_FAIL(K3HIP_EUNSUPPORTED, "%s: kv_lora=%d rope=%d (multiples of 8, at most %d and %d together)", who, kv_lora,
                 rope, TA_KL, TA_CW);
     if (!(scale > 0.0f)) K3_FAIL(K3HIP_EINVAL, "%s: scale=%g (positive)", who, scale);
+    if (B * (((long)max_pages * page + N) / 32 + 1) > 0x7fffffffL)
+        K3_FAIL(K3HIP_EINVAL, "%s: %d sequences of up to %ld positions", who, B, (long)max_pages * page);
+    if ((long)page * CW * 4 > 0x7fffffffL) K3_FAIL(K3HIP_EINVAL, "%s: pages of %d rows", who, page);
     if (B > 65535 || (long)N * H > 65535L * 16) K3_FAIL(K3HIP_EINVAL, "%s: B=%d N=%d H=%d", who, B, N, H);
     if (B == 0 || N == 0) return K3HIP_OK;
     if (!q || !o) K3_FAIL(K3HIP_EINVAL, "%s: NULL q or o", who);
@@ -1131,32 +1179,34 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     a.nrt = (int)(((long)N * H + rows - 1) / rows);
     a.B = B;
     const long tp = f32 ? 32 : TB_TP, tiles = ((long)max_pages * page + N + tp - 1) / tp;
-    long ranges;
+    long parts, grid16 = 0;
     bool split;
     if (f32) {
         a.nsplit = ta_split(B, a.nrt, (int)tiles);
-        ranges = (long)B * a.nrt * a.nsplit;
+        parts = (long)B * a.nrt * a.nsplit;
         split = a.nsplit > 1;
     } else {
-        a.room = ta_room(B, a.nrt);
-        ranges = a.room;
-        split = tiles > 1 && (long)B * a.nrt < a.room;
-        if (!split) a.room = 0;
+        grid16 = ta_grid(a.nrt);
+        parts = 2 * grid16;
+        split = true;
+        a.tcol = TB_TP / page;
+        a.trow = TB_TP % page;
+        a.page_bytes = (uint32_t)page * (uint32_t)CW * 2;
     }
     StreamBuf buf;
     if (split) {
-        const size_t need = ta_ws_bytes(ranges, rows, kv_lora, B);
+        const size_t need = ta_ws_bytes(parts, rows, kv_lora, B);
         if (!workspace) {
             if (int rc = stream_alloc(buf, need, st)) return rc;
             workspace = buf.p;
         } else if (workspace_bytes < need || ((uintptr_t)workspace & 15)) {
             K3_FAIL(K3HIP_EINVAL, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
         }
-        const size_t r = (size_t)ranges * rows;
+        const size_t r = (size_t)parts * rows;
         a.po = (float *)workspace;
         a.pm = (float *)((char *)workspace + up256(r * kv_lora * 4));
         a.pl = (float *)((char *)a.pm + up256(r * 4));
-        if (!f32) a.plan = (int2 *)((char *)a.pl + up256(r * 4));
+        if (!f32) a.plan = (int4 *)((char *)a.pl + up256(r * 4));
     }
     const void *kern;
     dim3 grid;
@@ -1167,9 +1217,10 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
         grid = dim3(a.nsplit, a.nrt, B);
         lds = TA_LDS;
     } else {
-        kern = CW == TA_CW ? (rows == 64 ? (const void *)tree_attn16_kernel<true, 1> : (const void *)tree_attn16_kernel<true, 2>)
-                           : (rows == 64 ? (const void *)tree_attn16_kernel<false, 1> : (const void *)tree_attn16_kernel<false, 2>);
-        grid = dim3((unsigned)((std::max((long)a.room, (long)B * a.nrt) + 7) & ~7L));   // a multiple of the XCDs
+        // whole rows of eight in one page go by buffer loads
+        kern = CW == TA_CW && page % 8 == 0 ? (rows == 64 ? (const void *)tree_attn16_kernel<true, 1> : (const void *)tree_attn16_kernel<true, 2>)
+                                            : (rows == 64 ? (const void *)tree_attn16_kernel<false, 1> : (const void *)tree_attn16_kernel<false, 2>);
+        grid = dim3((unsigned)grid16);
         lds = TB_LDS;
     }
     K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
