@@ -51,8 +51,6 @@ typedef __attribute__((address_space(3))) const char lds_cchar;
 
 constexpr int TA_NT = 256;
 constexpr int TA_KL = 512, TA_CW = 576;        // widest latent and cache row
-constexpr int TA_TILE = 64 * TA_CW * 2;        // bytes a staged tile: 64 bf16 or 32 fp32 rows
-constexpr int TA_LDS = 2 * TA_TILE + 64;       // two tiles, their rows' validity bits
 constexpr float TA_LOG2E = 1.4426950408889634f, TA_LN2 = 0.6931471805599453f;
 constexpr float TA_LAZY = 8.0f;                // log2 of the largest weight before a rescale
 
@@ -68,371 +66,12 @@ struct AttnArgs {
     int o_dt;
     float *lse;
     float scale2;     // scale log2(e)
-    int nsplit, nrt;  // fp32: position ranges a sequence, row tiles a sequence
-    float *po, *pm, *pl;   // partials of each range [rows of a tile] ( x KL)
     int B;
     uint32_t page_bytes;
-    int tcol, trow;   // bf16: a step in table columns and rows
-    int4 *plan;       // bf16: [B] first and last slot, workgroups a slot
+    int tcol, trow;        // a step in table columns and rows
+    float *po, *pm, *pl;   // parts, two a workgroup [rows of a tile] ( x KL): their sums, M and l
+    int4 *plan;            // [B] first and last slot, workgroups a slot
 };
-
-template <bool F32, int NR, int RG, int PG>
-__global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn_kernel(const AttnArgs a)
-{
-    constexpr int ROWS = 16 * NR * RG;
-    constexpr int ROWB = TA_CW * (F32 ? 4 : 2), UNITS = ROWB / 16;   // a staged row, its 16-byte units
-    constexpr int TP = TA_TILE / ROWB, NB = TP / 16;                 // positions and 16-row blocks a tile
-    constexpr int PB = NB / PG;                                      // blocks a wave
-    constexpr int NP = F32 ? PB : (PB + 1) / 2;                      // K = 16 (fp32) or 32 (bf16) groups of the second product
-    constexpr int DT = TA_KL / 16;                                   // latent tiles
-    constexpr int KS = F32 ? TA_CW / 16 : TA_CW / 32;                // K-steps of a 16-byte unit a lane
-    static_assert(PB * PG == NB, "position groups");
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    uint16_t *s_ok = reinterpret_cast<uint16_t *>(smem + 2 * TA_TILE);   // [2][NB] a bit a row
-
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c16 = lane & 15, kq = lane >> 4;
-    const int sp = blockIdx.x, rt = blockIdx.y, b = blockIdx.z;
-    const int rg = wv % RG, pg = wv / RG;
-    const bool works = pg < PG;                       // waves past the groups only stage
-    const int cnt = tree_count(a.t, b), rows = cnt * a.H, r0 = rt * ROWS;
-    if (r0 >= rows) return;
-    const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
-    const int ntile = (end + TP - 1) / TP;
-    const int t0 = (int)((long)ntile * sp / a.nsplit), t1 = (int)((long)ntile * (sp + 1) / a.nsplit);
-    const int H = a.H, CW = a.CW, KL = a.KL;
-    const size_t part = ((size_t)b * a.nrt + rt) * a.nsplit + sp;
-
-    // this lane's query rows: column c16 of each of the wave's NR row tiles
-    int row[NR];
-    uint64_t anc[NR];
-    {
-        const uint64_t m = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            row[r] = r0 + 16 * (NR * rg + r) + c16;
-            const int n = row[r] < rows ? row[r] / H : 0;
-            anc[r] = ((uint64_t)__shfl((uint32_t)(m >> 32), n, 64) << 32) | __shfl((uint32_t)m, n, 64);
-        }
-    }
-    // B fragments of the score product: 16-byte unit 4 ks + kq of the row
-    bf16x8 qb[F32 ? 1 : KS][NR];
-    f32x4 qf[F32 ? KS : 1][NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const char *src = reinterpret_cast<const char *>(a.q) + ((size_t)b * a.t.N * H + (row[r] < rows ? row[r] : 0)) * CW * (F32 ? 4 : 2);
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int u = 4 * ks + kq;
-            uint4 v = {0, 0, 0, 0};
-            if (works && row[r] < rows && u < CW / (F32 ? 4 : 8)) v = *reinterpret_cast<const uint4 *>(src + 16 * u);
-            if constexpr (F32) qf[ks][r] = __builtin_bit_cast(f32x4, v);
-            else qb[ks][r] = __builtin_bit_cast(bf16x8, v);
-        }
-    }
-
-    // staging: NB / 4 (at least one) blocks of 16 rows a wave; fp32 tiles have two blocks of twice the units
-    auto load_tile = [&](int t) {
-        const int buf = t & 1;
-        constexpr int RW = TP / 4;   // rows a wave: 16 (bf16) or 8 (fp32)
-        const int pos = t * TP + RW * wv + (lane % RW);
-        const long at = pos < end ? paged_row(a.c, b, pos) : -1;
-        const char *p = at >= 0 ? reinterpret_cast<const char *>(a.pages) + (size_t)at * CW * (F32 ? 4 : 2)
-                                : reinterpret_cast<const char *>(ta_zeros);
-        const uint64_t okb = __ballot(at >= 0);
-        if (lane == 0) {
-            if constexpr (F32) reinterpret_cast<uint8_t *>(s_ok)[8 * buf + wv] = (uint8_t)okb;
-            else s_ok[4 * buf + wv] = (uint16_t)okb;
-        }
-        const uint32_t plo = (uint32_t)(uintptr_t)p, phi = (uint32_t)((uintptr_t)p >> 32);
-        char *dst = smem + buf * TA_TILE + RW * wv * ROWB;
-        const int units = CW / (F32 ? 4 : 8);
-#pragma unroll
-        for (int i = 0; i < RW * UNITS / 64; i++) {
-            const int L = 64 * i + lane, r = L / UNITS, rr = RW * wv + r;
-            const int u = (L % UNITS) ^ (F32 ? rr & 15 : (rr >> 1) & 7);
-            const char *g = reinterpret_cast<const char *>(((uintptr_t)(uint32_t)__shfl(phi, r, 64) << 32) | (uint32_t)__shfl(plo, r, 64));
-            g = u < units ? g + 16 * u : reinterpret_cast<const char *>(ta_zeros);
-            __builtin_amdgcn_global_load_lds((glb_void *)g, (lds_void *)(dst + 1024 * i), 16, 0, 0);
-        }
-    };
-
-    f32x4 acc[DT][NR];
-    float M[NR], lsum[NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        M[r] = -INFINITY;
-        lsum[r] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; d++) acc[d][r] = 0.0f;
-    }
-    const int pi = 4 * (c16 & 3) + (c16 >> 2);   // LDS row of score row c16 in its block
-
-    if (t0 < t1) load_tile(t0);
-    for (int t = t0; t < t1; t++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (t + 1 < t1) load_tile(t + 1);
-        if (!works) continue;
-        const char *tile = smem + (t & 1) * TA_TILE + 16 * PB * pg * ROWB;   // this wave's blocks
-
-        f32x4 S[PB][NR];
-#pragma unroll
-        for (int i = 0; i < PB; i++)
-#pragma unroll
-            for (int r = 0; r < NR; r++) S[i][r] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int u = (4 * ks + kq) ^ (F32 ? pi & 15 : (pi >> 1) & 7);
-#pragma unroll
-            for (int i = 0; i < PB; i++) {
-                const char *at = tile + (16 * i + pi) * ROWB + 16 * u;
-                if constexpr (F32) {
-                    const f32x4 kf = *reinterpret_cast<const f32x4 *>(at);
-#pragma unroll
-                    for (int r = 0; r < NR; r++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            S[i][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[ks][r][j], S[i][r], 0, 0, 0);
-                } else {
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(at);
-#pragma unroll
-                    for (int r = 0; r < NR; r++) S[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qb[ks][r], S[i][r], 0, 0, 0);
-                }
-            }
-        }
-
-        // masks: bit p of a row's word is position t TP + p; this lane's element e of block i is
-        // position 16 i + 4 e + kq of the wave's blocks
-        const int p0 = t * TP;
-        uint64_t ok = F32 ? (uint64_t) reinterpret_cast<const uint32_t *>(s_ok)[2 * (t & 1)]
-                          : reinterpret_cast<const uint64_t *>(s_ok)[t & 1];
-        const uint64_t full = F32 ? 0xffffffffull : ~0ull;
-        const bool masked = ok != full || p0 + TP > len;   // uniform
-        uint64_t see[NR];
-        bool bad = false;
-        if (masked) {
-            const int s = len - p0;   // tile position of the first node
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                uint64_t w = s >= 64 ? ~0ull : s <= 0 ? 0ull : (1ull << s) - 1;
-                if (s >= 0 && s < 64) w |= anc[r] << s;
-                else if (s < 0 && s > -64) w |= anc[r] >> -s;
-                see[r] = (w & ok) >> (16 * PB * pg);
-#pragma unroll
-                for (int i = 0; i < PB; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (!(see[r] >> (16 * i + 4 * e + kq) & 1)) {
-                            bad = bad || !(fabsf(S[i][r][e]) < INFINITY);
-                            S[i][r][e] = -INFINITY;
-                        }
-            }
-        }
-
-        // online softmax, a row per lane column; p takes the place of S
-        float al[NR];
-        bool moved = false;
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-            float mt = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < PB; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mt = fmaxf(mt, S[i][r][e]);
-            mt *= a.scale2;
-            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const bool up = mt > M[r] + TA_LAZY;
-            const float mn = up ? mt : M[r];
-            al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
-            moved = moved || up;
-            M[r] = mn;
-            const float ref = mn == -INFINITY ? 0.0f : mn;
-            float l = 0.0f;
-#pragma unroll
-            for (int i = 0; i < PB; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[i][r][e], a.scale2, -ref));
-                    S[i][r][e] = p;
-                    l += p;
-                }
-            lsum[r] = lsum[r] * al[r] + l;
-        }
-        if (__ballot(moved)) {
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int r = 0; r < NR; r++) acc[d][r] *= al[r];
-        }
-
-        if (masked && __ballot(bad)) {
-            // position by position on the vector unit, only into the rows that see it
-            for (int x = 0; x < 16 * PB; x++) {
-                float p[NR];
-                bool sees[NR], any = false;
-#pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    p[r] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < PB; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if ((x >> 2) == 4 * i + e) p[r] = S[i][r][e];
-                    p[r] = __shfl(p[r], c16 + 16 * (x & 3), 64);
-                    sees[r] = see[r] >> x & 1;
-                    any = any || sees[r];
-                }
-                if (!__ballot(any)) continue;
-                const char *vrow = tile + x * ROWB;
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    float v[4];
-                    if constexpr (F32) {   // acc[4 D + j][e]: channel 64 D + 16 kq + 4 e + j
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            v[e] = *reinterpret_cast<const float *>(vrow + 16 * ((16 * (d >> 2) + 4 * kq + e) ^ (x & 15)) + 4 * (d & 3));
-                    } else {               // acc[d][e]: channel 16 d + 4 kq + e
-                        const uint2 w = *reinterpret_cast<const uint2 *>(vrow + 16 * ((2 * d + (kq >> 1)) ^ ((x >> 1) & 7)) + 8 * (kq & 1));
-                        v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
-                        v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
-                    }
-#pragma unroll
-                    for (int r = 0; r < NR; r++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            acc[d][r][e] = sees[r] ? __builtin_fmaf(p[r], v[e], acc[d][r][e]) : acc[d][r][e];
-                }
-            }
-            continue;
-        }
-#pragma unroll
-        for (int g = 0; g < NP; g++) {
-            if constexpr (F32) {
-                // K = 4 products on rows 16 g + 4 e + kq; a lane's 16 bytes are its column of four tiles:
-                // tile 4 D + j holds channels 64 D + 4 m + j
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int rr = 4 * e + kq;
-#pragma unroll
-                    for (int D = 0; D < DT / 4; D++) {
-                        const f32x4 v = *reinterpret_cast<const f32x4 *>(tile + (16 * g + rr) * ROWB + 16 * ((16 * D + c16) ^ rr));
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-#pragma unroll
-                            for (int r = 0; r < NR; r++)
-                                acc[4 * D + j][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], S[g][r][e], acc[4 * D + j][r], 0, 0, 0);
-                    }
-                }
-            } else {
-                constexpr bool HALF = PB == 1;   // a single block: the other half of K is zero
-                bf16x8 pf[NR];
-#pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    bf16x2 w[4];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const f32x4 x = j == 0 || !HALF ? S[HALF ? 0 : 2 * g + j][r] : f32x4(0.0f);
-                        w[2 * j] = __builtin_convertvector(f2{x[0], x[1]}, bf16x2);
-                        w[2 * j + 1] = __builtin_convertvector(f2{x[2], x[3]}, bf16x2);
-                    }
-                    pf[r] = bf16x8{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
-                }
-                const int rr = 4 * ((lane >> 2) & 3) + kq;   // row of the block this lane's address names
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const int u = (2 * d + ((lane >> 1) & 1)) ^ ((rr >> 1) & 7);
-                    const char *at = tile + (32 * g + rr) * ROWB + 16 * u + 8 * (lane & 1);
-                    const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
-                    s16x4 x1 = {0, 0, 0, 0};
-                    if constexpr (!HALF) x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 16 * ROWB));
-                    const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
-                    const bf16x8 vf = __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
-#pragma unroll
-                    for (int r = 0; r < NR; r++) acc[d][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[r], acc[d][r], 0, 0, 0);
-                }
-            }
-        }
-    }
-
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        lsum[r] += __shfl_xor(lsum[r], 16, 64);
-        lsum[r] += __shfl_xor(lsum[r], 32, 64);
-    }
-    if constexpr (PG > 1) {
-        // position groups 1 .. PG - 1 hand their sums to group 0, 16 bytes a lane and tile
-        f32x4 *xo = reinterpret_cast<f32x4 *>(smem);
-        float *xm = reinterpret_cast<float *>(smem + (PG - 1) * RG * NR * DT * 64 * 16);
-        static_assert((PG - 1) * RG * NR * (DT * 64 * 16 + 512) <= 2 * TA_TILE, "exchange fits the tiles");
-        __syncthreads();
-        if (works && pg > 0) {
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const int at = (((pg - 1) * RG + rg) * NR + r) * 64 + lane;
-                xm[2 * at] = M[r];
-                xm[2 * at + 1] = lsum[r];
-#pragma unroll
-                for (int d = 0; d < DT; d++) xo[(size_t)(((pg - 1) * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] = acc[d][r];
-            }
-        }
-        __syncthreads();
-        if (!works || pg > 0) return;
-#pragma unroll
-        for (int r = 0; r < NR; r++)
-#pragma unroll
-            for (int g = 0; g < PG - 1; g++) {
-                const int at = ((g * RG + rg) * NR + r) * 64 + lane;
-                const float m2 = xm[2 * at], l2 = xm[2 * at + 1], mm = fmaxf(M[r], m2);
-                const float w1 = M[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[r] - mm);
-                const float w2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mm);
-                lsum[r] = lsum[r] * w1 + l2 * w2;
-                M[r] = mm;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-                    acc[d][r] = acc[d][r] * w1 + xo[(size_t)((g * RG + rg) * NR + r) * DT * 64 + d * 64 + lane] * w2;
-            }
-    }
-    if (!works) return;
-
-    // results: o, or this range's sums
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        if (row[r] >= rows) continue;
-        const bool split = a.nsplit > 1;
-        const size_t orow = (size_t)b * a.t.N * H + row[r];
-        const size_t prow = part * ROWS + (row[r] - r0);
-        if (split) {
-            if (kq == 0) {
-                a.pm[prow] = M[r];
-                a.pl[prow] = lsum[r];
-            }
-            if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
-        } else if (kq == 0 && a.lse) {
-            a.lse[orow] = lsum[r] == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(lsum[r])) * TA_LN2;
-        }
-        const float inv = split ? 1.0f : lsum[r] == 0.0f ? 0.0f : 1.0f / lsum[r];
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            f32x4 v;
-            int ch;
-            if constexpr (F32) {   // element d % 4 of group d / 4: channels ch .. ch + 3 from the four tiles
-                ch = 64 * (d >> 2) + 16 * kq + 4 * (d & 3);
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[j] = acc[4 * (d >> 2) + j][r][d & 3] * inv;
-            } else {
-                ch = 16 * d + 4 * kq;
-                v = acc[d][r] * inv;
-            }
-            if (ch >= KL) continue;
-            if (split) *reinterpret_cast<f32x4 *>(a.po + prow * KL + ch) = v;
-            else if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * KL + ch) = v;
-            else
-                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * KL + ch) =
-                    uint2{(uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16), (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16)};
-        }
-    }
-}
 
 // The 16x16x32 MFMAs of the bf16 kernel. With 32 query rows a wave the second product's 256 accumulators fill
 // the accumulation registers: with the builtin the compiler moves them between the register files and
@@ -1041,65 +680,424 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     }
 }
 
-// The ranges of a row merged in order, a wave per row: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s.
-// A range that saw nothing (M_s = -inf) left no sums.
-__global__ __launch_bounds__(TA_NT) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows)
+// fp32 caches. The products run on the fp16 matrix cores at fp32's accuracy: a row is scaled by a power of
+// two that puts its largest value just under 2^15 and split into fp16 hi + lo, 22 bits together (what
+// falls under fp16's smallest step is under 2^-39 of the row's largest value), and hi hi + hi lo + lo hi are summed in
+// fp32, three matrix instructions where six are needed on bf16 parts and sixteen times the rate of the fp32
+// instruction. A cache row's scale 2^k goes with its weight: the reference that weights are taken
+// against is the largest of (score - k), so the scaled weight 2^(score - k - M) is at most 2^TS_UP ahead of its own
+// split, whatever the rows' sizes, and the sum of the weights takes the 2^k back out.
+//
+// A step is 32 positions, staged as two planes of column groups as in the bf16 kernel, two buffers. A wave
+// brings 8 rows of a step into registers while the step before it is converted and written to LDS between
+// the score products of the step before that. Four waves of 16 query rows.
+constexpr int TS_BUF = 2 * TB_BUF;
+constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 4 + 64 + TREE_MAX * 8;
+constexpr float TS_UP = 7.0f;     // log2 of the weight of the reference
+static_assert(TS_LDS <= 160 * 1024, "LDS");
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void split16(const float (&x)[8], f16x8 &hi, f16x8 &lo)
 {
-    const int b = blockIdx.y, lane = threadIdx.x & 63, row = blockIdx.x * (TA_NT / 64) + (threadIdx.x >> 6);
-    const int rows = tree_count(a.t, b) * a.H;
-    if (row >= rows) return;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const f16x2 h = __builtin_convertvector(f2{x[e], x[e + 1]}, f16x2);
+        const f16x2 l = __builtin_convertvector(f2{x[e] - (float)h[0], x[e + 1] - (float)h[1]}, f16x2);
+        hi[e] = h[0];
+        hi[e + 1] = h[1];
+        lo[e] = l[0];
+        lo[e + 1] = l[1];
+    }
+}
+
+// The power of two that a row whose largest magnitude has these bits is scaled by.
+__device__ __forceinline__ int row_scale(uint32_t most)
+{
+    return most == 0 ? 0 : min(14 - ((int)(most >> 23) - 127), 126);
+}
+
+template <bool FULL>
+__global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn32_kernel(const AttnArgs a)
+{
+    constexpr int ROWS = 64, DT = TA_KL / 16, KS = TA_CW / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *s_k = reinterpret_cast<int *>(smem + 2 * TS_BUF);               // [buffer][row] its scale
+    uint8_t *s_ok = reinterpret_cast<uint8_t *>(s_k + 64);               // [buffer][seen, not finite][wave] a bit a row
+    uint64_t *s_anc = reinterpret_cast<uint64_t *>(s_ok + 64);           // [node] its ancestors
+
+    const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kq = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    const int H = a.H, CW = FULL ? TA_CW : a.CW, KL = a.KL;
+    Slots sl;
+    int seq = 0, begin = 0;
+    if (!find_slot(a, ROWS, TB_TP, id, gridDim.x, sl, seq, begin)) return;
+    const int slot = id / sl.n, rt = id - slot * sl.n;
+    const int to = slot_start(sl, slot + 1);
+    int from = slot_start(sl, slot);
+    for (int b = seq; from < to; b++) {
+        const int cnt = tree_count(a.t, b), rows = cnt * H, r0 = rt * ROWS;
+        const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
+        const int nstep = cnt ? (end + TB_TP - 1) / TB_TP : 0;
+        const int s0 = from - begin, s1 = min(nstep, to - begin);
+        const bool split = s0 > 0 || s1 < nstep;
+        begin += nstep;
+        from = min(begin, to);
+        if (s0 >= s1 || r0 >= rows) continue;
+        __syncthreads();   // the staged steps of the sequence before
+
+        if (tid < 64) s_anc[lane] = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
+        const int row = r0 + 16 * wv + c16;   // this lane's query row
+
+        // staging: rows 8 wv .. + 7 of a step, units lane & 7 of eight channels of each column group
+        const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
+        const int ecol = min(end / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? end - ecol * a.c.page : 0;
+        int ncol = (s0 * TB_TP + prow) / a.c.page, nrow = s0 * TB_TP + prow - ncol * a.c.page, pgn = -1, pgo = 0;
+        const int *table = a.c.table + (size_t)b * a.c.max_pages;
+        auto find_rows = [&]() __attribute__((always_inline)) {
+            const bool in = (ncol < ecol) | ((ncol == ecol) & (nrow < erow));
+            const int n = table[in ? ncol : 0];
+            pgn = in ? n : -1;
+            pgo = nrow;
+            nrow += a.trow;
+            ncol += a.tcol + (nrow >= a.c.page);
+            nrow -= nrow >= a.c.page ? a.c.page : 0;
+        };
+        f4 R[18];          // the row's values in flight
+        bool rok = false;  // it has a page
+        auto load_rows = [&]() __attribute__((always_inline)) {
+            rok = pgn >= 0 && pgn < a.c.n_pages;
+            const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)pgn * a.page_bytes + (uint32_t)pgo * (uint32_t)(CW * 4);
+            p = rok ? p : reinterpret_cast<const char *>(ta_zeros);
+#pragma unroll
+            for (int i = 0; i < 9; i++) {
+                const char *src = p + 32 * (8 * i + (lane & 7));
+                if (!FULL && 8 * (8 * i + (lane & 7)) >= CW) src = reinterpret_cast<const char *>(ta_zeros);
+                R[2 * i] = *reinterpret_cast<const f4 *>(src);
+                R[2 * i + 1] = *reinterpret_cast<const f4 *>(src + 16);
+            }
+            find_rows();
+        };
+        // the row in registers to LDS in ten pieces: its scale, then a column group each
+        float scale = 0.0f;
+        auto put_piece = [&](int s, int i) __attribute__((always_inline)) {
+            const int buf = s & 1;
+            if (i == 0) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int x = 0; x < 18; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(R[x][e]) & 0x7fffffffu);
+#pragma unroll
+                for (int o = 4; o >= 1; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+                // a node's row that holds an infinity or a NaN: zeros, and noted, so that the query rows that see
+                // it become NaN and no others
+                const bool bad = m >= 0x7f800000u && s * TB_TP + prow >= len;
+                const int k = row_scale(m);
+                scale = bad ? 0.0f : __uint_as_float((uint32_t)(127 + k) << 23);
+                s_k[32 * buf + prow] = k;   // eight lanes the same
+                s_ok[8 * buf + wv] = (uint8_t)gather_rows(__ballot(rok));
+                s_ok[8 * buf + 4 + wv] = (uint8_t)gather_rows(__ballot(bad));
+            } else {
+                const f4 u = R[2 * i - 2], v = R[2 * i - 1];
+                const float x[8] = {u.x * scale, u.y * scale, u.z * scale, u.w * scale, v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+                f16x8 hi, lo;
+                split16(x, hi, lo);
+                if (scale == 0.0f) hi = lo = f16x8(0);
+                char *at = smem + buf * TS_BUF + TB_GRP * (i - 1) + 128 * prow + 16 * lu;
+                *reinterpret_cast<f16x8 *>(at) = hi;
+                *reinterpret_cast<f16x8 *>(at + TB_BUF) = lo;
+            }
+        };
+        find_rows();
+        load_rows();
+
+        // query fragments: unit 4 ks + kq of the row, scaled and split alike
+        f16x8 qh[KS], ql[KS];
+        float qscale;
+        {
+            const float *src = reinterpret_cast<const float *>(a.q) + ((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW;
+            uint32_t m = 0;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                if (row < rows && (FULL || 8 * (4 * ks + kq) < CW))
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const f4 v = *reinterpret_cast<const f4 *>(src + 8 * (4 * ks + kq) + e);
+#pragma unroll
+                        for (int x = 0; x < 4; x++) m = max(m, __float_as_uint(v[x]) & 0x7fffffffu);
+                    }
+            m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+            m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+            const int k = row_scale(m);
+            const float sc = __uint_as_float((uint32_t)(127 + k) << 23);
+            qscale = ldexpf(a.scale2, -k);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                if (row < rows && (FULL || 8 * (4 * ks + kq) < CW))
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = src[8 * (4 * ks + kq) + e] * sc;
+                split16(x, qh[ks], ql[ks]);
+            }
+        }
+
+        const int pi = 4 * (c16 & 3) + (c16 >> 2), vr = 4 * ((lane >> 2) & 3) + kq;
+        const int ka = 128 * pi + 16 * (kq ^ ((pi >> 1) & 6));
+        const int va = 128 * vr + 16 * (((lane >> 1) & 1) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
+        auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {   // block f % 2 of K-step f / 2
+            return *(const __attribute__((address_space(3))) f16x8 *)(buf + (ka ^ (f & 2 ? 64 : 0)) + TB_GRP * (f >> 2) + 2048 * (f & 1));
+        };
+        auto vread = [&](lds_cchar *buf, int d) __attribute__((always_inline)) {
+            lds_cchar *at = buf + (va ^ (32 * (d & 3))) + TB_GRP * (d >> 2);
+            const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+            const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
+            const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
+            return __builtin_bit_cast(f16x8, uint4{y0.x, y0.y, y1.x, y1.y});
+        };
+        f32x4 acc[DT];
+        float M = -INFINITY, lsum = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 10; i++) put_piece(s0, i);
+        load_rows();
+
+        for (int s = s0; s < s1; s++) {
+            __syncthreads();   // step s is staged, step s - 1 read
+            lds_cchar *cur = (lds_cchar *)smem + (s & 1) * TS_BUF;
+            constexpr int AK = 4, AV = 4;   // fragment pairs read ahead
+            f16x8 kh[AK], kl[AK];
+            f32x4 S[2], Sl[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) S[i] = Sl[i] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < AK; f++) {
+                kh[f] = kread(cur, f);
+                kl[f] = kread(cur + TB_BUF, f);
+            }
+#pragma unroll
+            for (int f = 0; f < 2 * KS; f++) {
+                const f16x8 h = kh[f % AK], l = kl[f % AK];
+                S[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, qh[f >> 1], S[f & 1], 0, 0, 0);
+                Sl[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, ql[f >> 1], Sl[f & 1], 0, 0, 0);
+                Sl[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l, qh[f >> 1], Sl[f & 1], 0, 0, 0);
+                if (f + AK < 2 * KS) {
+                    kh[f % AK] = kread(cur, f + AK);
+                    kl[f % AK] = kread(cur + TB_BUF, f + AK);
+                }
+                if (f >= 4 && f < 34 && (f - 4) % 3 == 0) put_piece(s + 1, (f - 4) / 3);   // past the end: rows of zeros
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_rows();   // of step s + 2
+            // scores in base 2 with their rows' scales, masks, softmax
+            int k[8];
+            float y[8];
+            const uint32_t *okw = reinterpret_cast<const uint32_t *>(s_ok) + 2 * (s & 1);
+            const uint32_t ok = okw[0], bad = okw[1];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    k[4 * i + e] = s_k[32 * (s & 1) + 16 * i + 4 * e + kq];
+                    y[4 * i + e] = ldexpf((S[i][e] + Sl[i][e]) * qscale, -k[4 * i + e]);
+                }
+            if (ok != 0xffffffffu || (s + 1) * TB_TP > len) {
+                const int n0 = len - s * TB_TP;   // place of the first node in the step
+                const uint64_t anc = s_anc[row < rows ? row / H : 0];
+                uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
+                if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc << n0);
+                else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc >> -n0);
+                w &= ok;
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const int bit = 16 * (x >> 2) + 4 * (x & 3) + kq;
+                    const float seen = bad >> bit & 1 ? NAN : 0.0f;
+                    y[x] = w >> bit & 1 ? y[x] + seen : -INFINITY;
+                }
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 8; x++) mt = fmaxf(mt, y[x] - (float)k[x]);
+            mt = quarter_max(mt);
+            if (__ballot(mt > M + TA_LAZY)) {
+                const float mn = mt > M + TA_LAZY ? mt : M;
+                const float al = mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+                M = mn;
+                lsum *= al;
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[d] *= al;
+            }
+            const float ref = M == -INFINITY ? 0.0f : M - TS_UP;
+            f16x8 ph, pl;
+            float pw[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                pw[x] = __builtin_amdgcn_exp2f(y[x] - (float)k[x] - ref);
+                lsum += ldexpf(pw[x], k[x]);
+            }
+            split16(pw, ph, pl);
+            f16x8 vh[AV], vl[AV];
+#pragma unroll
+            for (int d = 0; d < AV; d++) {
+                vh[d] = vread(cur, d);
+                vl[d] = vread(cur + TB_BUF, d);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d += 2) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[(d + i) % AV], ph, acc[d + i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 2; i++) acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[(d + i) % AV], pl, acc[d + i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 2; i++) acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[(d + i) % AV], ph, acc[d + i], 0, 0, 0);
+                if (d + AV < DT)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        vh[(d + i) % AV] = vread(cur, d + i + AV);
+                        vl[(d + i) % AV] = vread(cur + TB_BUF, d + i + AV);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        lsum += __shfl_xor(lsum, 16, 64);
+        lsum += __shfl_xor(lsum, 32, 64);
+
+        if (row >= rows) continue;
+        const size_t orow = (size_t)b * a.t.N * H + row, part = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
+        if (split) {
+            if (kq == 0) {
+                a.pm[part] = M;
+                a.pl[part] = lsum;
+            }
+            if (M == -INFINITY) continue;   // nothing seen: the merge does not read its sums
+            float *dst = a.po + part * KL + 4 * kq;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+                if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d];
+        } else {
+            if (kq == 0 && a.lse) a.lse[orow] = lsum == 0.0f ? -INFINITY : (M - TS_UP + __builtin_amdgcn_logf(lsum)) * TA_LN2;
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+            if (a.o_dt == K3HIP_F32) {
+                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * kq;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+                    if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d] * inv;
+            } else {
+                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * kq;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+                    if (16 * d + 4 * kq < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d] * inv);
+            }
+        }
+    }
+}
+
+// The parts of a row merged, by W waves: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s, wave w the parts
+// w, w + W, ..., the waves' sums in order. Four waves a row where there are few rows, and long sequences have many parts; one
+// where there are many (16,384 rows of two parts: 40 us with four waves, 21 with one). Every part's (M_s, l_s) is asked for at once, a part a lane, and
+// the sums four parts at a time (one after the other their latencies made a merge of 16 parts 27 us). A
+// part that saw nothing (M_s = -inf) left no sums: its memory is read, its weight not used.
+constexpr int TM_NT = 256, TM_PER = 4;
+template <int W>
+__global__ __launch_bounds__(TM_NT) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows, float up)
+{
+    __shared__ float s_m[4], s_l[4];
+    __shared__ f32x4 s_v[3][TA_KL / 4];
+    const int b = blockIdx.y, lane = threadIdx.x & 63, wv = W == 4 ? threadIdx.x >> 6 : 0;
+    const int row = W == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= tree_count(a.t, b) * a.H) return;
     const int rt = row / tile_rows, in = row % tile_rows;
-    int n = a.nsplit;
-    int4 p = {0, 0, 0, 0};
-    if (a.plan) {
-        p = a.plan[b];
-        n = p.y - p.x + 1;
-        if (n <= 1) return;   // written by its only workgroup
-    }
-    // part s: fp32 in order; bf16 the first slot's second part, then the others' first
-    auto at = [&](int s) -> size_t {
-        return (a.plan ? 2 * ((size_t)(p.x + s) * p.z + rt) + (s == 0) : ((size_t)b * a.nrt + rt) * n + s) * tile_rows + in;
-    };
+    const int4 p = a.plan[b];
+    const int n = p.y - p.x + 1;
+    if (n <= 1) return;   // written by its only workgroup
+    // part s: the first slot's second part, then the others' first
+    auto at = [&](int s) -> size_t { return (2 * ((size_t)(p.x + s) * p.z + rt) + (s == 0)) * tile_rows + in; };
+    const int mine = n > wv ? (n - wv + W - 1) / W : 0;   // this wave's parts
     float M = -INFINITY, l = 0.0f;
-    for (int s = 0; s < n; s++) M = fmaxf(M, a.pm[at(s)]);
-    for (int c0 = 0; c0 < a.KL; c0 += 256) {
-        const int c = c0 + 4 * lane;
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        l = 0.0f;
-        for (int s = 0; s < n; s++) {
-            const float m = a.pm[at(s)];
-            if (m == -INFINITY) continue;
-            const float w = __builtin_amdgcn_exp2f(m - M);
-            l += w * a.pl[at(s)];
-            if (c < a.KL) v += w * *reinterpret_cast<const f32x4 *>(a.po + at(s) * a.KL + c);
-        }
-        if (c < a.KL) {
-            const size_t at = ((size_t)b * a.t.N * a.H + row) * a.KL + c;
-            v *= l == 0.0f ? 0.0f : 1.0f / l;
-            if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + at) = v;
-            else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + at) = pack4(v);
+    f32x4 v[2] = {f32x4(0.0f), f32x4(0.0f)};
+    for (int i0 = 0; i0 < mine; i0 += 64) {
+        const bool has = i0 + lane < mine;
+        const size_t pa = at(wv + W * (has ? i0 + lane : 0));
+        const float m = has ? a.pm[pa] : -INFINITY, pl = a.pl[pa];
+        float mx = m;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+        if (mx == -INFINITY) continue;
+        const float mn = fmaxf(M, mx), old = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
+        const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        float ls = w == 0.0f ? 0.0f : w * pl;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o, 64);
+        l = l * old + ls;
+        v[0] *= old;
+        v[1] *= old;
+        M = mn;
+        for (int i = 0; i < min(64, mine - i0); i += TM_PER) {
+            f32x4 x[TM_PER][2];
+            float ws[TM_PER];
+#pragma unroll
+            for (int k = 0; k < TM_PER; k++) {
+                const bool ok = i0 + i + k < mine;
+                ws[k] = ok ? __shfl(w, i + k, 64) : 0.0f;
+                const float *src = a.po + at(wv + W * (ok ? i0 + i + k : i0 + i)) * a.KL;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int ch = 256 * c + 4 * lane;
+                    x[k][c] = ch < a.KL ? *reinterpret_cast<const f32x4 *>(src + ch) : f32x4(0.0f);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < TM_PER; k++)
+                if (ws[k] != 0.0f) {
+                    v[0] += ws[k] * x[k][0];
+                    v[1] += ws[k] * x[k][1];
+                }
         }
     }
-    if (a.lse && lane == 0)
-        a.lse[(size_t)b * a.t.N * a.H + row] = l == 0.0f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * TA_LN2;
+    float Mx = M;
+    f32x4 t[2] = {v[0], v[1]};
+    if constexpr (W == 4) {
+        if (lane == 0) {
+            s_m[wv] = M;
+            s_l[wv] = l;
+        }
+        if (wv > 0) {
+            s_v[wv - 1][lane] = v[0];
+            s_v[wv - 1][64 + lane] = v[1];
+        }
+        __syncthreads();
+        if (wv > 0) return;
+        Mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+        l = 0.0f;
+        t[0] = t[1] = f32x4(0.0f);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (s_m[k] == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(s_m[k] - Mx);
+            l += w * s_l[k];
+            t[0] += w * (k ? s_v[k ? k - 1 : 0][lane] : v[0]);
+            t[1] += w * (k ? s_v[k ? k - 1 : 0][64 + lane] : v[1]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t orow = (size_t)b * a.t.N * a.H + row;
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const int ch = 256 * c + 4 * lane;
+        if (ch >= a.KL) continue;
+        if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * a.KL + ch) = t[c] * inv;
+        else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * a.KL + ch) = pack4(t[c] * inv);
+    }
+    if (a.lse && lane == 0) a.lse[orow] = l == 0.0f ? -INFINITY : (Mx - up + __builtin_amdgcn_logf(l)) * TA_LN2;
 }
 
-// Query rows a workgroup takes: the fewest tiles of a sequence that its rows fill.
-int ta_rows(bool f32, long rows)
-{
-    if (f32) return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    return rows <= 64 ? 64 : 128;
-}
+// Query rows a workgroup takes: 128 only on bf16, where a sequence fills them.
+int ta_rows(bool f32, long rows) { return f32 || rows <= 64 ? 64 : 128; }
 
-int ta_split(int B, int nrt, int tiles)
-{
-    int ncu = 256;
-    (void)cu_count(ncu);
-    const long wg = (long)B * nrt;
-    return (int)std::max(1L, std::min({(long)tiles, ncu / wg, 64L}));
-}
-
-// bf16: the workgroups of a launch, the least multiple of the CUs whose slots of n leave no more than a
+// The workgroups of a launch, the least multiple of the CUs whose slots of n leave no more than a
 // tenth of them without work.
 long ta_grid(int n)
 {
@@ -1136,10 +1134,12 @@ using namespace k3kda;
 extern "C" size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora)
 {
     if (B <= 0 || N <= 0 || N > TREE_MAX || H <= 0 || kv_lora <= 0 || kv_lora > TA_KL) return 0;
-    const int r4 = ta_rows(true, (long)N * H), n4 = (int)(((long)N * H + r4 - 1) / r4);
-    const int r2 = ta_rows(false, (long)N * H), n2 = (int)(((long)N * H + r2 - 1) / r2);
-    return std::max(ta_ws_bytes((long)B * n4 * ta_split(B, n4, 1 << 20), r4, kv_lora, B),
-                    ta_ws_bytes(2 * ta_grid(n2), r2, kv_lora, B));
+    size_t most = 0;
+    for (bool f32 : {false, true}) {
+        const int rows = ta_rows(f32, (long)N * H);
+        most = std::max(most, ta_ws_bytes(2 * ta_grid((int)(((long)N * H + rows - 1) / rows)), rows, kv_lora, B));
+    }
+    return most;
 }
 
 extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int rope, float scale, const void *q,
@@ -1176,62 +1176,40 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     a.pages = pages; a.q = q; a.o = o; a.o_dt = o_dtype; a.lse = lse;
     a.scale2 = scale * TA_LOG2E;
     const int rows = ta_rows(f32, (long)N * H);
-    a.nrt = (int)(((long)N * H + rows - 1) / rows);
+    const long grid = ta_grid((int)(((long)N * H + rows - 1) / rows));
     a.B = B;
-    const long tp = f32 ? 32 : TB_TP, tiles = ((long)max_pages * page + N + tp - 1) / tp;
-    long parts, grid16 = 0;
-    bool split;
-    if (f32) {
-        a.nsplit = ta_split(B, a.nrt, (int)tiles);
-        parts = (long)B * a.nrt * a.nsplit;
-        split = a.nsplit > 1;
-    } else {
-        grid16 = ta_grid(a.nrt);
-        parts = 2 * grid16;
-        split = true;
-        a.tcol = TB_TP / page;
-        a.trow = TB_TP % page;
-        a.page_bytes = (uint32_t)page * (uint32_t)CW * 2;
-    }
+    a.tcol = TB_TP / page;
+    a.trow = TB_TP % page;
+    a.page_bytes = (uint32_t)page * (uint32_t)CW * (f32 ? 4 : 2);
+    const size_t need = ta_ws_bytes(2 * grid, rows, kv_lora, B);
     StreamBuf buf;
-    if (split) {
-        const size_t need = ta_ws_bytes(parts, rows, kv_lora, B);
-        if (!workspace) {
-            if (int rc = stream_alloc(buf, need, st)) return rc;
-            workspace = buf.p;
-        } else if (workspace_bytes < need || ((uintptr_t)workspace & 15)) {
-            K3_FAIL(K3HIP_EINVAL, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
-        }
-        const size_t r = (size_t)parts * rows;
-        a.po = (float *)workspace;
-        a.pm = (float *)((char *)workspace + up256(r * kv_lora * 4));
-        a.pl = (float *)((char *)a.pm + up256(r * 4));
-        if (!f32) a.plan = (int4 *)((char *)a.pl + up256(r * 4));
+    if (!workspace) {
+        if (int rc = stream_alloc(buf, need, st)) return rc;
+        workspace = buf.p;
+    } else if (workspace_bytes < need || ((uintptr_t)workspace & 15)) {
+        K3_FAIL(K3HIP_EINVAL, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, workspace_bytes, need);
     }
+    const size_t r = (size_t)2 * grid * rows;
+    a.po = (float *)workspace;
+    a.pm = (float *)((char *)workspace + up256(r * kv_lora * 4));
+    a.pl = (float *)((char *)a.pm + up256(r * 4));
+    a.plan = (int4 *)((char *)a.pl + up256(r * 4));
+    // bf16: whole rows of eight in one page go by buffer loads
     const void *kern;
-    dim3 grid;
-    size_t lds;
-    if (f32) {
-        kern = rows == 16 ? (const void *)tree_attn_kernel<true, 1, 1, 2> : rows == 32 ? (const void *)tree_attn_kernel<true, 1, 2, 2>
-                                                                                      : (const void *)tree_attn_kernel<true, 1, 4, 1>;
-        grid = dim3(a.nsplit, a.nrt, B);
-        lds = TA_LDS;
-    } else {
-        // whole rows of eight in one page go by buffer loads
-        kern = CW == TA_CW && page % 8 == 0 ? (rows == 64 ? (const void *)tree_attn16_kernel<true, 1> : (const void *)tree_attn16_kernel<true, 2>)
-                                            : (rows == 64 ? (const void *)tree_attn16_kernel<false, 1> : (const void *)tree_attn16_kernel<false, 2>);
-        grid = dim3((unsigned)grid16);
-        lds = TB_LDS;
-    }
+    const size_t lds = f32 ? TS_LDS : TB_LDS;
+    if (f32) kern = CW == TA_CW ? (const void *)tree_attn32_kernel<true> : (const void *)tree_attn32_kernel<false>;
+    else if (CW == TA_CW && page % 8 == 0)
+        kern = rows == 64 ? (const void *)tree_attn16_kernel<true, 1> : (const void *)tree_attn16_kernel<true, 2>;
+    else kern = rows == 64 ? (const void *)tree_attn16_kernel<false, 1> : (const void *)tree_attn16_kernel<false, 2>;
     K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *args[] = {&a};
-    K3_HIP(hipLaunchKernel(kern, grid, dim3(TA_NT), args, lds, st));
+    K3_HIP(hipLaunchKernel(kern, dim3((unsigned)grid), dim3(TA_NT), args, lds, st));
     K3_LAUNCHED();
-    if (split) {
-        const int per = TA_NT / 64;
-        hipLaunchKernelGGL(tree_attn_merge_kernel, dim3((unsigned)(((long)N * H + per - 1) / per), (unsigned)B), dim3(TA_NT),
-                           0, st, a, rows);
-        K3_LAUNCHED();
-    }
+    const float up = f32 ? TS_UP : 0.0f;
+    if ((long)B * N * H <= 2048)
+        hipLaunchKernelGGL((tree_attn_merge_kernel<4>), dim3((unsigned)(N * H), (unsigned)B), dim3(TM_NT), 0, st, a, rows, up);
+    else
+        hipLaunchKernelGGL((tree_attn_merge_kernel<1>), dim3((unsigned)((N * H + 3) / 4), (unsigned)B), dim3(TM_NT), 0, st, a, rows, up);
+    K3_LAUNCHED();
     return K3HIP_OK;
 }
