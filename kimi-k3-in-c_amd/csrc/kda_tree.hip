@@ -40,11 +40,28 @@ struct TreeArgs {
     void *y;
     int y_dt;
     const int *accept;
+    bool vec, vec_y;             // inputs and y may be accessed four elements at a time
 };
 
 __device__ __forceinline__ float load_any(const void *p, int dt, size_t i)
 {
     return dt == K3HIP_BF16 ? load_act<K3HIP_BF16>(p, i) : load_act<K3HIP_F32>(p, i);
+}
+
+// Four adjacent elements i .. i + 3 of an activation, 16-byte (fp32) or 8-byte (bf16) aligned where vec.
+__device__ __forceinline__ f4 load_four(const void *p, int dt, size_t i, bool vec)
+{
+    if (!vec) return f4{load_any(p, dt, i), load_any(p, dt, i + 1), load_any(p, dt, i + 2), load_any(p, dt, i + 3)};
+    if (dt == K3HIP_F32) return *reinterpret_cast<const f4 *>(reinterpret_cast<const float *>(p) + i);
+    const uint2 v = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
+    return f4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+              __uint_as_float(v.y & 0xffff0000u)};
+}
+
+// The decay e^g of logit z (without its bias dt), ea = e^A_log.
+__device__ __forceinline__ float decay_of(float lb, float ea, float z, float dt)
+{
+    return fast_exp(lb != 0.0f ? gate_bounded(lb, gate_a2(ea), z, dt) : -ea * softplus_ref(z + dt));
 }
 
 // K1 of one node by one half-wave, CPL adjacent channels a lane from channel c0 of the layer (cl of the
@@ -86,17 +103,13 @@ __device__ __forceinline__ void tree_conv(float (&x)[CPL], const TreeArgs &a, in
     if (which < 2) l2norm_half<CPL>(x);
 }
 
-// The decay of one node, as above.
+// The decays of one node.
 template <int CPL>
 __device__ __forceinline__ void tree_decay(float (&x)[CPL], const TreeArgs &a, size_t row, int h, size_t P, size_t c0)
 {
     const float ea = expf(a.A_log[h]);
 #pragma unroll
-    for (int e = 0; e < CPL; e++) {
-        const float z = a.z[row * P + c0 + e], dt = a.dt_bias[c0 + e];
-        const float g = a.lb != 0.0f ? gate_bounded(a.lb, gate_a2(ea), z, dt) : -ea * softplus_ref(z + dt);
-        x[e] = fast_exp(g);
-    }
+    for (int e = 0; e < CPL; e++) x[e] = decay_of(a.lb, ea, a.z[row * P + c0 + e], a.dt_bias[c0 + e]);
 }
 
 // Sum over the 16 lanes of a row, in every lane.
@@ -108,70 +121,196 @@ __device__ __forceinline__ float row_sum(float x)
     return x + dpp_f<0x140>(x);   // mirror in 16
 }
 
+// CPL adjacent floats between registers and LDS, 16 bytes at a time where there are four.
+template <int CPL>
+__device__ __forceinline__ void lds_get(float (&x)[CPL], const float *p)
+{
+    if constexpr (CPL == 4) {
+        const f4 v = *reinterpret_cast<const f4 *>(p);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < CPL; e++) x[e] = p[e];
+    }
+}
+template <int CPL>
+__device__ __forceinline__ void lds_put(float *p, const float (&x)[CPL])
+{
+    if constexpr (CPL == 4) *reinterpret_cast<f4 *>(p) = f4{x[0], x[1], x[2], x[3]};
+    else {
+#pragma unroll
+        for (int e = 0; e < CPL; e++) p[e] = x[e];
+    }
+}
+
+// The D / 16 channels of lane c16 of sixteen: quads 64 channels apart, so that sixteen lanes' reads are on
+// distinct banks.
+template <int CH>
+__device__ __forceinline__ void walk_get(float (&x)[CH], const float *row, int c16)
+{
+    if constexpr (CH >= 4) {
+#pragma unroll
+        for (int e = 0; e < CH; e += 4) {
+            const f4 v = *reinterpret_cast<const f4 *>(row + 16 * e + 4 * c16);
+            x[e] = v.x; x[e + 1] = v.y; x[e + 2] = v.z; x[e + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < CH; e++) x[e] = row[CH * c16 + e];
+    }
+}
+template <int CH>
+__device__ __forceinline__ void walk_put(float *row, const float (&x)[CH], int c16)
+{
+    if constexpr (CH >= 4) {
+#pragma unroll
+        for (int e = 0; e < CH; e += 4) *reinterpret_cast<f4 *>(row + 16 * e + 4 * c16) = f4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < CH; e++) row[CH * c16 + e] = x[e];
+    }
+}
+
 template <int D, int TILES>
-struct TreeLds {
+struct alignas(16) TreeLds {
     static constexpr int R = 16 * TILES;   // node rows, zero past the tree
     static constexpr int DP = D + 4;       // pitch: 16 rows x 4 adjacent floats on distinct banks
     static constexpr int AP = R + 4;
     float q[R * DP], k[R * DP], v[R * DP], a[R * DP];
-    float A[R * AP];   // [j][m] above the diagonal: k_m . E_mj k_j; [n][j] on and below: q_n . E_nj k_j
+    union {
+        float A[R * AP];   // [j][m] above the diagonal: k_m . E_mj k_j; [n][j] on and below: q_n . E_nj k_j
+        struct {
+            float w[3][4][D], h[3][3][D];   // before it: the head's conv taps and history, tap and slot major
+        } c;
+    };
     float beta[R];
     int par[R];
 };
 
 // One workgroup per (head, sequence), a wave per 16 value columns (value columns never meet before the
-// norm): the wave's columns of S are asked for first, as the B fragments of v_mfma_f32_16x16x4_f32, and
-// arrive while K1 and the pair products run. TILES: 16-row node tiles.
+// norm). Everything is asked for at the start, in the order in which it is needed: the raw inputs (vectors of
+// four channels), the conv's taps and history, the wave's columns of S as B fragments of
+// v_mfma_f32_16x16x4_f32, the output gate. (K1 with loads of its own for each tap, 2 and 4 bytes a lane, held a
+// workgroup for 42 us at 64 sequences x 16 nodes: 200 us a launch.) TILES: 16-row node tiles.
 template <int D, int TILES>
-__global__ __launch_bounds__(4 * D) void kda_tree_kernel(const TreeArgs a)
+__global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
 {
     constexpr int NT = 4 * D;
     using L = TreeLds<D, TILES>;
     constexpr int R = L::R, DP = L::DP, AP = L::AP;
     constexpr int CPL = D >= 32 ? D / 32 : 1;
+    constexpr int C4 = D / 4, HWS = NT / 32;
     extern __shared__ __attribute__((aligned(16))) char tree_smem[];
     L &s = *reinterpret_cast<L *>(tree_smem);
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int N = tree_count(a.t, b);
+    const int N = tree_count(a.t, b), K = a.K;
     if (N == 0) return;
-    const size_t P = (size_t)a.H * D, row0 = (size_t)b * a.t.N;
+    const size_t P = (size_t)a.H * D, row0 = (size_t)b * a.t.N, c0 = (size_t)h * D;
     const float *hist = a.hist + (size_t)b * a.h_stride;
     const float *S = a.S + (size_t)b * a.s_stride + (size_t)h * D * D;
 
-    // S fragments: lane l holds rows 4 t + l / 16, column 16 wv + l % 16
-    const int c16 = lane & 15, kq = lane >> 4;
-    float sf[D / 4];
+    // raw inputs: thread tid takes channels 4 (tid % C4) .. + 3 of rows tid / C4 + 16 i
+    const int rch = 4 * (tid % C4), rrow = tid / C4;
+    f4 raw[TILES][4];
 #pragma unroll
-    for (int t = 0; t < D / 4; t++) sf[t] = S[(size_t)(4 * t + kq) * D + 16 * wv + c16];
-
-    for (int i = tid; i < R * AP; i += NT) s.A[i] = 0.0f;
-    if (tid < R) {
-        s.par[tid] = tid < N ? tree_parent(a.t, b, tid) : -1;
-        s.beta[tid] = tid < N ? fast_sigmoid(a.bl[(row0 + tid) * a.H + h]) : 0.0f;
+    for (int i = 0; i < TILES; i++) {
+        const int n = rrow + 16 * i;
+        const size_t at = (row0 + (n < N ? n : 0)) * P + c0 + rch;
+        raw[i][0] = load_four(a.qi, a.in_dt, at, a.vec);
+        raw[i][1] = load_four(a.ki, a.in_dt, at, a.vec);
+        raw[i][2] = load_four(a.vi, a.in_dt, at, a.vec);
+        raw[i][3] = load_four(a.z, K3HIP_F32, at, a.vec);
     }
-    for (int i = tid; i < (R - N) * DP; i += NT) {
-        const int at = N * DP + i;
-        s.q[at] = s.k[at] = s.v[at] = s.a[at] = 0.0f;
+    const f4 dtb = load_four(a.dt_bias, K3HIP_F32, c0 + rch, a.vec);
+    const float A_log = a.A_log[h];
+    const int par0 = tid < N ? tree_parent(a.t, b, tid) : -1;
+    const float bl = tid < N ? a.bl[(row0 + tid) * a.H + h] : 0.0f;
+    // taps and history of the head's channels, one (matrix, channel) a thread
+    float tap[4], old[3];
+    const int cm = tid / D, cc = tid % D;   // the fourth part of the threads has none
+    if (cm < 3) {
+        const float *w = (cm == 0 ? a.q_conv : cm == 1 ? a.k_conv : a.v_conv) + (c0 + cc) * K;
+        const float *hs = hist + ((size_t)cm * P + c0 + cc) * (K - 1);
+#pragma unroll
+        for (int j = 0; j < 4; j++) tap[j] = j < K ? w[j] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 3; j++) old[j] = j < K - 1 ? hs[j] : 0.0f;
+    }
+    const int c16 = lane & 15, kq = lane >> 4, l32 = tid & 31, hw = tid >> 5;
+    const bool active = l32 * CPL < D;
+    const int cl = active ? l32 * CPL : 0;
+
+    // inputs to LDS (decays at once; zeros past the tree)
+    {
+        const float ea = expf(A_log);
+#pragma unroll
+        for (int i = 0; i < TILES; i++) {
+            const int n = rrow + 16 * i, at = n * DP + rch;
+            const bool ok = n < N;
+            f4 d;
+#pragma unroll
+            for (int e = 0; e < 4; e++) d[e] = decay_of(a.lb, ea, raw[i][3][e], dtb[e]);
+            *reinterpret_cast<f4 *>(s.q + at) = ok ? raw[i][0] : f4(0.0f);
+            *reinterpret_cast<f4 *>(s.k + at) = ok ? raw[i][1] : f4(0.0f);
+            *reinterpret_cast<f4 *>(s.v + at) = ok ? raw[i][2] : f4(0.0f);
+            *reinterpret_cast<f4 *>(s.a + at) = ok ? d : f4(0.0f);
+        }
+    }
+    if (tid < R) {
+        s.par[tid] = par0;
+        s.beta[tid] = tid < N ? fast_sigmoid(bl) : 0.0f;
+    }
+    if (cm < 3) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) s.c.w[cm][j][cc] = tap[j];
+#pragma unroll
+        for (int j = 0; j < 3; j++) s.c.h[cm][j][cc] = old[j];
     }
     __syncthreads();
 
-    // K1, a task of a node per half-wave
-    {
-        const int l32 = tid & 31;
-        const bool active = l32 * CPL < D;
-        const int cl = active ? l32 * CPL : 0;
-        const size_t c0 = (size_t)h * D + cl;
-        for (int task = tid >> 5; task < 4 * N; task += NT / 32) {
-            const int which = task & 3, n = task >> 2;
-            float x[CPL];
-            if (which < 3) tree_conv<CPL>(x, a, which, n, s.par, row0, P, c0, active, hist);
-            else tree_decay<CPL>(x, a, row0 + n, h, P, c0);
-            float *dst = (which == 0 ? s.q : which == 1 ? s.k : which == 2 ? s.v : s.a) + n * DP + cl;
-            if (active)
+    // K1: short conv over the node and its ancestors, then the history (kda_prep_math.h's arithmetic, taps oldest
+    // first), L2 norm of q and k; a (matrix, node) a half-wave, results held until all inputs were read
+    constexpr int KPT = 3 * R / HWS;
+    float kx[KPT][CPL];
 #pragma unroll
-                for (int e = 0; e < CPL; e++) dst[e] = which == 0 ? x[e] * a.q_scale : x[e];
+    for (int i = 0; i < KPT; i++) {
+        const int task = hw + HWS * i, which = task % 3, n = task / 3;
+        if (n >= N) continue;
+        const float *x = which == 0 ? s.q : (which == 1 ? s.k : s.v);
+        float in[4][CPL];
+        int m = n, past = 0;   // past: slots back into the history (1 = its newest)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            lds_get<CPL>(in[j], (m >= 0 ? x + m * DP : s.c.h[which][max(K - 1 - past, 0)]) + cl);
+            if (m >= 0) m = s.par[m];
+            if (m < 0) past++;
         }
+        float w[4][CPL];   // tap j tokens back
+#pragma unroll
+        for (int j = 0; j < 4; j++) lds_get<CPL>(w[j], s.c.w[which][max(K - 1 - j, 0)] + cl);
+#pragma unroll
+        for (int e = 0; e < CPL; e++) {
+            float acc = w[0][e] * in[0][e];
+#pragma unroll
+            for (int j = 3; j >= 1; j--) acc = j < K ? __builtin_fmaf(w[j][e], in[j][e], acc) : acc;
+            kx[i][e] = active ? acc * fast_sigmoid(acc) : 0.0f;
+        }
+        if (which < 2) l2norm_half<CPL>(kx[i]);
     }
+    // S fragments: lane l holds rows 4 t + l / 16, column 16 wv + l % 16
+    float sf[D / 4];
+#pragma unroll
+    for (int t = 0; t < D / 4; t++) sf[t] = S[(size_t)(4 * t + kq) * D + 16 * wv + c16];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < KPT; i++) {
+        const int task = hw + HWS * i, which = task % 3, n = task / 3;
+        if (n >= N || !active) continue;
+#pragma unroll
+        for (int e = 0; e < CPL; e++) kx[i][e] = which == 0 ? kx[i][e] * a.q_scale : kx[i][e];
+        lds_put<CPL>((which == 0 ? s.q : which == 1 ? s.k : s.v) + n * DP + cl, kx[i]);
+    }
+    for (int i = tid; i < R * AP; i += NT) s.A[i] = 0.0f;
     __syncthreads();
 
     // pair products: 16 lanes walk from node m up its path, D / 16 channels a lane, and end with E_m0
@@ -183,20 +322,21 @@ __global__ __launch_bounds__(4 * D) void kda_tree_kernel(const TreeArgs a)
         const int m = (tid >> 4) + r * GR;
         if (m < N) {
             float E[CH];
+            walk_get<CH>(kt[r], s.k + m * DP, c16);
+            walk_get<CH>(qt[r], s.q + m * DP, c16);
 #pragma unroll
-            for (int e = 0; e < CH; e++) {
-                E[e] = 1.0f;
-                kt[r][e] = s.k[m * DP + CH * c16 + e];
-                qt[r][e] = s.q[m * DP + CH * c16 + e];
-            }
-            for (int j = m; j >= 0; j = s.par[j]) {
-                float kk = 0.0f, qk = 0.0f;
+            for (int e = 0; e < CH; e++) E[e] = 1.0f;
+            for (int j = m; j >= 0;) {
+                const int up = s.par[j];
+                float kj[CH], aj[CH], kk = 0.0f, qk = 0.0f;
+                walk_get<CH>(kj, s.k + j * DP, c16);
+                walk_get<CH>(aj, s.a + j * DP, c16);
 #pragma unroll
                 for (int e = 0; e < CH; e++) {
-                    const float x = E[e] * s.k[j * DP + CH * c16 + e];
+                    const float x = E[e] * kj[e];
                     kk = __builtin_fmaf(kt[r][e], x, kk);
                     qk = __builtin_fmaf(qt[r][e], x, qk);
-                    E[e] *= s.a[j * DP + CH * c16 + e];
+                    E[e] *= aj[e];
                 }
                 kk = row_sum(kk);
                 qk = row_sum(qk);
@@ -204,6 +344,7 @@ __global__ __launch_bounds__(4 * D) void kda_tree_kernel(const TreeArgs a)
                     if (j != m) s.A[j * AP + m] = kk;
                     s.A[m * AP + j] = qk;
                 }
+                j = up;
             }
 #pragma unroll
             for (int e = 0; e < CH; e++) {
@@ -216,12 +357,10 @@ __global__ __launch_bounds__(4 * D) void kda_tree_kernel(const TreeArgs a)
 #pragma unroll
     for (int r = 0; r < RPG; r++) {
         const int m = (tid >> 4) + r * GR;
-        if (m < N)
-#pragma unroll
-            for (int e = 0; e < CH; e++) {
-                s.k[m * DP + CH * c16 + e] = kt[r][e];
-                s.q[m * DP + CH * c16 + e] = qt[r][e];
-            }
+        if (m < N) {
+            walk_put<CH>(s.k + m * DP, kt[r], c16);
+            walk_put<CH>(s.q + m * DP, qt[r], c16);
+        }
     }
     __syncthreads();
 
@@ -245,6 +384,18 @@ __global__ __launch_bounds__(4 * D) void kda_tree_kernel(const TreeArgs a)
         }
     }
     __syncthreads();
+
+    // output gate and norm: half-wave hw takes nodes hw, hw + HWS, ...
+    constexpr int GPT = R / HWS;   // its nodes
+    float gate[GPT][CPL], on[CPL];
+#pragma unroll
+    for (int i = 0; i < GPT; i++) {
+        const int n = hw + HWS * i;
+#pragma unroll
+        for (int e = 0; e < CPL; e++) gate[i][e] = load_any(a.gate, a.g_dt, (row0 + (n < N ? n : 0)) * P + c0 + cl + e);
+    }
+#pragma unroll
+    for (int e = 0; e < CPL; e++) on[e] = a.o_norm[cl + e];
 
     // forward substitution, a thread per value column: w_m = rhs_m - beta_m sum_j A_mj w_j, 16 rows at a
     // time in registers
@@ -288,25 +439,32 @@ __global__ __launch_bounds__(4 * D) void kda_tree_kernel(const TreeArgs a)
     __syncthreads();
 
     // K4, a node per half-wave
-    {
-        const int l32 = tid & 31;
-        const bool active = l32 * CPL < D;
-        const int cl = active ? l32 * CPL : 0;
-        for (int n = tid >> 5; n < N; n += NT / 32) {
-            float x[CPL], part = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GPT; i++) {
+        const int n = hw + HWS * i;
+        if (n >= N) continue;
+        float x[CPL], part = 0.0f;
+        lds_get<CPL>(x, s.v + n * DP + cl);
+#pragma unroll
+        for (int e = 0; e < CPL; e++) {
+            part += active ? x[e] * x[e] : 0.0f;
+        }
+        const float inv = __builtin_amdgcn_rsqf(half_wave_sum(part) / (float)D + a.eps);
+        if (!active) continue;
+        const size_t at = (row0 + n) * P + c0 + cl;
+#pragma unroll
+        for (int e = 0; e < CPL; e++) x[e] = on[e] * x[e] * inv * fast_sigmoid(gate[i][e]);
+        if (CPL == 4 && a.vec_y) {
+            if (a.y_dt == K3HIP_BF16)
+                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.y) + at) =
+                    uint2{(uint32_t)f2bf(x[0]) | ((uint32_t)f2bf(x[CPL > 1 ? 1 : 0]) << 16),
+                          (uint32_t)f2bf(x[CPL > 2 ? 2 : 0]) | ((uint32_t)f2bf(x[CPL > 3 ? 3 : 0]) << 16)};
+            else *reinterpret_cast<f4 *>(reinterpret_cast<float *>(a.y) + at) = f4{x[0], x[CPL > 1 ? 1 : 0], x[CPL > 2 ? 2 : 0], x[CPL > 3 ? 3 : 0]};
+        } else {
 #pragma unroll
             for (int e = 0; e < CPL; e++) {
-                x[e] = s.v[n * DP + cl + e];
-                part += active ? x[e] * x[e] : 0.0f;
-            }
-            const float inv = __builtin_amdgcn_rsqf(half_wave_sum(part) / (float)D + a.eps);
-            if (!active) continue;
-            const size_t at = (row0 + n) * P + (size_t)h * D + cl;
-#pragma unroll
-            for (int e = 0; e < CPL; e++) {
-                const float y = a.o_norm[cl + e] * x[e] * inv * fast_sigmoid(load_any(a.gate, a.g_dt, at + e));
-                if (a.y_dt == K3HIP_BF16) reinterpret_cast<uint16_t *>(a.y)[at + e] = f2bf(y);
-                else reinterpret_cast<float *>(a.y)[at + e] = y;
+                if (a.y_dt == K3HIP_BF16) reinterpret_cast<uint16_t *>(a.y)[at + e] = f2bf(x[e]);
+                else reinterpret_cast<float *>(a.y)[at + e] = x[e];
             }
         }
     }
@@ -450,6 +608,8 @@ int tree_args(const char *who, TreeArgs &a, int B, int N, int H, int D, int K, f
     a.q_conv = q_conv; a.k_conv = k_conv; a.v_conv = v_conv; a.A_log = A_log; a.dt_bias = dt_bias;
     a.hist = const_cast<float *>(conv_state); a.h_stride = conv_stride;
     a.S = const_cast<float *>(S); a.s_stride = s_stride;
+    a.vec = (((uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in) & (in_dtype == K3HIP_F32 ? 15 : 7)) == 0 &&
+            (((uintptr_t)z | (uintptr_t)dt_bias) & 15) == 0;
     return K3HIP_OK;
 }
 
@@ -481,6 +641,7 @@ extern "C" int k3hip_kda_tree_step(int B, int N, int H, int D, int K, float gate
     a.eps = rms_eps; a.q_scale = q_scale;
     a.gate = gate; a.g_dt = gate_dtype; a.o_norm = o_norm;
     a.y = y; a.y_dt = y_dtype;
+    a.vec_y = ((uintptr_t)y & (y_dtype == K3HIP_F32 ? 15 : 7)) == 0;
     switch (D) {
     case 16: return launch_tree_d<16>(B, a, as_stream(stream));
     case 32: return launch_tree_d<32>(B, a, as_stream(stream));
