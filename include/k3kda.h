@@ -371,7 +371,7 @@ int k3hip_mla_decode(const k3hip_mla_weights *w, int B, int pos, int cap, float 
  *           NULL: a chain
  *   accept  [B] the last accepted node; anything that is no node of its sequence: none
  * all int32 device memory, read when the call runs. N is at most 64 (a chain's append: any). Rows of
- * nodes past counts[b] are not read and their results are left as they were. Values out of range are
+ * nodes past counts[b] have no effect and their results are left as they were. Values out of range are
  * taken as said, never as an address: lengths are limited to what the table holds.
  *
  * A paged latent cache holds what k3hip_mla_decode's cache holds per position, the rmsnorm'd latent

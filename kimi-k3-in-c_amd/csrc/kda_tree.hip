@@ -112,15 +112,6 @@ __device__ __forceinline__ void tree_decay(float (&x)[CPL], const TreeArgs &a, s
     for (int e = 0; e < CPL; e++) x[e] = decay_of(a.lb, ea, a.z[row * P + c0 + e], a.dt_bias[c0 + e]);
 }
 
-// Sum over the 16 lanes of a row, in every lane.
-__device__ __forceinline__ float row_sum(float x)
-{
-    x = x + dpp_f<0xB1>(x);    // lane ^ 1
-    x = x + dpp_f<0x4E>(x);    // lane ^ 2
-    x = x + dpp_f<0x141>(x);   // mirror in 8
-    return x + dpp_f<0x140>(x);   // mirror in 16
-}
-
 // CPL adjacent floats between registers and LDS, 16 bytes at a time where there are four.
 template <int CPL>
 __device__ __forceinline__ void lds_get(float (&x)[CPL], const float *p)
@@ -143,34 +134,6 @@ __device__ __forceinline__ void lds_put(float *p, const float (&x)[CPL])
     }
 }
 
-// The D / 16 channels of lane c16 of sixteen: quads 64 channels apart, so that sixteen lanes' reads are on
-// distinct banks.
-template <int CH>
-__device__ __forceinline__ void walk_get(float (&x)[CH], const float *row, int c16)
-{
-    if constexpr (CH >= 4) {
-#pragma unroll
-        for (int e = 0; e < CH; e += 4) {
-            const f4 v = *reinterpret_cast<const f4 *>(row + 16 * e + 4 * c16);
-            x[e] = v.x; x[e + 1] = v.y; x[e + 2] = v.z; x[e + 3] = v.w;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < CH; e++) x[e] = row[CH * c16 + e];
-    }
-}
-template <int CH>
-__device__ __forceinline__ void walk_put(float *row, const float (&x)[CH], int c16)
-{
-    if constexpr (CH >= 4) {
-#pragma unroll
-        for (int e = 0; e < CH; e += 4) *reinterpret_cast<f4 *>(row + 16 * e + 4 * c16) = f4{x[e], x[e + 1], x[e + 2], x[e + 3]};
-    } else {
-#pragma unroll
-        for (int e = 0; e < CH; e++) row[CH * c16 + e] = x[e];
-    }
-}
-
 template <int D, int TILES>
 struct alignas(16) TreeLds {
     static constexpr int R = 16 * TILES;   // node rows, zero past the tree
@@ -184,7 +147,8 @@ struct alignas(16) TreeLds {
         } c;
     };
     float beta[R];
-    int par[R];
+    uint64_t anc[R];   // the node and its ancestors, a bit each
+    uint32_t up[R];    // the node, its parent, the parent's and the one after, a byte each; 0x80 + i: i back in the history
 };
 
 // One workgroup per (head, sequence), a wave per 16 value columns (value columns never meet before the
@@ -193,7 +157,7 @@ struct alignas(16) TreeLds {
 // v_mfma_f32_16x16x4_f32, the output gate. (K1 with loads of its own for each tap, 2 and 4 bytes a lane, held a
 // workgroup for 42 us at 64 sequences x 16 nodes: 200 us a launch.) TILES: 16-row node tiles.
 template <int D, int TILES>
-__global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
+__global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tree_kernel(const TreeArgs a)
 {
     constexpr int NT = 4 * D;
     using L = TreeLds<D, TILES>;
@@ -204,7 +168,6 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
     L &s = *reinterpret_cast<L *>(tree_smem);
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int N = tree_count(a.t, b), K = a.K;
-    if (N == 0) return;
     const size_t P = (size_t)a.H * D, row0 = (size_t)b * a.t.N, c0 = (size_t)h * D;
     const float *hist = a.hist + (size_t)b * a.h_stride;
     const float *S = a.S + (size_t)b * a.s_stride + (size_t)h * D * D;
@@ -215,7 +178,7 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
 #pragma unroll
     for (int i = 0; i < TILES; i++) {
         const int n = rrow + 16 * i;
-        const size_t at = (row0 + (n < N ? n : 0)) * P + c0 + rch;
+        const size_t at = (row0 + (n < a.t.N ? n : 0)) * P + c0 + rch;   // also of rows that are no nodes: no wait for the count
         raw[i][0] = load_four(a.qi, a.in_dt, at, a.vec);
         raw[i][1] = load_four(a.ki, a.in_dt, at, a.vec);
         raw[i][2] = load_four(a.vi, a.in_dt, at, a.vec);
@@ -223,8 +186,13 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
     }
     const f4 dtb = load_four(a.dt_bias, K3HIP_F32, c0 + rch, a.vec);
     const float A_log = a.A_log[h];
-    const int par0 = tid < N ? tree_parent(a.t, b, tid) : -1;
-    const float bl = tid < N ? a.bl[(row0 + tid) * a.H + h] : 0.0f;
+    const int par0 = tid < a.t.N ? tree_parent(a.t, b, tid) : -1;
+    float s_bl[R / HWS];   // of this half-wave's rows
+#pragma unroll
+    for (int r = 0; r < R / HWS; r++) {
+        const int n = (tid >> 5) + HWS * r;
+        s_bl[r] = a.bl[(row0 + (n < a.t.N ? n : 0)) * a.H + h];
+    }
     // taps and history of the head's channels, one (matrix, channel) a thread
     float tap[4], old[3];
     const int cm = tid / D, cc = tid % D;   // the fourth part of the threads has none
@@ -240,6 +208,8 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
     const bool active = l32 * CPL < D;
     const int cl = active ? l32 * CPL : 0;
 
+    if (N == 0) return;
+    constexpr int TPR = R / HWS;   // rows a half-wave, hw + HWS r
     // inputs to LDS (decays at once; zeros past the tree)
     {
         const float ea = expf(A_log);
@@ -256,9 +226,21 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
             *reinterpret_cast<f4 *>(s.a + at) = ok ? d : f4(0.0f);
         }
     }
-    if (tid < R) {
-        s.par[tid] = par0;
-        s.beta[tid] = tid < N ? fast_sigmoid(bl) : 0.0f;
+    if (tid < 64) {   // lane = node
+        const uint64_t anc = tree_ancestors(par0);
+        uint32_t up = lane & 0x7f;
+        int m = lane, past = 0;
+#pragma unroll
+        for (int j = 1; j < 4; j++) {
+            const int p = __shfl(par0, m < 0 ? 0 : m, 64);
+            m = m < 0 ? -1 : p;
+            past += m < 0;
+            up |= (uint32_t)(m < 0 ? 0x80 + past : m) << (8 * j);
+        }
+        if (lane < R) {
+            s.anc[lane] = anc;
+            s.up[lane] = up;
+        }
     }
     if (cm < 3) {
 #pragma unroll
@@ -277,13 +259,12 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
         const int task = hw + HWS * i, which = task % 3, n = task / 3;
         if (n >= N) continue;
         const float *x = which == 0 ? s.q : (which == 1 ? s.k : s.v);
+        const uint32_t up = s.up[n];
         float in[4][CPL];
-        int m = n, past = 0;   // past: slots back into the history (1 = its newest)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            lds_get<CPL>(in[j], (m >= 0 ? x + m * DP : s.c.h[which][max(K - 1 - past, 0)]) + cl);
-            if (m >= 0) m = s.par[m];
-            if (m < 0) past++;
+            const int m = up >> (8 * j) & 0xff;
+            lds_get<CPL>(in[j], (m < 0x80 ? x + m * DP : s.c.h[which][max(K - 1 - (m - 0x80), 0)]) + cl);
         }
         float w[4][CPL];   // tap j tokens back
 #pragma unroll
@@ -313,41 +294,49 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
     for (int i = tid; i < R * AP; i += NT) s.A[i] = 0.0f;
     __syncthreads();
 
-    // pair products: 16 lanes walk from node m up its path, D / 16 channels a lane, and end with E_m0
-    constexpr int CH = D / 16, GR = NT / 16;
-    constexpr int RPG = (R + GR - 1) / GR;   // rows a group of lanes
-    float kt[RPG][CH], qt[RPG][CH];
+    // pair products: a half-wave walks from node m up its path (its ancestors from the highest number down),
+    // the next ancestor's row asked for before the current one's products, and ends with E_m0
+    float kt[TPR][CPL], qt[TPR][CPL];
 #pragma unroll
-    for (int r = 0; r < RPG; r++) {
-        const int m = (tid >> 4) + r * GR;
+    for (int r = 0; r < TPR; r++) {
+        const int m = hw + HWS * r;
         if (m < N) {
-            float E[CH];
-            walk_get<CH>(kt[r], s.k + m * DP, c16);
-            walk_get<CH>(qt[r], s.q + m * DP, c16);
+            const float beta = fast_sigmoid(s_bl[r]);
+            uint64_t left = s.anc[m];
+            float E[CPL], kj[CPL], aj[CPL];
+            lds_get<CPL>(kt[r], s.k + m * DP + cl);
+            lds_get<CPL>(qt[r], s.q + m * DP + cl);
+            lds_get<CPL>(aj, s.a + m * DP + cl);
 #pragma unroll
-            for (int e = 0; e < CH; e++) E[e] = 1.0f;
+            for (int e = 0; e < CPL; e++) {
+                E[e] = active ? 1.0f : 0.0f;
+                kj[e] = kt[r][e];
+            }
             for (int j = m; j >= 0;) {
-                const int up = s.par[j];
-                float kj[CH], aj[CH], kk = 0.0f, qk = 0.0f;
-                walk_get<CH>(kj, s.k + j * DP, c16);
-                walk_get<CH>(aj, s.a + j * DP, c16);
+                left &= (1ull << j) - 1;
+                const int up = left ? 63 - __builtin_clzll(left) : -1, ld = max(up, 0);
+                float kn[CPL], an[CPL], kk = 0.0f, qk = 0.0f;
+                lds_get<CPL>(kn, s.k + ld * DP + cl);
+                lds_get<CPL>(an, s.a + ld * DP + cl);
 #pragma unroll
-                for (int e = 0; e < CH; e++) {
+                for (int e = 0; e < CPL; e++) {
                     const float x = E[e] * kj[e];
                     kk = __builtin_fmaf(kt[r][e], x, kk);
                     qk = __builtin_fmaf(qt[r][e], x, qk);
                     E[e] *= aj[e];
+                    kj[e] = kn[e];
+                    aj[e] = an[e];
                 }
-                kk = row_sum(kk);
-                qk = row_sum(qk);
-                if (c16 == 0) {
-                    if (j != m) s.A[j * AP + m] = kk;
+                kk = half_wave_sum(kk);
+                qk = half_wave_sum(qk);
+                if (l32 == 0) {
+                    if (j != m) s.A[j * AP + m] = beta * kk;
                     s.A[m * AP + j] = qk;
                 }
                 j = up;
             }
 #pragma unroll
-            for (int e = 0; e < CH; e++) {
+            for (int e = 0; e < CPL; e++) {
                 kt[r][e] *= E[e];
                 qt[r][e] *= E[e];
             }
@@ -355,11 +344,12 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RPG; r++) {
-        const int m = (tid >> 4) + r * GR;
-        if (m < N) {
-            walk_put<CH>(s.k + m * DP, kt[r], c16);
-            walk_put<CH>(s.q + m * DP, qt[r], c16);
+    for (int r = 0; r < TPR; r++) {
+        const int m = hw + HWS * r;
+        if (l32 == 0) s.beta[m] = m < N ? fast_sigmoid(s_bl[r]) : 0.0f;
+        if (m < N && active) {
+            lds_put<CPL>(s.k + m * DP + cl, kt[r]);
+            lds_put<CPL>(s.q + m * DP + cl, qt[r]);
         }
     }
     __syncthreads();
@@ -392,34 +382,38 @@ __global__ __launch_bounds__(4 * D, 1) void kda_tree_kernel(const TreeArgs a)
     for (int i = 0; i < GPT; i++) {
         const int n = hw + HWS * i;
 #pragma unroll
-        for (int e = 0; e < CPL; e++) gate[i][e] = load_any(a.gate, a.g_dt, (row0 + (n < N ? n : 0)) * P + c0 + cl + e);
+        for (int e = 0; e < CPL; e++) gate[i][e] = load_any(a.gate, a.g_dt, (row0 + (n < a.t.N ? n : 0)) * P + c0 + cl + e);
     }
 #pragma unroll
     for (int e = 0; e < CPL; e++) on[e] = a.o_norm[cl + e];
 
-    // forward substitution, a thread per value column: w_m = rhs_m - beta_m sum_j A_mj w_j, 16 rows at a
-    // time in registers
+    // forward substitution, a thread per value column, 16 rows at a time in registers: w_m = rhs_m - sum_j
+    // beta_m A_mj w_j
     if (tid < D) {
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
             float w[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = 0.0f;
+            for (int i = 0; i < 16; i++) w[i] = s.a[(16 * t + i) * DP + tid];
             for (int j = 0; j < 16 * t; j++) {
                 const float x = s.a[j * DP + tid];
                 const float *Aj = s.A + j * AP + 16 * t;
 #pragma unroll
-                for (int i = 0; i < 16; i++) w[i] = __builtin_fmaf(Aj[i], x, w[i]);
+                for (int i = 0; i < 16; i++) w[i] = __builtin_fmaf(-Aj[i], x, w[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int m = 16 * t + i;
-                w[i] = __builtin_fmaf(-s.beta[m], w[i], s.a[m * DP + tid]);
-                s.a[m * DP + tid] = w[i];
-                const float *Ai = s.A + m * AP + 16 * t;
+            for (int i = 0; i < 15; i++) {
+                const float *Ai = s.A + (16 * t + i) * AP + 16 * t;
 #pragma unroll
-                for (int i2 = i + 1; i2 < 16; i2++) w[i2] = __builtin_fmaf(Ai[i2], w[i], w[i2]);
+                for (int q = (i + 1) / 4; q < 4; q++) {
+                    const f4 c = *reinterpret_cast<const f4 *>(Ai + 4 * q);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (4 * q + e > i) w[4 * q + e] = __builtin_fmaf(-c[e], w[i], w[4 * q + e]);
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 16; i++) s.a[(16 * t + i) * DP + tid] = w[i];
         }
     }
     __syncthreads();
