@@ -318,24 +318,34 @@ def kda_epilogue(o, gate, o_norm, y, H: int, D: int, rms_eps: float, stream=None
 ROPE_PAIRS, ROPE_HALVES = 0, 1
 
 
-def _i32(t, *shape):
+def _get(t, dtype, shape):
+    """Device pointer of a dense tensor of the given dtype (a torch dtype, None: any) and shape, None -> NULL. One
+    expression for what is right: a call has up to twenty tensors, and its host time is that of its checks."""
     if t is None:
         return None
-    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape:
-        raise ValueError(f"k3kda: int32 tensor of shape {shape} required, got {t.dtype} {tuple(t.shape)}")
-    return _ptr(t)
+    if (dtype is None or t.dtype is dtype) and t.shape == shape and t.is_cuda and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"k3kda: dense device tensor of shape {shape}{'' if dtype is None else f' and {dtype}'} required, "
+                     f"got {tuple(t.shape)}, {t.dtype}, strides {t.stride()} on {t.device}")
 
 
-def _shape(t, *shape):
-    if t is not None and tuple(t.shape) != shape:
-        raise ValueError(f"k3kda: shape {shape} required, got {tuple(t.shape)}")
-    return _ptr(t)
+_I32 = _F32 = None
 
 
-def _f32(t, *shape):
-    if t is not None and str(t.dtype) != "torch.float32":
-        raise ValueError(f"k3kda: float32 required, got {t.dtype}")
-    return _shape(t, *shape)
+def _types():
+    """torch's int32 and float32 (imported with the first call: the module itself needs no torch)."""
+    global _I32, _F32
+    import torch
+    _I32, _F32 = torch.int32, torch.float32
+
+
+def _table(pages, table, B: int):
+    """(pages, dtype, n_pages, page, table, max_pages) as the C entry points take them."""
+    if _I32 is None:
+        _types()
+    n_pages, page, width = pages.shape
+    cols = table.shape[1]
+    return _get(pages, None, (n_pages, page, width)), _dt(pages), n_pages, page, _get(table, _I32, (B, cols)), cols
 
 
 def _rows(t, inner: int):
@@ -358,23 +368,22 @@ def latent_append(rows, pages, table, lens, kv_lora: int, norm_w=None, eps: floa
     """rows [B, N, kv_lora + rope] normalised, rotated and written to the cache at lens[b] + n; q [B, N, H, rope]
     rotated into q_out (either may be a slice of wider rows)."""
     B, N, W = rows.shape
-    n_pages, page, width = pages.shape
-    if width != W:
-        raise ValueError(f"k3kda: rows of {W} for a cache of {width}")
+    if pages.shape[2] != W:
+        raise ValueError(f"k3kda: rows of {W} for a cache of {pages.shape[2]}")
     R = W - kv_lora
     at, ld = _rows(rows, 1)
+    pp, dt, n_pages, page, tp, cols = _table(pages, table, B)
     H = qp = qd = ql = qh = op = od = ol = oh = 0
     if q is not None:
         H = q.shape[2]
-        if tuple(q.shape) != (B, N, H, R) or q_out is None or q_out.shape != q.shape:
+        if q.shape != (B, N, H, R) or q_out is None or q_out.shape != q.shape:
             raise ValueError(f"k3kda: q and q_out of shape {(B, N, H, R)} required")
         (qp, ql), (op, ol) = _rows(q, 2), _rows(q_out, 2)
         qd, od, qh, oh = _dt(q), _dt(q_out), q.stride(2), q_out.stride(2)
-    _check(lib().k3hip_latent_append(B, N, kv_lora, R, _ptr(pages), _dt(pages), n_pages, page,
-                                     _i32(table, B, table.shape[1]), table.shape[1], _i32(lens, B), _i32(counts, B),
-                                     _i32(parents, B, N), at, _dt(rows), ld, _f32(norm_w, kv_lora), eps,
-                                     _f32(inv_freq, R // 2), rope_style, H, qp, qd, ql, qh, op, od, ol, oh,
-                                     _stream(stream)))
+    _check(lib().k3hip_latent_append(B, N, kv_lora, R, pp, dt, n_pages, page, tp, cols, _get(lens, _I32, (B,)),
+                                     _get(counts, _I32, (B,)), _get(parents, _I32, (B, N)), at, _dt(rows), ld,
+                                     _get(norm_w, _F32, (kv_lora,)), eps, _get(inv_freq, _F32, (R // 2,)), rope_style,
+                                     H, qp, qd, ql, qh, op, od, ol, oh, _stream(stream)))
 
 
 def mla_tree_workspace(B: int, N: int, H: int, kv_lora: int) -> int:
@@ -386,42 +395,51 @@ def mla_tree_attention(q, pages, table, lens, o, kv_lora: int, scale: float, cou
     """q [B, N, H, kv_lora + rope] (absorbed, the cache's dtype) over the cache and each node's ancestors;
     o [B, N, H, kv_lora], lse [B, N, H] fp32."""
     B, N, H, W = q.shape
-    n_pages, page, width = pages.shape
-    if width != W or q.dtype != pages.dtype:
-        raise ValueError(f"k3kda: q rows of {W} {q.dtype} for a cache of {width} {pages.dtype}")
+    if pages.shape[2] != W:
+        raise ValueError(f"k3kda: q rows of {W} for a cache of {pages.shape[2]}")
+    pp, dt, n_pages, page, tp, cols = _table(pages, table, B)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _check(lib().k3hip_mla_tree_attention(B, N, H, kv_lora, W - kv_lora, scale, _ptr(q), _ptr(pages), _dt(pages), n_pages,
-                                          page, _i32(table, B, table.shape[1]), table.shape[1], _i32(lens, B),
-                                          _i32(counts, B), _i32(parents, B, N), _shape(o, B, N, H, kv_lora), _dt(o),
-                                          _f32(lse, B, N, H), _ptr(workspace), ws_bytes, _stream(stream)))
+    _check(lib().k3hip_mla_tree_attention(B, N, H, kv_lora, W - kv_lora, scale, _get(q, pages.dtype, (B, N, H, W)), pp, dt,
+                                          n_pages, page, tp, cols, _get(lens, _I32, (B,)), _get(counts, _I32, (B,)),
+                                          _get(parents, _I32, (B, N)), _get(o, None, (B, N, H, kv_lora)), _dt(o),
+                                          _get(lse, _F32, (B, N, H)), _ptr(workspace), ws_bytes, _stream(stream)))
 
 
 def latent_commit(pages, table, lens, accept, N: int, lens_out=None, counts=None, parents=None, stream=None) -> None:
     """The accepted path's rows moved to lens[b], lens[b] + 1, ...; lens_out = lens + the path's length."""
-    n_pages, page, width = pages.shape
     B = lens.shape[0]
-    _check(lib().k3hip_latent_commit(B, N, width, _ptr(pages), _dt(pages), n_pages, page,
-                                     _i32(table, B, table.shape[1]), table.shape[1], _i32(lens, B), _i32(counts, B),
-                                     _i32(parents, B, N), _i32(accept, B), _i32(lens_out, B), _stream(stream)))
+    pp, dt, n_pages, page, tp, cols = _table(pages, table, B)
+    _check(lib().k3hip_latent_commit(B, N, pages.shape[2], pp, dt, n_pages, page, tp, cols, _get(lens, _I32, (B,)),
+                                     _get(counts, _I32, (B,)), _get(parents, _I32, (B, N)), _get(accept, _I32, (B,)),
+                                     _get(lens_out, _I32, (B,)), _stream(stream)))
 
 
-def _slots(t, *shape):
+def _slots(t, shape):
     """(address, stride between sequences) of per-sequence state that is dense within a sequence."""
     if t is None:
         return None, 0
-    if not t.is_cuda or str(t.dtype) != "torch.float32" or tuple(t.shape) != shape:
+    if t.dtype is not _F32 or t.shape != shape or not t.is_cuda:
         raise ValueError(f"k3kda: float32 device tensor of shape {shape} required, got {t.dtype} {tuple(t.shape)}")
-    if t.shape[0] and not t[0].is_contiguous():
-        raise ValueError("k3kda: state must be contiguous within a sequence")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else 0
+    if t.is_contiguous():
+        n = 1
+        for d in shape[1:]:
+            n *= d
+        return t.data_ptr(), n
+    if shape[0] and not t[0].is_contiguous():
+        raise ValueError("k3kda: state must be dense within a sequence")
+    return t.data_ptr(), t.stride(0)
 
 
-def _tree_inputs(q_in, k_in, v_in, z, b_logit, convs, A_log, dt_bias, H: int, D: int, K: int):
+def _tree_inputs(q_in, k_in, v_in, z, b_logit, q_conv, k_conv, v_conv, A_log, dt_bias, H: int, D: int, K: int):
+    if _I32 is None:
+        _types()
     B, N, P = q_in.shape
-    if P != H * D or k_in.dtype != q_in.dtype or v_in.dtype != q_in.dtype:
-        raise ValueError(f"k3kda: q_in, k_in, v_in [B, N, {H * D}] of one dtype required")
-    return (_dt(q_in), _ptr(q_in), _shape(k_in, B, N, P), _shape(v_in, B, N, P), _f32(z, B, N, P), _f32(b_logit, B, N, H),
-            *(_f32(w, P, K) for w in convs), _f32(A_log, H), _f32(dt_bias, P))
+    if P != H * D:
+        raise ValueError(f"k3kda: q_in, k_in, v_in [B, N, {H * D}] required")
+    rows, conv, act, f32 = (B, N, P), (P, K), q_in.dtype, _F32
+    return (_dt(q_in), _get(q_in, act, rows), _get(k_in, act, rows), _get(v_in, act, rows), _get(z, f32, rows),
+            _get(b_logit, f32, (B, N, H)), _get(q_conv, f32, conv), _get(k_conv, f32, conv), _get(v_conv, f32, conv),
+            _get(A_log, f32, (H,)), _get(dt_bias, f32, (P,)))
 
 
 def kda_tree_step(q_in, k_in, v_in, z, b_logit, gate, q_conv, k_conv, v_conv, A_log, dt_bias, o_norm, conv_state, S, y,
@@ -430,23 +448,25 @@ def kda_tree_step(q_in, k_in, v_in, z, b_logit, gate, q_conv, k_conv, v_conv, A_
     """kda_decode_step for every node of a tree: inputs and y [B, N, P]; S [B, H, D, D] and conv_state
     [B, 3, P, K-1] (dense within a sequence) are only read."""
     B, N, P = q_in.shape
-    dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp = _tree_inputs(q_in, k_in, v_in, z, b_logit, (q_conv, k_conv, v_conv), A_log,
+    dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp = _tree_inputs(q_in, k_in, v_in, z, b_logit, q_conv, k_conv, v_conv, A_log,
                                                               dt_bias, H, D, K)
-    (Sp, ss), (hp, hs) = _slots(S, B, H, D, D), _slots(conv_state, B, 3, P, K - 1)
-    _check(lib().k3hip_kda_tree_step(B, N, H, D, K, gate_lb, rms_eps, dt, qp, kp, vp, zp, bp, _shape(gate, B, N, P),
-                                     _dt(gate), cq, ck, cv, Ap, dp, _f32(o_norm, D), hp, hs, q_scale, Sp, ss,
-                                     _i32(counts, B), _i32(parents, B, N), _shape(y, B, N, P), _dt(y), _stream(stream)))
+    (Sp, ss), (hp, hs) = _slots(S, (B, H, D, D)), _slots(conv_state, (B, 3, P, K - 1))
+    _check(lib().k3hip_kda_tree_step(B, N, H, D, K, gate_lb, rms_eps, dt, qp, kp, vp, zp, bp, _get(gate, None, (B, N, P)),
+                                     _dt(gate), cq, ck, cv, Ap, dp, _get(o_norm, _F32, (D,)), hp, hs, q_scale, Sp, ss,
+                                     _get(counts, _I32, (B,)), _get(parents, _I32, (B, N)), _get(y, None, (B, N, P)), _dt(y),
+                                     _stream(stream)))
 
 
 def kda_tree_commit(q_in, k_in, v_in, z, b_logit, q_conv, k_conv, v_conv, A_log, dt_bias, conv_state, S, accept, H: int,
                     D: int, K: int, gate_lb: float, counts=None, parents=None, stream=None) -> None:
     """S and conv_state moved to those of each sequence's accepted node (-1: left), from the step's inputs."""
     B, N, P = q_in.shape
-    dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp = _tree_inputs(q_in, k_in, v_in, z, b_logit, (q_conv, k_conv, v_conv), A_log,
+    dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp = _tree_inputs(q_in, k_in, v_in, z, b_logit, q_conv, k_conv, v_conv, A_log,
                                                               dt_bias, H, D, K)
-    (Sp, ss), (hp, hs) = _slots(S, B, H, D, D), _slots(conv_state, B, 3, P, K - 1)
+    (Sp, ss), (hp, hs) = _slots(S, (B, H, D, D)), _slots(conv_state, (B, 3, P, K - 1))
     _check(lib().k3hip_kda_tree_commit(B, N, H, D, K, gate_lb, dt, qp, kp, vp, zp, bp, cq, ck, cv, Ap, dp, hp, hs, Sp, ss,
-                                       _i32(counts, B), _i32(parents, B, N), _i32(accept, B), _stream(stream)))
+                                       _get(counts, _I32, (B,)), _get(parents, _I32, (B, N)), _get(accept, _I32, (B,)),
+                                       _stream(stream)))
 
 
 class DeviceWeights:
