@@ -64,54 +64,6 @@ __device__ __forceinline__ float decay_of(float lb, float ea, float z, float dt)
     return fast_exp(lb != 0.0f ? gate_bounded(lb, gate_a2(ea), z, dt) : -ea * softplus_ref(z + dt));
 }
 
-// K1 of one node by one half-wave, CPL adjacent channels a lane from channel c0 of the layer (cl of the
-// head): which = 0, 1, 2 the short conv of q, k, v over the node and its ancestors, then the history
-// (the arithmetic of kda_prep_math.h, taps oldest first), L2-normalised for q and k. par: the sequence's
-// parents in LDS; row0: its first row.
-template <int CPL>
-__device__ __forceinline__ void tree_conv(float (&x)[CPL], const TreeArgs &a, int which, int n, const int *par, size_t row0,
-                                          size_t P, size_t c0, bool active, const float *hist)
-{
-    const float *cw = which == 0 ? a.q_conv : (which == 1 ? a.k_conv : a.v_conv);
-    const void *src = which == 0 ? a.qi : (which == 1 ? a.ki : a.vi);
-    const int K = a.K;
-    float in[4][CPL];   // inputs 0 .. 3 tokens back
-    int m = n, past = 0;   // past: tokens back into the history (1 = its newest)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int hs = (K - 1) - past;
-#pragma unroll
-        for (int e = 0; e < CPL; e++) {
-            in[j][e] = 0.0f;
-            if (j < K) {
-                if (m >= 0) in[j][e] = load_any(src, a.in_dt, (row0 + m) * P + c0 + e);
-                else in[j][e] = hist[((size_t)which * P + c0 + e) * (K - 1) + hs];
-            }
-        }
-        if (m >= 0) m = par[m];
-        if (m < 0) past++;
-    }
-#pragma unroll
-    for (int e = 0; e < CPL; e++) {
-        const float *w = cw + (c0 + e) * K;
-        float acc = w[K - 1] * in[0][e];
-#pragma unroll
-        for (int j = 3; j >= 1; j--)
-            if (j < K) acc = __builtin_fmaf(w[K - 1 - j], in[j][e], acc);
-        x[e] = active ? acc * fast_sigmoid(acc) : 0.0f;
-    }
-    if (which < 2) l2norm_half<CPL>(x);
-}
-
-// The decays of one node.
-template <int CPL>
-__device__ __forceinline__ void tree_decay(float (&x)[CPL], const TreeArgs &a, size_t row, int h, size_t P, size_t c0)
-{
-    const float ea = expf(a.A_log[h]);
-#pragma unroll
-    for (int e = 0; e < CPL; e++) x[e] = decay_of(a.lb, ea, a.z[row * P + c0 + e], a.dt_bias[c0 + e]);
-}
-
 // CPL adjacent floats between registers and LDS, 16 bytes at a time where there are four.
 template <int CPL>
 __device__ __forceinline__ void lds_get(float (&x)[CPL], const float *p)
@@ -466,55 +418,108 @@ __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tre
 
 // S := S of the accepted node, one workgroup per (head, sequence): the path's nodes one after the other
 // on a state held in registers (kda_decode_kernel's tile), so S is read once and written once whatever
-// the path's length. K1 of up to CK nodes at a time runs in parallel before them. The conv history of
-// the head's channels becomes the last K - 1 inputs of history and path.
+// the path's length. K1 of up to TREE_CK nodes at a time runs before them, from their inputs and the three before
+// them in LDS. The conv history of the head's channels becomes the last K - 1 inputs of history and path.
 constexpr int TREE_CK = 16;
 
 template <int D>
 __global__ __launch_bounds__(4 * D) void kda_tree_commit_kernel(const TreeArgs a)
 {
     constexpr int NT = 4 * D, CPR = D / 4, RPP = NT / CPR, NPASS = D / RPP;
-    constexpr int CPL = D >= 32 ? D / 32 : 1;
-    __shared__ float s_k[TREE_CK][D], s_v[TREE_CK][D], s_a[TREE_CK][D], s_b[TREE_CK];
+    constexpr int CPL = D >= 32 ? D / 32 : 1, HWS = NT / 32, KPT = 2 * TREE_CK / HWS;
+    static_assert(RPP == TREE_CK, "a pass of the workgroup covers the rows of a chunk");
+    // inputs of k and v: row 3 + i is path node i0 + i, rows 0 .. 2 the three before; then, from row 0, k and v
+    __shared__ __attribute__((aligned(16))) float s_x[2][3 + TREE_CK][D], s_a[TREE_CK][D], s_w[2][4][D];
+    __shared__ float s_b[TREE_CK];
     __shared__ f4 s_red[2][RPP][CPR];
-    __shared__ int s_par[TREE_MAX], s_node[TREE_MAX], s_n;
+    __shared__ int s_node[TREE_MAX], s_n;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int cg = tid % CPR, rs = tid / CPR;
-    const int N = tree_count(a.t, b), node = a.accept[b];
+    const int N = tree_count(a.t, b), node = a.accept[b], K = a.K, K1 = K - 1;
     if (node < 0 || node >= N) return;
-    const size_t P = (size_t)a.H * D, row0 = (size_t)b * a.t.N;
+    const size_t P = (size_t)a.H * D, row0 = (size_t)b * a.t.N, c0 = (size_t)h * D;
     float *hist = a.hist + (size_t)b * a.h_stride;
+    const int par0 = tid < 64 && lane < N ? tree_parent(a.t, b, lane) : -1;
+    float tap[4];   // of one (matrix, channel) a thread, half the threads
+    const int cm = tid / D, cc = tid % D;
+    if (cm < 2) {
+        const float *w = (cm == 0 ? a.k_conv : a.v_conv) + (c0 + cc) * K;
+#pragma unroll
+        for (int j = 0; j < 4; j++) tap[j] = j < K ? w[j] : 0.0f;
+    }
+    const f4 dtb = load_four(a.dt_bias, K3HIP_F32, c0 + 4 * cg, a.vec);
+    const float A_log = a.A_log[h];
     f4 *Sp = reinterpret_cast<f4 *>(a.S + (size_t)b * a.s_stride + (size_t)h * D * D);
     f4 s[NPASS];
 #pragma unroll
-    for (int m = 0; m < NPASS; m++) s[m] = Sp[(rs + m * RPP) * CPR + cg];
+    for (int m = 0; m < NPASS; m++) s[m] = __builtin_nontemporal_load(&Sp[(rs + m * RPP) * CPR + cg]);
     if (tid < 64) {
-        const int p = lane < N ? tree_parent(a.t, b, lane) : -1;
-        const uint64_t m = tree_ancestors(p);
+        const uint64_t m = tree_ancestors(par0);
         const uint64_t path = ((uint64_t)__shfl((uint32_t)(m >> 32), node, 64) << 32) | __shfl((uint32_t)m, node, 64);
-        s_par[lane] = p;
         if (path >> lane & 1) s_node[__popcll(path & ((1ull << lane) - 1))] = lane;
         if (lane == 0) s_n = __popcll(path);
     }
+    if (cm < 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s_w[cm][j][cc] = tap[j];
     __syncthreads();
     const int n = s_n;
-    const int l32 = tid & 31;
+    const int l32 = tid & 31, hw = tid >> 5;
     const bool active = l32 * CPL < D;
     const int cl = active ? l32 * CPL : 0;
-    const size_t c0 = (size_t)h * D + cl;
+    // inputs 4 cg .. + 3 of path position i: a node's, or the history's
+    auto input = [&](int which, int i) -> f4 {
+        if (i >= 0) return load_four(which ? a.vi : a.ki, a.in_dt, (row0 + s_node[i]) * P + c0 + 4 * cg, a.vec);
+        f4 x = 0.0f;
+        if (K1 + i >= 0)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = hist[((size_t)(1 + which) * P + c0 + 4 * cg + e) * K1 + K1 + i];
+        return x;
+    };
     for (int i0 = 0; i0 < n; i0 += TREE_CK) {
         const int ni = min(TREE_CK, n - i0);
-        for (int task = tid >> 5; task < 3 * ni; task += NT / 32) {
-            const int which = task % 3 + 1, i = task / 3, m = s_node[i0 + i];
-            float x[CPL];
-            if (which < 3) tree_conv<CPL>(x, a, which, m, s_par, row0, P, c0, active, hist);
-            else tree_decay<CPL>(x, a, row0 + m, h, P, c0);
-            float *dst = (which == 1 ? s_k[i] : which == 2 ? s_v[i] : s_a[i]) + cl;
-            if (active)
+        if (rs < ni) {
+            const f4 k = input(0, i0 + rs), v = input(1, i0 + rs);
+            const f4 z = load_four(a.z, K3HIP_F32, (row0 + s_node[i0 + rs]) * P + c0 + 4 * cg, a.vec);
+            const float ea = expf(A_log);
+            f4 d;
 #pragma unroll
-                for (int e = 0; e < CPL; e++) dst[e] = x[e];
+            for (int e = 0; e < 4; e++) d[e] = decay_of(a.lb, ea, z[e], dtb[e]);
+            *reinterpret_cast<f4 *>(&s_x[0][3 + rs][4 * cg]) = k;
+            *reinterpret_cast<f4 *>(&s_x[1][3 + rs][4 * cg]) = v;
+            *reinterpret_cast<f4 *>(&s_a[rs][4 * cg]) = d;
         }
+        if (rs >= RPP - 3)
+#pragma unroll
+            for (int which = 0; which < 2; which++)
+                *reinterpret_cast<f4 *>(&s_x[which][rs - (RPP - 3)][4 * cg]) = input(which, i0 - 3 + rs - (RPP - 3));
         if (tid < ni) s_b[tid] = fast_sigmoid(a.bl[(row0 + s_node[i0 + tid]) * a.H + h]);
+        __syncthreads();
+        float kx[KPT][CPL];
+#pragma unroll
+        for (int t = 0; t < KPT; t++) {
+            const int task = hw + HWS * t, which = task & 1, i = task >> 1;
+            if (i >= ni) continue;
+            float acc[CPL];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {   // tap 0 now, then the oldest first (kda_prep_math.h)
+                const int back = j == 0 ? 0 : 4 - j;
+                float x[CPL], w[CPL];
+                lds_get<CPL>(x, &s_x[which][3 + i - back][cl]);
+                lds_get<CPL>(w, &s_w[which][max(K1 - back, 0)][cl]);
+#pragma unroll
+                for (int e = 0; e < CPL; e++) acc[e] = j == 0 ? w[e] * x[e] : (back < K ? __builtin_fmaf(w[e], x[e], acc[e]) : acc[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < CPL; e++) kx[t][e] = active ? acc[e] * fast_sigmoid(acc[e]) : 0.0f;
+            if (which == 0) l2norm_half<CPL>(kx[t]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < KPT; t++) {
+            const int task = hw + HWS * t, which = task & 1, i = task >> 1;
+            if (i < ni && active) lds_put<CPL>(&s_x[which][i][cl], kx[t]);
+        }
         __syncthreads();
         for (int i = 0; i < ni; i++) {
             f4 u = 0.0f;
@@ -522,27 +527,26 @@ __global__ __launch_bounds__(4 * D) void kda_tree_commit_kernel(const TreeArgs a
             for (int m = 0; m < NPASS; m++) {
                 const int r = rs + m * RPP;
                 s[m] = s[m] * s_a[i][r];
-                u = u + s_k[i][r] * s[m];
+                u = u + s_x[0][i][r] * s[m];
             }
             s_red[i & 1][rs][cg] = u;
             __syncthreads();   // the other half was last read before this barrier's predecessor
             f4 ut = s_red[i & 1][0][cg];
 #pragma unroll
             for (int r = 1; r < RPP; r++) ut = ut + s_red[i & 1][r][cg];
-            const f4 d = (reinterpret_cast<const f4 *>(s_v[i])[cg] - ut) * s_b[i];
+            const f4 d = (*reinterpret_cast<const f4 *>(&s_x[1][i][4 * cg]) - ut) * s_b[i];
 #pragma unroll
-            for (int m = 0; m < NPASS; m++) s[m] = s[m] + s_k[i][rs + m * RPP] * d;
+            for (int m = 0; m < NPASS; m++) s[m] = s[m] + s_x[0][i][rs + m * RPP] * d;
         }
-        __syncthreads();   // s_k .. s_b are free; the history's last reader is done
+        __syncthreads();   // the chunk's arrays are free; the history's last reader is done
     }
 #pragma unroll
-    for (int m = 0; m < NPASS; m++) Sp[(rs + m * RPP) * CPR + cg] = s[m];
+    for (int m = 0; m < NPASS; m++) __builtin_nontemporal_store(s[m], &Sp[(rs + m * RPP) * CPR + cg]);
     // history: slot j of the new one is entry n + j of (the old K - 1, then the path's inputs); ascending
     // order, so a slot is read before the one that replaces it is written
-    const int K1 = a.K - 1;
     for (int c = tid; c < 3 * D; c += NT) {
         const int which = c / D;
-        const size_t ch = (size_t)h * D + c % D;
+        const size_t ch = c0 + c % D;
         const void *src = which == 0 ? a.qi : (which == 1 ? a.ki : a.vi);
         float *hs = hist + ((size_t)which * P + ch) * K1;
         for (int j = 0; j < K1; j++) {
