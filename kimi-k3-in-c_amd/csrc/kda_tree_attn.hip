@@ -46,6 +46,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef s16x4 __attribute__((address_space(3))) *lds_s16x4_ptr;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
+typedef __attribute__((address_space(1))) const char glb_cchar;
 typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) const char lds_cchar;
 
@@ -140,6 +141,27 @@ __device__ __forceinline__ void acc_scale(f32x4 &c, float m)
 __device__ __forceinline__ uint32_t gather_rows(uint64_t ballot)
 {
     return (uint32_t)(((ballot & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
+}
+
+// Sixteen lanes a row that agree: a bit a row.
+__device__ __forceinline__ uint32_t gather_rows16(uint64_t ballot)
+{
+    return (uint32_t)(ballot & 1) | (uint32_t)(ballot >> 15 & 2) | (uint32_t)(ballot >> 30 & 4) | (uint32_t)(ballot >> 45 & 8);
+}
+
+// The larger of x and another lane's, by a DPP control (a NaN is passed over).
+template <int C>
+__device__ __forceinline__ float dpp_max(float x)
+{
+    return fmaxf(x, __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), C, 0xf, 0xf, true)));
+}
+
+// The largest of m, |x| and |y| (NaNs are passed over), in one instruction: left to the compiler, values from
+// memory are each made canonical first. The wait states are those of a DPP read behind it.
+__device__ __forceinline__ float max_abs(float m, float x, float y)
+{
+    asm("v_max3_f32 %0, %0, |%1|, |%2|\n\ts_nop 1" : "+v"(m) : "v"(x), "v"(y));
+    return m;
 }
 
 // Either of two bf16 is an infinity or a NaN.
@@ -267,7 +289,7 @@ static_assert(TB_LDS <= 160 * 1024, "LDS");
 template <bool FAST, int NR>
 __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn16_kernel(const AttnArgs a)
 {
-    constexpr bool ASM = NR == 2;
+    constexpr bool ASM = true;
     constexpr int ROWS = 64 * NR, DT = TA_KL / 16, KS = TA_CW / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint8_t *s_ok = reinterpret_cast<uint8_t *>(smem + TB_NB * TB_BUF);   // [buffer][wave] a bit a row; [16 + wave]: not finite
@@ -294,22 +316,9 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     if (s0 >= s1 || r0 >= rows) continue;
     __syncthreads();   // the staged steps of the sequence before
 
-    if (tid < 64) s_anc[lane] = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
+    const int par = tid < 64 && lane < cnt ? tree_parent(a.t, b, lane) : -1;
     // this lane's query rows: column c16 of each of the wave's NR row tiles
     auto row_of = [&](int r) __attribute__((always_inline)) { return r0 + 16 * (NR * wv + r) + (opaque(tid) & 15); };
-    bf16x8 qb[KS][NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const int row = row_of(r);
-        const char *src = reinterpret_cast<const char *>(a.q) + ((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW * 2;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int u = 4 * ks + kq;
-            uint4 v = {0, 0, 0, 0};
-            if (row < rows && (FAST || u < CW / 8)) v = *reinterpret_cast<const uint4 *>(src + 16 * u);
-            qb[ks][r] = __builtin_bit_cast(bf16x8, v);
-        }
-    }
 
     // staging: wave wv brings rows 8 wv .. + 7 of a step
     const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
@@ -373,6 +382,36 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     auto buf_of = [](int s) { return s & (TB_NB - 1); };
     lds_char *lds = (lds_char *)smem;
 
+    // steps s0 .. s0 + 2 on their way, the page of s0 + 3 looked up; all lookups first
+    const int sm = min(s1, max(s0, len / TB_TP));   // whole steps of committed positions end here
+    {
+        int n[4], o[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            find_rows();
+            n[i] = pgn;
+            o[i] = pgo;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            pgn = n[i];
+            pgo = o[i];
+            if (i < 3) load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i));
+        }
+    }
+    // Queries; rows behind the last one read the first, their sums are not written.
+    bf16x8 qb[KS][NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const int row = row_of(r);
+        glb_cchar *src = (glb_cchar *)a.q + (((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW + 8 * kq) * 2;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            glb_cchar *at = src + 64 * ks;
+            if (!FAST && 4 * ks + kq >= CW / 8) at = (glb_cchar *)ta_zeros;
+            qb[ks][r] = *(const __attribute__((address_space(1))) bf16x8 *)at;
+        }
+    }
     f32x4 acc[DT][NR], lacc[NR];
     float M[NR];
 #pragma unroll
@@ -380,9 +419,13 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         M[r] = -INFINITY;
         lacc[r] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DT; d++) acc[d][r] = 0.0f;
+        for (int d = 0; d < DT; d++) {
+            acc[d][r] = 0.0f;
+            if constexpr (ASM) asm volatile("" : "+a"(acc[d][r]));   // there from here on, not constants
+        }
     }
     wait<ASM>();
+    if (tid < 64) s_anc[lane] = tree_ancestors(par);
     // LDS addresses in a block of 16 rows. Score product: row pi, units 4 (ks & 1) + kq of group ks / 2.
     // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4. Unit u
     // of row r stands at u ^ ((r / 2) & 6), so the other units are the first ones with a bit or two turned. The
@@ -505,20 +548,6 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
                     for (int r = 0; r < NR; r++) S[i][r][e] = -INFINITY;
     };
 
-    // steps s0 .. s0 + 2 on their way, the page of s0 + 3 looked up
-    const int sm = min(s1, max(s0, len / TB_TP));   // whole steps of committed positions end here
-    find_rows();
-#pragma unroll
-    for (int i = 0; i < 3; i++) {
-        const int n = pgn, o = pgo;
-        find_rows();   // the next lookup before this step's loads, so that waiting for it waits for none of them
-        const int n1 = pgn, o1 = pgo;
-        pgn = n;
-        pgo = o;
-        load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i));
-        pgn = n1;
-        pgo = o1;
-    }
     if (s0 < sm) {
         f32x4 S[2][NR];
         bf16x8 kf[AH], vf[AH], pf[NR];
@@ -537,7 +566,7 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 #pragma unroll
             for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
         }
-        rescale(x);
+        // the sums are zeros yet: nothing to rescale
         // Step s's sum and step s + 1's scores. The buffers as parameters that do not alias: else the compiler
         // has every transposed read wait for the loads in flight.
         auto step = [&](lds_cchar *__restrict__ cur, lds_cchar *__restrict__ nxt, lds_cchar *__restrict__ nx2,
@@ -688,21 +717,27 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // against is the largest of (score - k), so the scaled weight 2^(score - k - M) is at most 2^TS_UP ahead of its own
 // split, whatever the rows' sizes, and the sum of the weights takes the 2^k back out.
 //
-// A step is 32 positions, staged as two planes of column groups as in the bf16 kernel, two buffers. A wave
-// brings 8 rows of a step into registers while the step before it is converted and written to LDS between
-// the score products of the step before that. Four waves of 16 query rows.
+// A step is 32 positions, staged as two planes of column groups as in the bf16 kernel, two buffers. Eight
+// waves, two a SIMD: waves w and w + 4 own 16 query rows; each scores half of the cache row's channels (so it holds half
+// of the query's hi + lo, 72 registers), they add their halves through LDS, both work out the softmax, and each sums half of the
+// latent's channels (64 registers). A step has two barriers, behind the halves of the scores and behind the
+// sum; a wave keeps 4 rows on their way to registers and converts and stages them, a column group at a time, between the
+// products: groups 4 .. 8 beside the scores, where groups 0 .. 3 of the buffer carry the halves, those beside the sum.
 constexpr int TS_BUF = 2 * TB_BUF;
+constexpr int TS_NT = 512;
 constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 4 + 64 + TREE_MAX * 8;
 constexpr float TS_UP = 7.0f;     // log2 of the weight of the reference
 static_assert(TS_LDS <= 160 * 1024, "LDS");
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ void split16(const float (&x)[8], f16x8 &hi, f16x8 &lo)
+template <int N, typename V>
+__device__ __forceinline__ void split16(const float (&x)[N], V &hi, V &lo)
 {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
+    for (int e = 0; e < N; e += 2) {
         const f16x2 h = __builtin_convertvector(f2{x[e], x[e + 1]}, f16x2);
         const f16x2 l = __builtin_convertvector(f2{x[e] - (float)h[0], x[e + 1] - (float)h[1]}, f16x2);
         hi[e] = h[0];
@@ -718,17 +753,23 @@ __device__ __forceinline__ int row_scale(uint32_t most)
     return most == 0 ? 0 : min(14 - ((int)(most >> 23) - 127), 126);
 }
 
-template <bool FULL>
-__global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn32_kernel(const AttnArgs a)
+// Behind it every wave's LDS accesses before it; loads to registers stay on their way.
+__device__ __forceinline__ void lds_barrier()
 {
-    constexpr int ROWS = 64, DT = TA_KL / 16, KS = TA_CW / 32;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+template <bool FULL>
+__global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) void tree_attn32_kernel(const AttnArgs a)
+{
+    constexpr int ROWS = 64, DT = TA_KL / 32, KS = TA_CW / 64;   // a wave's halves
     extern __shared__ __attribute__((aligned(16))) char smem[];
     int *s_k = reinterpret_cast<int *>(smem + 2 * TS_BUF);               // [buffer][row] its scale
     uint8_t *s_ok = reinterpret_cast<uint8_t *>(s_k + 64);               // [buffer][seen, not finite][wave] a bit a row
     uint64_t *s_anc = reinterpret_cast<uint64_t *>(s_ok + 64);           // [node] its ancestors
 
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, kq = lane >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), half = wv >> 2;
     const int per = gridDim.x / 8, id = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     const int H = a.H, CW = FULL ? TA_CW : a.CW, KL = a.KL;
     Slots sl;
@@ -748,135 +789,172 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
         if (s0 >= s1 || r0 >= rows) continue;
         __syncthreads();   // the staged steps of the sequence before
 
-        if (tid < 64) s_anc[lane] = tree_ancestors(lane < cnt ? tree_parent(a.t, b, lane) : -1);
-        const int row = r0 + 16 * wv + c16;   // this lane's query row
+        const int par = tid < 64 && lane < cnt ? tree_parent(a.t, b, lane) : -1;
+        const int row = r0 + 16 * (wv & 3) + c16;   // this lane's query row
 
-        // staging: rows 8 wv .. + 7 of a step, units lane & 7 of eight channels of each column group
-        const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
+        // staging: rows 4 wv .. + 3 of a step, channels 4 (lane & 15) .. + 3 of each column group
+        const int prow = 4 * wv + kq;
         const int ecol = min(end / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? end - ecol * a.c.page : 0;
-        int ncol = (s0 * TB_TP + prow) / a.c.page, nrow = s0 * TB_TP + prow - ncol * a.c.page, pgn = -1, pgo = 0;
+        int col = (s0 * TB_TP + prow) / a.c.page, prw = s0 * TB_TP + prow - col * a.c.page;   // of the row to load next
         const int *table = a.c.table + (size_t)b * a.c.max_pages;
-        auto find_rows = [&]() __attribute__((always_inline)) {
-            const bool in = (ncol < ecol) | ((ncol == ecol) & (nrow < erow));
-            const int n = table[in ? ncol : 0];
-            pgn = in ? n : -1;
-            pgo = nrow;
-            nrow += a.trow;
-            ncol += a.tcol + (nrow >= a.c.page);
-            nrow -= nrow >= a.c.page ? a.c.page : 0;
+        auto has_page = [&]() __attribute__((always_inline)) { return (col < ecol) | ((col == ecol) & (prw < erow)); };
+        int page = table[has_page() ? col : 0];
+        f4 R[9];                       // the row's values in flight
+        bool rok = false, nok = false; // that row, and the one that next_row found, have a page
+        glb_cchar *src = nullptr;
+        auto next_row = [&]() __attribute__((always_inline)) {
+            rok = nok;
+            nok = has_page() & (page >= 0) & (page < a.c.n_pages);
+            const uint64_t at = (uint64_t)(uint32_t)page * a.page_bytes + (uint32_t)prw * (uint32_t)(CW * 4);
+            src = (nok ? (glb_cchar *)a.pages + at : (glb_cchar *)ta_zeros) + 16 * c16;
+            prw += a.trow;
+            col += a.tcol + (prw >= a.c.page);
+            prw -= prw >= a.c.page ? a.c.page : 0;
+            page = table[has_page() ? col : 0];
         };
-        f4 R[18];          // the row's values in flight
-        bool rok = false;  // it has a page
-        auto load_rows = [&]() __attribute__((always_inline)) {
-            rok = pgn >= 0 && pgn < a.c.n_pages;
-            const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)pgn * a.page_bytes + (uint32_t)pgo * (uint32_t)(CW * 4);
-            p = rok ? p : reinterpret_cast<const char *>(ta_zeros);
-#pragma unroll
-            for (int i = 0; i < 9; i++) {
-                const char *src = p + 32 * (8 * i + (lane & 7));
-                if (!FULL && 8 * (8 * i + (lane & 7)) >= CW) src = reinterpret_cast<const char *>(ta_zeros);
-                R[2 * i] = *reinterpret_cast<const f4 *>(src);
-                R[2 * i + 1] = *reinterpret_cast<const f4 *>(src + 16);
-            }
-            find_rows();
+        auto load = [&](int g) __attribute__((always_inline)) {
+            glb_cchar *at = src + 256 * g;
+            if (!FULL && 64 * g + 4 * c16 >= CW) at = (glb_cchar *)ta_zeros;
+            R[g] = *(const __attribute__((address_space(1))) f4 *)at;
         };
-        // the row in registers to LDS in ten pieces: its scale, then a column group each
+        // the row's scale, from its largest value
         float scale = 0.0f;
-        auto put_piece = [&](int s, int i) __attribute__((always_inline)) {
+        auto scale_row = [&](int s) __attribute__((always_inline)) {
             const int buf = s & 1;
-            if (i == 0) {
-                uint32_t m = 0;
+            float m = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 18; x++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(R[x][e]) & 0x7fffffffu);
-#pragma unroll
-                for (int o = 4; o >= 1; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-                // a node's row that holds an infinity or a NaN: zeros, and noted, so that the query rows that see
-                // it become NaN and no others
-                const bool bad = m >= 0x7f800000u && s * TB_TP + prow >= len;
-                const int k = row_scale(m);
-                scale = bad ? 0.0f : __uint_as_float((uint32_t)(127 + k) << 23);
-                s_k[32 * buf + prow] = k;   // eight lanes the same
-                s_ok[8 * buf + wv] = (uint8_t)gather_rows(__ballot(rok));
-                s_ok[8 * buf + 4 + wv] = (uint8_t)gather_rows(__ballot(bad));
-            } else {
-                const f4 u = R[2 * i - 2], v = R[2 * i - 1];
-                const float x[8] = {u.x * scale, u.y * scale, u.z * scale, u.w * scale, v.x * scale, v.y * scale, v.z * scale, v.w * scale};
-                f16x8 hi, lo;
-                split16(x, hi, lo);
-                if (scale == 0.0f) hi = lo = f16x8(0);
-                char *at = smem + buf * TS_BUF + TB_GRP * (i - 1) + 128 * prow + 16 * lu;
-                *reinterpret_cast<f16x8 *>(at) = hi;
-                *reinterpret_cast<f16x8 *>(at + TB_BUF) = lo;
+            for (int g = 0; g < 9; g++) {
+                m = max_abs(m, R[g].x, R[g].y);
+                m = max_abs(m, R[g].z, R[g].w);
             }
+            m = dpp_max<0x121>(m);   // row_ror 1, 2, 4, 8: over the row's sixteen lanes
+            m = dpp_max<0x122>(m);
+            m = dpp_max<0x124>(m);
+            m = dpp_max<0x128>(m);
+            uint32_t bits = 0;
+            // a node's row that holds an infinity or a NaN: zeros, and noted, so that the query rows that see
+            // it become NaN and no others
+            if ((s + 1) * TB_TP > len) {
+                bool bad = false;
+#pragma unroll
+                for (int g = 0; g < 9; g++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) bad |= (__float_as_uint(R[g][e]) & 0x7f800000u) == 0x7f800000u;
+                bad &= s * TB_TP + prow >= len;
+                const uint64_t any = __ballot(bad);
+#pragma unroll
+                for (int r = 0; r < 4; r++) bits |= any >> (16 * r) & 0xffff ? 1u << r : 0u;
+                if (bits >> kq & 1)
+#pragma unroll
+                    for (int g = 0; g < 9; g++) R[g] = 0.0f;
+            }
+            const int k = row_scale(__float_as_uint(m));
+            scale = __uint_as_float((uint32_t)(127 + k) << 23);
+            s_k[32 * buf + prow] = k;   // sixteen lanes the same
+            s_ok[16 * buf + wv] = (uint8_t)gather_rows16(__ballot(rok));
+            s_ok[16 * buf + 8 + wv] = (uint8_t)bits;
         };
-        find_rows();
-        load_rows();
+        // a column group of it to LDS
+        auto put = [&](int s, int g, int sa) __attribute__((always_inline)) {
+            const float x[4] = {R[g].x * scale, R[g].y * scale, R[g].z * scale, R[g].w * scale};
+            f16x4 hi, lo;
+            split16(x, hi, lo);
+            char *at = smem + (s & 1) * TS_BUF + TB_GRP * g + sa;
+            *reinterpret_cast<f16x4 *>(at) = hi;
+            *reinterpret_cast<f16x4 *>(at + TB_BUF) = lo;
+        };
+        next_row();
+#pragma unroll
+        for (int g = 0; g < 9; g++) load(g);
+        next_row();
 
-        // query fragments: unit 4 ks + kq of the row, scaled and split alike
+        // query fragments, scaled and split alike: channels 32 kstep(ks) + 8 kq .. + 7 of the row
+        auto kstep = [&](int ks) __attribute__((always_inline)) { return ks < 8 ? 8 * half + ks : 16 + half; };
         f16x8 qh[KS], ql[KS];
-        float qscale;
+        float qscale;   // of the scores of this half
         {
-            const float *src = reinterpret_cast<const float *>(a.q) + ((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW;
-            uint32_t m = 0;
+            glb_cchar *src = (glb_cchar *)a.q + (((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW + 8 * kq) * 4;
+            f4 x[2 * KS];
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                if (row < rows && (FULL || 8 * (4 * ks + kq) < CW))
+            for (int i = 0; i < 2 * KS; i++) {
+                glb_cchar *at = src + 128 * kstep(i >> 1) + 16 * (i & 1);
+                if (!FULL && 32 * kstep(i >> 1) + 8 * kq >= CW) at = (glb_cchar *)ta_zeros;
+                x[i] = *(const __attribute__((address_space(1))) f4 *)at;
+            }
+            float m = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 8; e += 4) {
-                        const f4 v = *reinterpret_cast<const f4 *>(src + 8 * (4 * ks + kq) + e);
-#pragma unroll
-                        for (int x = 0; x < 4; x++) m = max(m, __float_as_uint(v[x]) & 0x7fffffffu);
-                    }
-            m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-            m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-            const int k = row_scale(m);
+            for (int i = 0; i < 2 * KS; i++) {
+                m = max_abs(m, x[i].x, x[i].y);
+                m = max_abs(m, x[i].z, x[i].w);
+            }
+            m = quarter_max(m);
+            const int k = row_scale(__float_as_uint(m));
             const float sc = __uint_as_float((uint32_t)(127 + k) << 23);
             qscale = ldexpf(a.scale2, -k);
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                if (row < rows && (FULL || 8 * (4 * ks + kq) < CW))
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = src[8 * (4 * ks + kq) + e] * sc;
-                split16(x, qh[ks], ql[ks]);
+                const f4 u = x[2 * ks] * sc, v = x[2 * ks + 1] * sc;
+                const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                split16(y, qh[ks], ql[ks]);
             }
         }
 
-        const int pi = 4 * (c16 & 3) + (c16 >> 2), vr = 4 * ((lane >> 2) & 3) + kq;
-        const int ka = 128 * pi + 16 * (kq ^ ((pi >> 1) & 6));
-        const int va = 128 * vr + 16 * (((lane >> 1) & 1) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
-        auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {   // block f % 2 of K-step f / 2
-            return *(const __attribute__((address_space(3))) f16x8 *)(buf + (ka ^ (f & 2 ? 64 : 0)) + TB_GRP * (f >> 2) + 2048 * (f & 1));
+        // LDS places, worked out from the lane anew in every step: staged channels, fragments of the scores'
+        // K-steps and of the half's last, of the sum
+        auto put_at = [&](int t) __attribute__((always_inline)) {
+            const int r = 4 * wv + (t >> 4 & 3), u = t >> 1 & 7;
+            return 128 * r + 16 * (u ^ ((r >> 1) & 6)) + 8 * (t & 1);
         };
-        auto vread = [&](lds_cchar *buf, int d) __attribute__((always_inline)) {
+        auto key_at = [&](int t, int first) __attribute__((always_inline)) {
+            const int r = 4 * (t & 3) + (t >> 2 & 3);
+            return 128 * r + 16 * (((t >> 4 & 3) + first) ^ ((r >> 1) & 6));
+        };
+        auto sum_at = [&](int t) __attribute__((always_inline)) {
+            const int r = 4 * (t >> 2 & 3) + (t >> 4 & 3);
+            return 128 * r + 16 * ((t >> 1 & 1) ^ ((r >> 1) & 6)) + 8 * (t & 1) + 4 * half * TB_GRP;
+        };
+        auto kread = [&](lds_cchar *buf, int f, int ka, int kb) __attribute__((always_inline)) {   // block f % 2 of K-step f / 2
+            lds_cchar *at = f < 16 ? buf + (ka ^ (f & 2 ? 64 : 0)) + 4 * half * TB_GRP + TB_GRP * (f >> 2) : buf + kb + 8 * TB_GRP;
+            return *(const __attribute__((address_space(3))) f16x8 *)(at + 2048 * (f & 1));
+        };
+        auto vread = [&](lds_cchar *buf, int d, int va) __attribute__((always_inline)) {
             lds_cchar *at = buf + (va ^ (32 * (d & 3))) + TB_GRP * (d >> 2);
             const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
             const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
             const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
             return __builtin_bit_cast(f16x8, uint4{y0.x, y0.y, y1.x, y1.y});
         };
+        // A wave hands its half of the scores over where its partner will stage rows of the next step: nothing
+        // is read there any more, and the partner, which reads them, is the only one to write there next.
+        auto half_at = [&](int s, int w, int i) __attribute__((always_inline)) {
+            return reinterpret_cast<f4 *>(smem + ((s + 1) & 1) * TS_BUF + TB_GRP * (2 * i + (lane >> 5)) + 512 * w + 16 * (lane & 31));
+        };
         f32x4 acc[DT];
         float M = -INFINITY, lsum = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) acc[d] = 0.0f;
+        if (tid < 64) s_anc[lane] = tree_ancestors(par);
+        scale_row(s0);
 #pragma unroll
-        for (int i = 0; i < 10; i++) put_piece(s0, i);
-        load_rows();
+        for (int g = 0; g < 9; g++) {
+            put(s0, g, put_at(tid));
+            load(g);
+        }
+        next_row();
+        lds_barrier();
 
         for (int s = s0; s < s1; s++) {
-            __syncthreads();   // step s is staged, step s - 1 read
             lds_cchar *cur = (lds_cchar *)smem + (s & 1) * TS_BUF;
-            constexpr int AK = 4, AV = 4;   // fragment pairs read ahead
+            const int ka = key_at(opaque(tid), 0), kb = key_at(opaque(tid), 4 * half), sa = put_at(opaque(tid));
+            constexpr int AK = 3, AV = 2;   // fragment pairs read ahead
             f16x8 kh[AK], kl[AK];
             f32x4 S[2], Sl[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) S[i] = Sl[i] = 0.0f;
 #pragma unroll
             for (int f = 0; f < AK; f++) {
-                kh[f] = kread(cur, f);
-                kl[f] = kread(cur + TB_BUF, f);
+                kh[f] = kread(cur, f, ka, kb);
+                kl[f] = kread(cur + TB_BUF, f, ka, kb);
             }
 #pragma unroll
             for (int f = 0; f < 2 * KS; f++) {
@@ -885,37 +963,55 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
                 Sl[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, ql[f >> 1], Sl[f & 1], 0, 0, 0);
                 Sl[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l, qh[f >> 1], Sl[f & 1], 0, 0, 0);
                 if (f + AK < 2 * KS) {
-                    kh[f % AK] = kread(cur, f + AK);
-                    kl[f % AK] = kread(cur + TB_BUF, f + AK);
+                    kh[f % AK] = kread(cur, f + AK, ka, kb);
+                    kl[f % AK] = kread(cur + TB_BUF, f + AK, ka, kb);
                 }
-                if (f >= 4 && f < 34 && (f - 4) % 3 == 0) put_piece(s + 1, (f - 4) / 3);   // past the end: rows of zeros
+                // step s + 1 (past the end: rows of zeros), and the loads of step s + 2
+                if (f == 1) scale_row(s + 1);
+                if (f >= 5 && f < 15 && (f & 1)) {
+                    put(s + 1, f / 2 + 2, sa);
+                    load(f / 2 + 2);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            load_rows();   // of step s + 2
-            // scores in base 2 with their rows' scales, masks, softmax
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                S[i] = (S[i] + Sl[i]) * qscale;
+                *half_at(s, wv ^ 4, i) = f4{S[i][0], S[i][1], S[i][2], S[i][3]};
+            }
+            lds_barrier();
+            const int va = sum_at(opaque(tid));
+            f16x8 vh[AV], vl[AV];
             int k[8];
             float y[8];
-            const uint32_t *okw = reinterpret_cast<const uint32_t *>(s_ok) + 2 * (s & 1);
-            const uint32_t ok = okw[0], bad = okw[1];
+            f4 other[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) other[i] = *half_at(s, wv, i);
+            const uint64_t *okw = reinterpret_cast<const uint64_t *>(s_ok) + 2 * (s & 1);
+            const uint64_t ok = okw[0], bad = okw[1];
+#pragma unroll
+            for (int x = 0; x < 8; x++) k[x] = s_k[32 * (s & 1) + 16 * (x >> 2) + 4 * (x & 3) + kq];
+#pragma unroll
+            for (int d = 0; d < AV; d++) {
+                vh[d] = vread(cur, d, va);
+                vl[d] = vread(cur + TB_BUF, d, va);
+            }
+            // scores in base 2 with their rows' scales, masks, softmax
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    k[4 * i + e] = s_k[32 * (s & 1) + 16 * i + 4 * e + kq];
-                    y[4 * i + e] = ldexpf((S[i][e] + Sl[i][e]) * qscale, -k[4 * i + e]);
-                }
-            if (ok != 0xffffffffu || (s + 1) * TB_TP > len) {
+                for (int e = 0; e < 4; e++) y[4 * i + e] = ldexpf(S[i][e] + other[i][e], -k[4 * i + e]);
+            if (ok != 0x0f0f0f0f0f0f0f0full || (s + 1) * TB_TP > len) {
                 const int n0 = len - s * TB_TP;   // place of the first node in the step
                 const uint64_t anc = s_anc[row < rows ? row / H : 0];
                 uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
                 if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc << n0);
                 else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc >> -n0);
-                w &= ok;
 #pragma unroll
                 for (int x = 0; x < 8; x++) {
-                    const int bit = 16 * (x >> 2) + 4 * (x & 3) + kq;
-                    const float seen = bad >> bit & 1 ? NAN : 0.0f;
-                    y[x] = w >> bit & 1 ? y[x] + seen : -INFINITY;
+                    const int bit = 16 * (x >> 2) + 4 * (x & 3) + kq, byte = 8 * (4 * (x >> 2) + (x & 3)) + kq;
+                    const float seen = bad >> byte & 1 ? NAN : 0.0f;
+                    y[x] = (w >> bit & 1) && (ok >> byte & 1) ? y[x] + seen : -INFINITY;
                 }
             }
             float mt = -INFINITY;
@@ -939,12 +1035,6 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
                 lsum += ldexpf(pw[x], k[x]);
             }
             split16(pw, ph, pl);
-            f16x8 vh[AV], vl[AV];
-#pragma unroll
-            for (int d = 0; d < AV; d++) {
-                vh[d] = vread(cur, d);
-                vl[d] = vread(cur + TB_BUF, d);
-            }
 #pragma unroll
             for (int d = 0; d < DT; d += 2) {
 #pragma unroll
@@ -956,40 +1046,47 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
                 if (d + AV < DT)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        vh[(d + i) % AV] = vread(cur, d + i + AV);
-                        vl[(d + i) % AV] = vread(cur + TB_BUF, d + i + AV);
+                        vh[(d + i) % AV] = vread(cur, d + i + AV, va);
+                        vl[(d + i) % AV] = vread(cur + TB_BUF, d + i + AV, va);
                     }
+                if (d < 8) {
+                    put(s + 1, d / 2, sa);
+                    load(d / 2);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            next_row();
+            lds_barrier();
         }
         lsum += __shfl_xor(lsum, 16, 64);
         lsum += __shfl_xor(lsum, 32, 64);
 
         if (row >= rows) continue;
         const size_t orow = (size_t)b * a.t.N * H + row, part = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
+        const int ch = 16 * DT * half + 4 * kq;   // this lane's first channels
         if (split) {
-            if (kq == 0) {
+            if (kq == 0 && half == 0) {
                 a.pm[part] = M;
                 a.pl[part] = lsum;
             }
             if (M == -INFINITY) continue;   // nothing seen: the merge does not read its sums
-            float *dst = a.po + part * KL + 4 * kq;
+            float *dst = a.po + part * KL + ch;
 #pragma unroll
             for (int d = 0; d < DT; d++)
-                if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d];
+                if (16 * d + ch < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d];
         } else {
-            if (kq == 0 && a.lse) a.lse[orow] = lsum == 0.0f ? -INFINITY : (M - TS_UP + __builtin_amdgcn_logf(lsum)) * TA_LN2;
+            if (kq == 0 && half == 0 && a.lse) a.lse[orow] = lsum == 0.0f ? -INFINITY : (M - TS_UP + __builtin_amdgcn_logf(lsum)) * TA_LN2;
             const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
             if (a.o_dt == K3HIP_F32) {
-                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * kq;
+                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + ch;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + 4 * kq < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d] * inv;
+                    if (16 * d + ch < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d] * inv;
             } else {
-                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * kq;
+                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + ch;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + 4 * kq < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d] * inv);
+                    if (16 * d + ch < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d] * inv);
             }
         }
     }
@@ -1203,7 +1300,7 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     else kern = rows == 64 ? (const void *)tree_attn16_kernel<false, 1> : (const void *)tree_attn16_kernel<false, 2>;
     K3_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *args[] = {&a};
-    K3_HIP(hipLaunchKernel(kern, dim3((unsigned)grid), dim3(TA_NT), args, lds, st));
+    K3_HIP(hipLaunchKernel(kern, dim3((unsigned)grid), dim3(f32 ? TS_NT : TA_NT), args, lds, st));
     K3_LAUNCHED();
     const float up = f32 ? TS_UP : 0.0f;
     if ((long)B * N * H <= 2048)
