@@ -156,11 +156,12 @@ __device__ __forceinline__ float dpp_max(float x)
     return fmaxf(x, __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), C, 0xf, 0xf, true)));
 }
 
-// The largest of m, |x| and |y| (NaNs are passed over), in one instruction: left to the compiler, values from
-// memory are each made canonical first. The wait states are those of a DPP read behind it.
-__device__ __forceinline__ float max_abs(float m, float x, float y)
+// The largest of m and the magnitudes of x and y (NaNs are passed over), two values an instruction: left to
+// the compiler, values from memory are each made canonical first.
+__device__ __forceinline__ float max_abs(float m, const f4 &x, const f4 &y)
 {
-    asm("v_max3_f32 %0, %0, |%1|, |%2|\n\ts_nop 1" : "+v"(m) : "v"(x), "v"(y));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|\n\tv_max3_f32 %0, %0, |%3|, |%4|\n\tv_max3_f32 %0, %0, |%5|, |%6|\n\tv_max3_f32 %0, %0, |%7|, |%8|"
+        : "+v"(m) : "v"(x.x), "v"(x.y), "v"(x.z), "v"(x.w), "v"(y.x), "v"(y.y), "v"(y.z), "v"(y.w));
     return m;
 }
 
@@ -725,19 +726,17 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // products: groups 4 .. 8 beside the scores, where groups 0 .. 3 of the buffer carry the halves, those beside the sum.
 constexpr int TS_BUF = 2 * TB_BUF;
 constexpr int TS_NT = 512;
-constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 4 + 64 + TREE_MAX * 8;
+constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 8 + 64 + TREE_MAX * 8;
 constexpr float TS_UP = 7.0f;     // log2 of the weight of the reference
 static_assert(TS_LDS <= 160 * 1024, "LDS");
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-template <int N, typename V>
-__device__ __forceinline__ void split16(const float (&x)[N], V &hi, V &lo)
+__device__ __forceinline__ void split16(const float (&x)[8], f16x8 &hi, f16x8 &lo)
 {
 #pragma unroll
-    for (int e = 0; e < N; e += 2) {
+    for (int e = 0; e < 8; e += 2) {
         const f16x2 h = __builtin_convertvector(f2{x[e], x[e + 1]}, f16x2);
         const f16x2 l = __builtin_convertvector(f2{x[e] - (float)h[0], x[e + 1] - (float)h[1]}, f16x2);
         hi[e] = h[0];
@@ -745,6 +744,23 @@ __device__ __forceinline__ void split16(const float (&x)[N], V &hi, V &lo)
         lo[e] = l[0];
         lo[e + 1] = l[1];
     }
+}
+
+// The same of x times a power of two, a product and its rounding in one instruction. Between two that write halves of a
+// register, or one that writes and one that reads it, stands another.
+__device__ __forceinline__ void split4(const f4 &x, float scale, uint2 &hi, uint2 &lo)
+{
+    asm("v_fma_mixlo_f16 %0, %4, %8, 0\n\t"
+        "v_fma_mixlo_f16 %1, %6, %8, 0\n\t"
+        "v_fma_mixhi_f16 %0, %5, %8, 0\n\t"
+        "v_fma_mixhi_f16 %1, %7, %8, 0\n\t"
+        "v_fma_mixlo_f16 %2, %4, %8, -%0 op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixlo_f16 %3, %6, %8, -%1 op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %2, %5, %8, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %3, %7, %8, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "s_nop 0"
+        : "=&v"(hi.x), "=&v"(hi.y), "=&v"(lo.x), "=&v"(lo.y)
+        : "v"(x.x), "v"(x.y), "v"(x.z), "v"(x.w), "v"(scale));
 }
 
 // The power of two that a row whose largest magnitude has these bits is scaled by.
@@ -764,7 +780,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 {
     constexpr int ROWS = 64, DT = TA_KL / 32, KS = TA_CW / 64;   // a wave's halves
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int *s_k = reinterpret_cast<int *>(smem + 2 * TS_BUF);               // [buffer][row] its scale
+    f2 *s_k = reinterpret_cast<f2 *>(smem + 2 * TS_BUF);                 // [buffer][row] of its scale 2^k: 2^-k, k
     uint8_t *s_ok = reinterpret_cast<uint8_t *>(s_k + 64);               // [buffer][seen, not finite][wave] a bit a row
     uint64_t *s_anc = reinterpret_cast<uint64_t *>(s_ok + 64);           // [node] its ancestors
 
@@ -819,14 +835,13 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         };
         // the row's scale, from its largest value
         float scale = 0.0f;
-        auto scale_row = [&](int s) __attribute__((always_inline)) {
-            const int buf = s & 1;
-            float m = 0.0f;
+        auto largest = [&](float &m, int i) __attribute__((always_inline)) {   // in three pieces
 #pragma unroll
-            for (int g = 0; g < 9; g++) {
-                m = max_abs(m, R[g].x, R[g].y);
-                m = max_abs(m, R[g].z, R[g].w);
-            }
+            for (int g = 4 * i; g < min(4 * i + 4, 9); g += 2) m = max_abs(m, R[g], R[min(g + 1, 8)]);
+        };
+        auto scale_row = [&](int s, float m) __attribute__((always_inline)) {
+            const int buf = s & 1;
+            asm volatile("s_nop 1" : "+v"(m));   // the compiler does not see that a vector instruction wrote what DPP reads
             m = dpp_max<0x121>(m);   // row_ror 1, 2, 4, 8: over the row's sixteen lanes
             m = dpp_max<0x122>(m);
             m = dpp_max<0x124>(m);
@@ -850,18 +865,17 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             }
             const int k = row_scale(__float_as_uint(m));
             scale = __uint_as_float((uint32_t)(127 + k) << 23);
-            s_k[32 * buf + prow] = k;   // sixteen lanes the same
+            s_k[32 * buf + 4 * wv + (opaque(tid) >> 4 & 3)] = f2{__uint_as_float((uint32_t)(127 - k) << 23), (float)k};   // sixteen lanes the same
             s_ok[16 * buf + wv] = (uint8_t)gather_rows16(__ballot(rok));
             s_ok[16 * buf + 8 + wv] = (uint8_t)bits;
         };
         // a column group of it to LDS
         auto put = [&](int s, int g, int sa) __attribute__((always_inline)) {
-            const float x[4] = {R[g].x * scale, R[g].y * scale, R[g].z * scale, R[g].w * scale};
-            f16x4 hi, lo;
-            split16(x, hi, lo);
+            uint2 hi, lo;
+            split4(R[g], scale, hi, lo);
             char *at = smem + (s & 1) * TS_BUF + TB_GRP * g + sa;
-            *reinterpret_cast<f16x4 *>(at) = hi;
-            *reinterpret_cast<f16x4 *>(at + TB_BUF) = lo;
+            *reinterpret_cast<uint2 *>(at) = hi;
+            *reinterpret_cast<uint2 *>(at + TB_BUF) = lo;
         };
         next_row();
 #pragma unroll
@@ -883,10 +897,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             }
             float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2 * KS; i++) {
-                m = max_abs(m, x[i].x, x[i].y);
-                m = max_abs(m, x[i].z, x[i].w);
-            }
+            for (int i = 0; i < 2 * KS; i += 2) m = max_abs(m, x[i], x[i + 1]);
             m = quarter_max(m);
             const int k = row_scale(__float_as_uint(m));
             const float sc = __uint_as_float((uint32_t)(127 + k) << 23);
@@ -926,15 +937,18 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         };
         // A wave hands its half of the scores over where its partner will stage rows of the next step: nothing
         // is read there any more, and the partner, which reads them, is the only one to write there next.
-        auto half_at = [&](int s, int w, int i) __attribute__((always_inline)) {
-            return reinterpret_cast<f4 *>(smem + ((s + 1) & 1) * TS_BUF + TB_GRP * (2 * i + (lane >> 5)) + 512 * w + 16 * (lane & 31));
+        auto half_at = [&](int s, int w, int i, int t) __attribute__((always_inline)) {
+            return reinterpret_cast<f4 *>(smem + ((s + 1) & 1) * TS_BUF + TB_GRP * 2 * i + (t >> 5 & 1) * TB_GRP + 512 * w + 16 * (t & 31));
         };
         f32x4 acc[DT];
         float M = -INFINITY, lsum = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++) acc[d] = 0.0f;
         if (tid < 64) s_anc[lane] = tree_ancestors(par);
-        scale_row(s0);
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 3; i++) largest(most, i);
+        scale_row(s0, most);
 #pragma unroll
         for (int g = 0; g < 9; g++) {
             put(s0, g, put_at(tid));
@@ -945,8 +959,8 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 
         for (int s = s0; s < s1; s++) {
             lds_cchar *cur = (lds_cchar *)smem + (s & 1) * TS_BUF;
-            const int ka = key_at(opaque(tid), 0), kb = key_at(opaque(tid), 4 * half), sa = put_at(opaque(tid));
-            constexpr int AK = 3, AV = 2;   // fragment pairs read ahead
+            const int st = opaque(tid), ka = key_at(st, 0), kb = key_at(st, 4 * half), sa = put_at(st);
+            constexpr int AK = 2, AV = 2;   // fragment pairs read ahead
             f16x8 kh[AK], kl[AK];
             f32x4 S[2], Sl[2];
 #pragma unroll
@@ -956,67 +970,83 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
                 kh[f] = kread(cur, f, ka, kb);
                 kl[f] = kread(cur + TB_BUF, f, ka, kb);
             }
+            most = 0.0f;
 #pragma unroll
-            for (int f = 0; f < 2 * KS; f++) {
-                const f16x8 h = kh[f % AK], l = kl[f % AK];
-                S[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, qh[f >> 1], S[f & 1], 0, 0, 0);
-                Sl[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, ql[f >> 1], Sl[f & 1], 0, 0, 0);
-                Sl[f & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l, qh[f >> 1], Sl[f & 1], 0, 0, 0);
-                if (f + AK < 2 * KS) {
-                    kh[f % AK] = kread(cur, f + AK, ka, kb);
-                    kl[f % AK] = kread(cur + TB_BUF, f + AK, ka, kb);
+            for (int f = 0; f < 2 * KS; f += 2) {   // both blocks of a K-step
+                f16x8 h[2], l[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    h[i] = kh[(f + i) % AK];
+                    l[i] = kl[(f + i) % AK];
                 }
+#pragma unroll
+                for (int i = 0; i < 2; i++) S[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[i], qh[f >> 1], S[i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 2; i++) Sl[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[i], ql[f >> 1], Sl[i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 2; i++) Sl[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[i], qh[f >> 1], Sl[i], 0, 0, 0);
+                if (f + AK < 2 * KS)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        kh[(f + i) % AK] = kread(cur, f + i + AK, ka, kb);
+                        kl[(f + i) % AK] = kread(cur + TB_BUF, f + i + AK, ka, kb);
+                    }
                 // step s + 1 (past the end: rows of zeros), and the loads of step s + 2
-                if (f == 1) scale_row(s + 1);
-                if (f >= 5 && f < 15 && (f & 1)) {
-                    put(s + 1, f / 2 + 2, sa);
-                    load(f / 2 + 2);
+                if (f < 6) largest(most, f / 2);
+                if (f == 6) scale_row(s + 1, most);
+                if (f >= 8) {
+                    put(s + 1, f / 2, sa);
+                    load(f / 2);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            const int ht = opaque(tid);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 S[i] = (S[i] + Sl[i]) * qscale;
-                *half_at(s, wv ^ 4, i) = f4{S[i][0], S[i][1], S[i][2], S[i][3]};
+                asm volatile("" : "+v"(S[i]));   // rounded here, as its partner gets it: both have to come to the same bits
+                *half_at(s, wv ^ 4, i, ht) = f4{S[i][0], S[i][1], S[i][2], S[i][3]};
             }
-            lds_barrier();
-            const int va = sum_at(opaque(tid));
+            const int va = sum_at(ht);
             f16x8 vh[AV], vl[AV];
-            int k[8];
-            float y[8];
-            f4 other[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) other[i] = *half_at(s, wv, i);
-            const uint64_t *okw = reinterpret_cast<const uint64_t *>(s_ok) + 2 * (s & 1);
-            const uint64_t ok = okw[0], bad = okw[1];
-#pragma unroll
-            for (int x = 0; x < 8; x++) k[x] = s_k[32 * (s & 1) + 16 * (x >> 2) + 4 * (x & 3) + kq];
 #pragma unroll
             for (int d = 0; d < AV; d++) {
                 vh[d] = vread(cur, d, va);
                 vl[d] = vread(cur + TB_BUF, d, va);
             }
-            // scores in base 2 with their rows' scales, masks, softmax
+            f2 k[8];
+            const f2 *ks = s_k + 32 * (s & 1) + (ht >> 4 & 3);
+#pragma unroll
+            for (int x = 0; x < 8; x++) k[x] = ks[16 * (x >> 2) + 4 * (x & 3)];
+            const uint64_t *okw = reinterpret_cast<const uint64_t *>(s_ok) + 2 * (s & 1);
+            const uint64_t ok = okw[0], bad = okw[1];
+            lds_barrier();
+            float y[8];   // scores in base 2 less k
+            f4 other[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) other[i] = *half_at(s, wv, i, ht);
+            // scores with their rows' scales, masks, softmax
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[4 * i + e] = ldexpf(S[i][e] + other[i][e], -k[4 * i + e]);
+                for (int e = 0; e < 4; e++) y[4 * i + e] = __builtin_fmaf(S[i][e] + other[i][e], k[4 * i + e].x, -k[4 * i + e].y);
             if (ok != 0x0f0f0f0f0f0f0f0full || (s + 1) * TB_TP > len) {
                 const int n0 = len - s * TB_TP;   // place of the first node in the step
+                const int q4 = opaque(tid) >> 4 & 3, row = r0 + 16 * (wv & 3) + (opaque(tid) & 15);
                 const uint64_t anc = s_anc[row < rows ? row / H : 0];
                 uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
                 if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc << n0);
                 else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc >> -n0);
 #pragma unroll
                 for (int x = 0; x < 8; x++) {
-                    const int bit = 16 * (x >> 2) + 4 * (x & 3) + kq, byte = 8 * (4 * (x >> 2) + (x & 3)) + kq;
+                    const int bit = 16 * (x >> 2) + 4 * (x & 3) + q4, byte = 8 * (4 * (x >> 2) + (x & 3)) + q4;
                     const float seen = bad >> byte & 1 ? NAN : 0.0f;
                     y[x] = (w >> bit & 1) && (ok >> byte & 1) ? y[x] + seen : -INFINITY;
                 }
             }
             float mt = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 8; x++) mt = fmaxf(mt, y[x] - (float)k[x]);
+            for (int x = 0; x < 8; x++) mt = fmaxf(mt, y[x]);
             mt = quarter_max(mt);
             if (__ballot(mt > M + TA_LAZY)) {
                 const float mn = mt > M + TA_LAZY ? mt : M;
@@ -1031,8 +1061,8 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             float pw[8];
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                pw[x] = __builtin_amdgcn_exp2f(y[x] - (float)k[x] - ref);
-                lsum += ldexpf(pw[x], k[x]);
+                pw[x] = __builtin_amdgcn_exp2f(y[x] - ref);
+                lsum = __builtin_fmaf(pw[x], __uint_as_float(0x7f000000u - __float_as_uint(k[x].x)), lsum);   // times 2^k
             }
             split16(pw, ph, pl);
 #pragma unroll
@@ -1053,9 +1083,9 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
                     put(s + 1, d / 2, sa);
                     load(d / 2);
                 }
+                if (d == 8) next_row();
                 __builtin_amdgcn_sched_barrier(0);
             }
-            next_row();
             lds_barrier();
         }
         lsum += __shfl_xor(lsum, 16, 64);
