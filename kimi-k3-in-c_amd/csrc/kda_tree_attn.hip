@@ -8,26 +8,23 @@
 // Every head of every node reads the same rows, so a sequence is one product of (nodes x heads) rows with
 // its cache: bytes bind for one node, the matrix cores from a few nodes on.
 //
-//  * A workgroup (four waves, one a SIMD) owns a tile of query rows and a range of positions and walks it
-//    in tiles of 64 (bf16) or 32 (fp32) positions, staged as they lie by loads that write LDS directly,
-//    two buffers, one barrier a tile. Rows that have no page, or lie past the last node, are staged as zeros.
-//  * A wave owns 16 NR query rows (RG such groups a workgroup) and the tile's 16-row blocks of its
-//    position group (PG of them): scores^T (positions x query rows), the online softmax in base 2 and
-//    o^T (latent channels x query rows) += latents^T . p. With the query row in the column, a softmax
-//    row is a lane: its max, its sum, its rescale and its mask are per-lane values, and p goes from the score
-//    product's output layout into the second product's operand without leaving the lane. Position groups
-//    are merged through LDS at the end.
+//  * A workgroup owns a tile of query rows and a range of steps of 32 positions, which it walks once; all
+//    sequences' steps stand on one axis that is cut into equal ranges, one for as many workgroups as the largest
+//    sequence has row tiles (find_slot). A range that ends inside a sequence leaves unnormalised sums with (M, l); a
+//    second launch merges them in order, so results do not depend on timing.
+//  * Scores^T (positions x query rows), the softmax in base 2 and o^T (latent channels x query rows) += latents^T . p.
+//    With the query row in the column, a softmax row is a lane: its max, its sum, its rescale and its mask are
+//    per-lane values, and p goes from the score product's output layout into the second product's operand
+//    without leaving the lane.
 //  * The 16 rows of a block stand in the score product in the order 4 (m % 4) + m / 4, so that the four
-//    positions a lane quarter ends up with are four rows apart: its transposed reads (bf16,
-//    ds_read_b64_tr_b16) and the 16-byte reads of the score product then both fall on distinct banks, with
-//    16-byte unit u of row r at u ^ ((r / 2) % 8) (bf16) or u ^ (r % 16) (fp32).
-//  * fp32 runs on v_mfma_f32_16x16x4_f32.
-//  * The reference max of a row moves only when a score passes it by AT_LAZY, so sums are rescaled rarely.
-//  * Ranges of a sequence leave unnormalised sums with (M, l); a second launch merges them in order.
+//    positions a lane quarter ends up with are four rows apart, which is what the transposed reads of the second
+//    product (ds_read_b64_tr_b16) hand out. A step is staged as column groups [32 rows][8 units of 16 bytes] with
+//    unit u of row r at u ^ ((r / 2) & 6): free of bank conflicts for these and for the 16-byte reads of the
+//    score product (of the 64 lanes, 0-3, 12-15, 20-27 go together, and so on).
+//  * The reference max of a row moves only when a score passes it by TA_LAZY, so sums are rescaled rarely.
 //
-// What a row does not see cannot reach it: masked scores are selected away, and where a masked position
-// of a tile holds an infinity or a NaN (its scores show it) the tile's sum is taken position by position
-// instead of by the product, whose zero weights would still spread it.
+// What a row does not see cannot reach it: masked scores are selected away, and a node's row that holds an
+// infinity or a NaN is staged as zeros and noted; the query rows that see it become NaN.
 #include <math.h>
 
 #include <algorithm>
@@ -76,64 +73,48 @@ struct AttnArgs {
 
 // The 16x16x32 MFMAs of the bf16 kernel. With 32 query rows a wave the second product's 256 accumulators fill
 // the accumulation registers: with the builtin the compiler moves them between the register files and
-// spills hundreds, so ASM issues the instruction itself, acc tied to its registers, everything else in
-// ordinary ones. The compiler then knows no MFMA; wait() stands where it would have put wait states.
-template <bool ASM>
+// spills hundreds (with 16 rows it moves a hundred a step), so the instruction is issued by itself, acc tied to its
+// registers, everything else in ordinary ones. The compiler then knows no MFMA; wait() stands where it would
+// have put wait states.
 __device__ __forceinline__ void mfma_acc(const bf16x8 &a, const bf16x8 &b, f32x4 &c)
 {
-    if constexpr (ASM) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-    else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
 // In ordinary registers; both operands come from memory (of a vector instruction's result it would have to wait).
-template <bool ASM>
 __device__ __forceinline__ void mfma_vec(const bf16x8 &a, const bf16x8 &b, f32x4 &c, bool first)
 {
-    if constexpr (ASM) {
-        if (first) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
-        else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
-    } else {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, first ? f32x4(0.0f) : c, 0, 0, 0);
-    }
+    if (first) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+    else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
 
 // c += column sums of b; b, c and the ones may have been written just before, b is ready for others after it.
-template <bool ASM>
 __device__ __forceinline__ void mfma_sum(bf16x8 &b, f32x4 &c)
 {
     const bf16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-    if constexpr (ASM) asm volatile("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %1, %0" : "+v"(c), "+v"(b) : "v"(ones));
-    else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b, c, 0, 0, 0);
+    asm volatile("s_nop 3\n\tv_mfma_f32_16x16x32_bf16 %0, %2, %1, %0" : "+v"(c), "+v"(b) : "v"(ones));
 }
 
 // Ten wait states, between MFMAs and other instructions on their results (eight are needed for this one) or
 // between other instructions' results and MFMAs on them; nothing is scheduled across.
-template <bool ASM>
 __device__ __forceinline__ void wait()
 {
-    if constexpr (ASM) {
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_nop 9");
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 9");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // c *= m, a register at a time through one ordinary register (left to the compiler, all of them are brought
 // over at once and spill).
-template <bool ASM>
 __device__ __forceinline__ void acc_scale(f32x4 &c, float m)
 {
-    if constexpr (ASM) {
-        float t;
+    float t;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float v = c[e];
-            asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
-                         : "+a"(v), "=&v"(t) : "v"(m));
-            c[e] = v;
-        }
-    } else {
-        c *= m;
+    for (int e = 0; e < 4; e++) {
+        float v = c[e];
+        asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+                     : "+a"(v), "=&v"(t) : "v"(m));
+        c[e] = v;
     }
 }
 
@@ -290,7 +271,6 @@ static_assert(TB_LDS <= 160 * 1024, "LDS");
 template <bool FAST, int NR>
 __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) void tree_attn16_kernel(const AttnArgs a)
 {
-    constexpr bool ASM = true;
     constexpr int ROWS = 64 * NR, DT = TA_KL / 16, KS = TA_CW / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint8_t *s_ok = reinterpret_cast<uint8_t *>(smem + TB_NB * TB_BUF);   // [buffer][wave] a bit a row; [16 + wave]: not finite
@@ -307,416 +287,417 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     const int to = slot_start(sl, slot + 1);
     int from = slot_start(sl, slot);
     for (int b = seq; from < to; b++) {
-    const int cnt = tree_count(a.t, b), rows = cnt * H, r0 = rt * ROWS;
-    const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
-    const int nstep = cnt ? (end + TB_TP - 1) / TB_TP : 0;
-    const int s0 = from - begin, s1 = min(nstep, to - begin);
-    const bool split = s0 > 0 || s1 < nstep;
-    begin += nstep;
-    from = min(begin, to);
-    if (s0 >= s1 || r0 >= rows) continue;
-    __syncthreads();   // the staged steps of the sequence before
+        const int cnt = tree_count(a.t, b), rows = cnt * H, r0 = rt * ROWS;
+        const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
+        const int nstep = cnt ? (end + TB_TP - 1) / TB_TP : 0;
+        const int s0 = from - begin, s1 = min(nstep, to - begin);
+        const bool split = s0 > 0 || s1 < nstep;
+        begin += nstep;
+        from = min(begin, to);
+        if (s0 >= s1 || r0 >= rows) continue;
+        __syncthreads();   // the staged steps of the sequence before
 
-    const int par = tid < 64 && lane < cnt ? tree_parent(a.t, b, lane) : -1;
-    // this lane's query rows: column c16 of each of the wave's NR row tiles
-    auto row_of = [&](int r) __attribute__((always_inline)) { return r0 + 16 * (NR * wv + r) + (opaque(tid) & 15); };
+        const int par = tid < 64 && lane < cnt ? tree_parent(a.t, b, lane) : -1;
+        // this lane's query rows: column c16 of each of the wave's NR row tiles
+        auto row_of = [&](int r) __attribute__((always_inline)) { return r0 + 16 * (NR * wv + r) + (opaque(tid) & 15); };
 
-    // staging: wave wv brings rows 8 wv .. + 7 of a step
-    const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
-    // The page number `pgn` (-1: none) and row in it of the step loaded next; (ncol, nrow) the table column and
-    // row of the one after it, which end at (ecol, erow). A step is tcol columns, trow rows. FAST: of the
-    // wave's first row, its eight lie in one page; else of each lane's.
-    const int ecol = min(end / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? end - ecol * a.c.page : 0;
-    const int frow = s0 * TB_TP + (FAST ? 8 * wv : prow);
-    int pgn = -1, pgo = 0, ncol = frow / a.c.page, nrow = frow - ncol * a.c.page;
-    const int *table = a.c.table + (size_t)b * a.c.max_pages;
-    auto find_rows = [&]() __attribute__((always_inline)) {   // no branch: it stands between products
-        const bool in = (ncol < ecol) | ((ncol == ecol) & (nrow < erow));
-        int at = in ? ncol : 0;
-        if constexpr (FAST) asm volatile("" : "+v"(at));   // a vector load: a scalar one shares the counter of the LDS reads
-        const int n = table[at];
-        pgn = in ? n : -1;
-        pgo = nrow;
-        nrow += a.trow;
-        ncol += a.tcol + (nrow >= a.c.page);
-        nrow -= nrow >= a.c.page ? a.c.page : 0;
-    };
-    // Loads of a step into LDS. FAST: buffer loads from the page's start (of zeros, where there is none; rows
-    // behind the last node are zeroed where they are used). The others go by global loads, a lane's row where
-    // it is, which the compiler takes for LDS accesses too: it then waits for all LDS reads after each.
-    const int fast_off = lrow * (TA_CW * 2) + 16 * lu;
-    int ldo = 0, ldn = 0;
-    const char *ldp = nullptr;
-    auto load_row = [&](int buf) __attribute__((always_inline)) {
-        uint32_t okb;
-        if constexpr (FAST) {
-            const int page = __builtin_amdgcn_readfirstlane(pgn);
-            const bool ok = page >= 0 && page < a.c.n_pages;
-            const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)page * a.page_bytes;
-            ldp = ok ? p : reinterpret_cast<const char *>(ta_zeros);
-            ldn = ok ? (int)a.page_bytes : 8 * TA_CW * 2;
-            ldo = ok ? pgo * (TA_CW * 2) : 0;
-            okb = ok ? 0xff : 0;
-        } else {
-            const bool ok = pgn >= 0 && pgn < a.c.n_pages;
-            const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)pgn * a.page_bytes + (uint32_t)pgo * (uint32_t)(CW * 2);
-            ldp = (ok ? p : reinterpret_cast<const char *>(ta_zeros)) + 16 * lu;
-            okb = gather_rows(__ballot(ok));
-        }
-        s_ok[4 * buf + wv] = (uint8_t)okb;   // every lane the same
-    };
-    auto load_group = [&](lds_char *dst, int g) __attribute__((always_inline)) {
-        lds_void *to = (lds_void *)(dst + TB_GRP * g + 1024 * wv);
-        if constexpr (FAST) {
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void *)ldp, (short)0, ldn, 0x00020000), to, 16, fast_off, ldo + 128 * g, 0, 0);
-        } else {
-            const char *src = ldp + 128 * g;
-            if (8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
-            __builtin_amdgcn_global_load_lds((glb_void *)src, to, 16, 0, 0);
-        }
-    };
-    auto load_step = [&](lds_char *dst, int buf) __attribute__((always_inline)) {
-        load_row(buf);
-#pragma unroll
-        for (int g = 0; g < 9; g++) load_group(dst, g);
-    };
-    auto buf_of = [](int s) { return s & (TB_NB - 1); };
-    lds_char *lds = (lds_char *)smem;
-
-    // steps s0 .. s0 + 2 on their way, the page of s0 + 3 looked up; all lookups first
-    const int sm = min(s1, max(s0, len / TB_TP));   // whole steps of committed positions end here
-    {
-        int n[4], o[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            find_rows();
-            n[i] = pgn;
-            o[i] = pgo;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            pgn = n[i];
-            pgo = o[i];
-            if (i < 3) load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i));
-        }
-    }
-    // Queries; rows behind the last one read the first, their sums are not written.
-    bf16x8 qb[KS][NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const int row = row_of(r);
-        glb_cchar *src = (glb_cchar *)a.q + (((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW + 8 * kq) * 2;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            glb_cchar *at = src + 64 * ks;
-            if (!FAST && 4 * ks + kq >= CW / 8) at = (glb_cchar *)ta_zeros;
-            qb[ks][r] = *(const __attribute__((address_space(1))) bf16x8 *)at;
-        }
-    }
-    f32x4 acc[DT][NR], lacc[NR];
-    float M[NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        M[r] = -INFINITY;
-        lacc[r] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            acc[d][r] = 0.0f;
-            if constexpr (ASM) asm volatile("" : "+a"(acc[d][r]));   // there from here on, not constants
-        }
-    }
-    wait<ASM>();
-    if (tid < 64) s_anc[lane] = tree_ancestors(par);
-    // LDS addresses in a block of 16 rows. Score product: row pi, units 4 (ks & 1) + kq of group ks / 2.
-    // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4. Unit u
-    // of row r stands at u ^ ((r / 2) & 6), so the other units are the first ones with a bit or two turned. The
-    // fragments go in an order that changes the unit seldom, and each address is worked out when it does.
-    const int pi = 4 * (c16 & 3) + (c16 >> 2), vr = 4 * ((lane >> 2) & 3) + kq;
-    const int ka = 128 * pi + 16 * (kq ^ ((pi >> 1) & 6));
-    const int va = 128 * vr + 16 * (((lane >> 1) & 1) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
-
-    // fragments read ahead, and score fragments of a step (fragment 2 ks + block)
-    constexpr int AH = 8, NF = 2 * KS;
-    // fragment f of the scores: block f % 2 of K-step ks_of(f); of the sum: latent tile d_of(i)
-    auto ks_of = [](int f) { return f < KS ? 2 * (f >> 1) : 2 * ((f - KS) >> 1) + 1; };
-    auto d_of = [](int i) { return 4 * (i & 7) + (i >> 3); };
-    static_assert(KS % 2 == 0 && DT == 32, "fragment orders");
-    int kat = 0, vat = 0;
-    auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {
-        if (f == 0 || f == KS) kat = opaque(ka) ^ (f == KS ? 64 : 0);
-        return *(const __attribute__((address_space(3))) bf16x8 *)(buf + kat + TB_GRP * (ks_of(f) >> 1) + 2048 * (f & 1));
-    };
-    auto vread = [&](lds_cchar *buf, int i) __attribute__((always_inline)) {
-        if (i % 8 == 0) vat = opaque(va) ^ (4 * i);
-        lds_cchar *at = buf + vat + TB_GRP * (d_of(i) >> 2);
-        const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
-        const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
-        const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
-        return __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
-    };
-    // Scores of a step, its first AH fragments already read; the last AH products read the first fragments of
-    // the sum from `sum`. between(f): work that goes between the products.
-    auto scores = [&](lds_cchar *buf, lds_cchar *sum, bf16x8 (&kf)[AH], bf16x8 (&vf)[AH], f32x4 (&S)[2][NR], auto between)
-                      __attribute__((always_inline)) {
-#pragma unroll
-        for (int f = 0; f < NF; f++) {
-            const bf16x8 x = kf[f % AH];
-#pragma unroll
-            for (int r = 0; r < NR; r++) mfma_vec<ASM>(x, qb[ks_of(f)][r], S[f & 1][r], f < 2);
-            if (f + AH < NF) kf[f % AH] = kread(buf, f + AH);
-            else vf[f + AH - NF] = vread(sum, f + AH - NF);
-            between(f);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    auto nothing = [](int) __attribute__((always_inline)) {};
-    // The sum of a step, its first AH fragments already read; between(d) before the next fragment but AH is read.
-    auto values = [&](lds_cchar *buf, bf16x8 (&vf)[AH], const bf16x8 (&pf)[NR], auto between) __attribute__((always_inline)) {
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const bf16x8 v = vf[d % AH];
-#pragma unroll
-            for (int r = 0; r < NR; r++) mfma_acc<ASM>(v, pf[r], acc[d_of(d)][r]);
-            if (d + AH < DT) vf[d % AH] = vread(buf, d + AH);
-            between(d);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    // the softmax of a step in 28 pieces: S to weights in the second product's operand, M and the factor al
-    // that the sums before it are to be scaled by
-    struct Soft {
-        float mt[NR], ref[NR], al[NR];
-        bool moved;
-    };
-    auto soft_piece = [&](int i, f32x4 (&S)[2][NR], Soft &x, bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
-        if (i < NR) {
-            const f32x4 u = S[0][i], v = S[1][i];
-            x.mt[i] = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-        } else if (i == 2) {
-#pragma unroll
-            for (int r = 0; r < NR; r++) x.mt[r] = quarter_max(x.mt[r]) * a.scale2;
-        } else if (i == 3) {
-            x.moved = false;
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const bool up = x.mt[r] > M[r] + TA_LAZY;
-                const float mn = up ? x.mt[r] : M[r];
-                x.al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
-                x.moved = x.moved || up;
-                M[r] = mn;
-                x.ref[r] = mn == -INFINITY ? 0.0f : mn;
-            }
-        } else if (i >= 4 && i < 4 + 8 * NR) {
-            const int k = i - 4, r = k >> 3, e = k & 7;
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e >> 2][r][e & 3], a.scale2, -x.ref[r]));
-            asm volatile("" : "+v"(p));   // here, not where it is used
-            S[e >> 2][r][e & 3] = p;
-        } else if (i >= 20 && i < 20 + 4 * NR) {
-            const int k = i - 20, r = k >> 2, w = k & 3;
-            const bf16x2 y = __builtin_convertvector(f2{S[w >> 1][r][2 * (w & 1)], S[w >> 1][r][2 * (w & 1) + 1]}, bf16x2);
-            pf[r][2 * w] = y[0];
-            pf[r][2 * w + 1] = y[1];
-        }
-    };
-    auto rescale = [&](const Soft &x) __attribute__((always_inline)) {
-        if (!__ballot(x.moved)) return;
-        wait<ASM>();
-#pragma unroll
-        for (int r = 0; r < NR; r++) lacc[r] *= x.al[r];
-#pragma unroll
-        for (int r = 0; r < NR; r++)
-#pragma unroll
-            for (int d = 0; d < DT; d++) acc_scale<ASM>(acc[d][r], x.al[r]);
-        wait<ASM>();
-    };
-    auto publish = [](int left) __attribute__((always_inline)) {   // this wave's loads but the last `left`, then every wave's
-        if (left) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    auto pages_of = [&](int s) __attribute__((always_inline)) { return reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)]; };
-    auto mask_pages = [&](uint32_t held, f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(held);
-        if (ok == 0xffffffffu) return;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (!(ok >> (16 * i + 4 * e + kq) & 1))
-#pragma unroll
-                    for (int r = 0; r < NR; r++) S[i][r][e] = -INFINITY;
-    };
-
-    if (s0 < sm) {
-        f32x4 S[2][NR];
-        bf16x8 kf[AH], vf[AH], pf[NR];
-        Soft x;
-        publish(9);
-        {
-            lds_cchar *cur = lds + buf_of(s0) * TB_BUF;
-#pragma unroll
-            for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
-            scores(cur, cur, kf, vf, S, nothing);
-            wait<ASM>();
-            mask_pages(pages_of(s0), S);
-#pragma unroll
-            for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
-            cur = lds + buf_of(s0 + 1) * TB_BUF;
-#pragma unroll
-            for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
-        }
-        // the sums are zeros yet: nothing to rescale
-        // Step s's sum and step s + 1's scores. The buffers as parameters that do not alias: else the compiler
-        // has every transposed read wait for the loads in flight.
-        auto step = [&](lds_cchar *__restrict__ cur, lds_cchar *__restrict__ nxt, lds_cchar *__restrict__ nx2,
-                        lds_char *__restrict__ fill, int s) __attribute__((always_inline)) {
-            uint32_t held = 0;
-            scores(nxt, cur, kf, vf, S, [&](int f) __attribute__((always_inline)) {
-                if (f == 6) held = pages_of(s + 1);
-                if (f == 2) load_row(buf_of(s + 3));
-                if (f == 4) find_rows();
-                if (f >= 8 && f < 26 && f % 2 == 0) load_group(fill, (f - 8) / 2);
-            });
-            bf16x8 pn[NR];
-#pragma unroll
-            for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);   // with its wait states, S is there
-            __builtin_amdgcn_sched_barrier(0);
-            mask_pages(held, S);
-            values(cur, vf, pf, [&](int d) __attribute__((always_inline)) {
-                if (d < 28) soft_piece(d, S, x, pn);
-                if (d == 28) {
-                    // every fragment of step s is in registers: its buffer is free behind the barrier
-                    publish(9);
-#pragma unroll
-                    for (int f = 0; f < 4; f++) kf[f] = kread(nx2, f);
-                }
-                if (d > 28) kf[d - 25] = kread(nx2, d - 25);
-                if (d == 31) kf[7] = kread(nx2, 7);
-            });
-            rescale(x);
-#pragma unroll
-            for (int r = 0; r < NR; r++) pf[r] = pn[r];
+        // staging: wave wv brings rows 8 wv .. + 7 of a step
+        const int lrow = lane >> 3, prow = 8 * wv + lrow, lu = (lane & 7) ^ ((prow >> 1) & 6);
+        // The page number `pgn` (-1: none) and row in it of the step loaded next; (ncol, nrow) the table column and
+        // row of the one after it, which end at (ecol, erow). A step is tcol columns, trow rows. FAST: of the
+        // wave's first row, its eight lie in one page; else of each lane's.
+        const int stop = min(end, s1 * TB_TP);   // what lies behind is not brought in
+        const int ecol = min(stop / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? stop - ecol * a.c.page : 0;
+        const int frow = s0 * TB_TP + (FAST ? 8 * wv : prow);
+        int pgn = -1, pgo = 0, ncol = frow / a.c.page, nrow = frow - ncol * a.c.page;
+        const int *table = a.c.table + (size_t)b * a.c.max_pages;
+        auto find_rows = [&]() __attribute__((always_inline)) {   // no branch: it stands between products
+            const bool in = (ncol < ecol) | ((ncol == ecol) & (nrow < erow));
+            int at = in ? ncol : 0;
+            if constexpr (FAST) asm volatile("" : "+v"(at));   // a vector load: a scalar one shares the counter of the LDS reads
+            const int n = table[at];
+            pgn = in ? n : -1;
+            pgo = nrow;
+            nrow += a.trow;
+            ncol += a.tcol + (nrow >= a.c.page);
+            nrow -= nrow >= a.c.page ? a.c.page : 0;
         };
-        for (int s = s0; s + 1 < sm; s++)
-            step(lds + buf_of(s) * TB_BUF, lds + buf_of(s + 1) * TB_BUF, lds + buf_of(s + 2) * TB_BUF, lds + buf_of(s + 3) * TB_BUF, s);
-        wait<ASM>();
+        // Loads of a step into LDS. FAST: buffer loads from the page's start (of zeros, where there is none; rows
+        // behind the last node are zeroed where they are used). The others go by global loads, a lane's row where
+        // it is, which the compiler takes for LDS accesses too: it then waits for all LDS reads after each.
+        const int fast_off = lrow * (TA_CW * 2) + 16 * lu;
+        int ldo = 0, ldn = 0;
+        const char *ldp = nullptr;
+        auto load_row = [&](int buf) __attribute__((always_inline)) {
+            uint32_t okb;
+            if constexpr (FAST) {
+                const int page = __builtin_amdgcn_readfirstlane(pgn);
+                const bool ok = page >= 0 && page < a.c.n_pages;
+                const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)page * a.page_bytes;
+                ldp = ok ? p : reinterpret_cast<const char *>(ta_zeros);
+                ldn = ok ? (int)a.page_bytes : 8 * TA_CW * 2;
+                ldo = ok ? pgo * (TA_CW * 2) : 0;
+                okb = ok ? 0xff : 0;
+            } else {
+                const bool ok = pgn >= 0 && pgn < a.c.n_pages;
+                const char *p = reinterpret_cast<const char *>(a.pages) + (uint64_t)(uint32_t)pgn * a.page_bytes + (uint32_t)pgo * (uint32_t)(CW * 2);
+                ldp = (ok ? p : reinterpret_cast<const char *>(ta_zeros)) + 16 * lu;
+                okb = gather_rows(__ballot(ok));
+            }
+            s_ok[4 * buf + wv] = (uint8_t)okb;   // every lane the same
+        };
+        auto load_group = [&](lds_char *dst, int g) __attribute__((always_inline)) {
+            lds_void *to = (lds_void *)(dst + TB_GRP * g + 1024 * wv);
+            if constexpr (FAST) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void *)ldp, (short)0, ldn, 0x00020000), to, 16, fast_off, ldo + 128 * g, 0, 0);
+            } else {
+                const char *src = ldp + 128 * g;
+                if (8 * g + lu >= CW / 8) src = reinterpret_cast<const char *>(ta_zeros);
+                __builtin_amdgcn_global_load_lds((glb_void *)src, to, 16, 0, 0);
+            }
+        };
+        auto load_step = [&](lds_char *dst, int buf) __attribute__((always_inline)) {
+            load_row(buf);
+#pragma unroll
+            for (int g = 0; g < 9; g++) load_group(dst, g);
+        };
+        auto buf_of = [](int s) { return s & (TB_NB - 1); };
+        lds_char *lds = (lds_char *)smem;
+
+        // steps s0 .. s0 + 2 on their way, the page of s0 + 3 looked up; all lookups first
+        const int sm = min(s1, max(s0, len / TB_TP));   // whole steps of committed positions end here
         {
-            lds_cchar *cur = lds + buf_of(sm - 1) * TB_BUF;
-            publish(0);
-            load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2));
+            int n[4], o[4];
 #pragma unroll
-            for (int d = 0; d < AH; d++) vf[d] = vread(cur, d);
+            for (int i = 0; i < 4; i++) {
+                find_rows();
+                n[i] = pgn;
+                o[i] = pgo;
+            }
 #pragma unroll
-            for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
-            values(cur, vf, pf, nothing);
-            wait<ASM>();
-        }
-    }
-    // the steps that hold nodes: at most three, on their way by now
-    for (int s = sm; s < s1; s++) {
-        publish(0);
-        const int ln = opaque(tid) & 63, pr = 8 * wv + (ln >> 3), q4 = ln >> 4;
-        char *at = smem + buf_of(s) * TB_BUF + 1024 * wv + 16 * ln;
-        lds_cchar *cur = lds + buf_of(s) * TB_BUF;
-        const uint32_t ok = reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)];
-        const int n0 = len - s * TB_TP;   // place of the first node in the step
-        // Zeros in the rows behind the last node, and in rows of nodes that hold an infinity or a NaN, which are
-        // noted, so that the query rows that see them become NaN and no others
-        bool inf = false;
-        if (cnt > 1) {
-#pragma unroll
-            for (int g = 0; g < 9; g++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(at + TB_GRP * g);
-                inf = inf || not_finite16(w.x) || not_finite16(w.y) || not_finite16(w.z) || not_finite16(w.w);
+            for (int i = 0; i < 4; i++) {
+                pgn = n[i];
+                pgo = o[i];
+                if (i < 3) load_step(lds + buf_of(s0 + i) * TB_BUF, buf_of(s0 + i));
             }
         }
-        const bool behind = s * TB_TP + pr >= end;
-        const uint64_t m = __ballot(inf && pr >= n0);
-        const bool mine = (m >> (ln & 56) & 0xff) != 0 && !behind;
-        if (mine || behind)
-#pragma unroll
-            for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + TB_GRP * g) = uint4{0, 0, 0, 0};
-        s_ok[16 + wv] = (uint8_t)gather_rows(__ballot(mine));
-        __syncthreads();
-        const uint32_t bad = reinterpret_cast<const uint32_t *>(s_ok)[4];
-        f32x4 S[2][NR];
-        bf16x8 kf[AH], vf[AH], pf[NR];
-        Soft x;
-#pragma unroll
-        for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
-        scores(cur, cur, kf, vf, S, nothing);
-        wait<ASM>();
+        // Queries; rows behind the last one read the first, their sums are not written.
+        bf16x8 qb[KS][NR];
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             const int row = row_of(r);
-            const uint64_t anc = s_anc[row < rows ? row / H : 0];
-            uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
-            if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc << n0);
-            else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc >> -n0);
-            w &= ok;
+            glb_cchar *src = (glb_cchar *)a.q + (((size_t)b * a.t.N * H + (row < rows ? row : 0)) * CW + 8 * kq) * 2;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                glb_cchar *at = src + 64 * ks;
+                if (!FAST && 4 * ks + kq >= CW / 8) at = (glb_cchar *)ta_zeros;
+                qb[ks][r] = *(const __attribute__((address_space(1))) bf16x8 *)at;
+            }
+        }
+        f32x4 acc[DT][NR], lacc[NR];
+        float M[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            M[r] = -INFINITY;
+            lacc[r] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                acc[d][r] = 0.0f;
+                asm volatile("" : "+a"(acc[d][r]));   // there from here on, not constants
+            }
+        }
+        wait();
+        if (tid < 64) s_anc[lane] = tree_ancestors(par);
+        // LDS addresses in a block of 16 rows. Score product: row pi, units 4 (ks & 1) + kq of group ks / 2.
+        // Second product: rows 4 ((lane / 4) % 4) + kq, units 2 (d % 4) + (lane / 2) % 2 of group d / 4. Unit u
+        // of row r stands at u ^ ((r / 2) & 6), so the other units are the first ones with a bit or two turned. The
+        // fragments go in an order that changes the unit seldom, and each address is worked out when it does.
+        const int pi = 4 * (c16 & 3) + (c16 >> 2), vr = 4 * ((lane >> 2) & 3) + kq;
+        const int ka = 128 * pi + 16 * (kq ^ ((pi >> 1) & 6));
+        const int va = 128 * vr + 16 * (((lane >> 1) & 1) ^ ((vr >> 1) & 6)) + 8 * (lane & 1);
+
+        // fragments read ahead, and score fragments of a step (fragment 2 ks + block)
+        constexpr int AH = 8, NF = 2 * KS;
+        // fragment f of the scores: block f % 2 of K-step ks_of(f); of the sum: latent tile d_of(i)
+        auto ks_of = [](int f) { return f < KS ? 2 * (f >> 1) : 2 * ((f - KS) >> 1) + 1; };
+        auto d_of = [](int i) { return 4 * (i & 7) + (i >> 3); };
+        static_assert(KS % 2 == 0 && DT == 32, "fragment orders");
+        int kat = 0, vat = 0;
+        auto kread = [&](lds_cchar *buf, int f) __attribute__((always_inline)) {
+            if (f == 0 || f == KS) kat = opaque(ka) ^ (f == KS ? 64 : 0);
+            return *(const __attribute__((address_space(3))) bf16x8 *)(buf + kat + TB_GRP * (ks_of(f) >> 1) + 2048 * (f & 1));
+        };
+        auto vread = [&](lds_cchar *buf, int i) __attribute__((always_inline)) {
+            if (i % 8 == 0) vat = opaque(va) ^ (4 * i);
+            lds_cchar *at = buf + vat + TB_GRP * (d_of(i) >> 2);
+            const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+            const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 2048));
+            const uint2 y0 = __builtin_bit_cast(uint2, x0), y1 = __builtin_bit_cast(uint2, x1);
+            return __builtin_bit_cast(bf16x8, uint4{y0.x, y0.y, y1.x, y1.y});
+        };
+        // Scores of a step, its first AH fragments already read; the last AH products read the first fragments of
+        // the sum from `sum`. between(f): work that goes between the products.
+        auto scores = [&](lds_cchar *buf, lds_cchar *sum, bf16x8 (&kf)[AH], bf16x8 (&vf)[AH], f32x4 (&S)[2][NR], auto between)
+                          __attribute__((always_inline)) {
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                const bf16x8 x = kf[f % AH];
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_vec(x, qb[ks_of(f)][r], S[f & 1][r], f < 2);
+                if (f + AH < NF) kf[f % AH] = kread(buf, f + AH);
+                else vf[f + AH - NF] = vread(sum, f + AH - NF);
+                between(f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto nothing = [](int) __attribute__((always_inline)) {};
+        // The sum of a step, its first AH fragments already read; between(d) before the next fragment but AH is read.
+        auto values = [&](lds_cchar *buf, bf16x8 (&vf)[AH], const bf16x8 (&pf)[NR], auto between) __attribute__((always_inline)) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const bf16x8 v = vf[d % AH];
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_acc(v, pf[r], acc[d_of(d)][r]);
+                if (d + AH < DT) vf[d % AH] = vread(buf, d + AH);
+                between(d);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // the softmax of a step in 28 pieces: S to weights in the second product's operand, M and the factor al
+        // that the sums before it are to be scaled by
+        struct Soft {
+            float mt[NR], ref[NR], al[NR];
+            bool moved;
+        };
+        auto soft_piece = [&](int i, f32x4 (&S)[2][NR], Soft &x, bf16x8 (&pf)[NR]) __attribute__((always_inline)) {
+            if (i < NR) {
+                const f32x4 u = S[0][i], v = S[1][i];
+                x.mt[i] = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+            } else if (i == 2) {
+#pragma unroll
+                for (int r = 0; r < NR; r++) x.mt[r] = quarter_max(x.mt[r]) * a.scale2;
+            } else if (i == 3) {
+                x.moved = false;
+#pragma unroll
+                for (int r = 0; r < NR; r++) {
+                    const bool up = x.mt[r] > M[r] + TA_LAZY;
+                    const float mn = up ? x.mt[r] : M[r];
+                    x.al[r] = up ? __builtin_amdgcn_exp2f(M[r] - mn) : 1.0f;
+                    x.moved = x.moved || up;
+                    M[r] = mn;
+                    x.ref[r] = mn == -INFINITY ? 0.0f : mn;
+                }
+            } else if (i >= 4 && i < 4 + 8 * NR) {
+                const int k = i - 4, r = k >> 3, e = k & 7;
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[e >> 2][r][e & 3], a.scale2, -x.ref[r]));
+                asm volatile("" : "+v"(p));   // here, not where it is used
+                S[e >> 2][r][e & 3] = p;
+            } else if (i >= 20 && i < 20 + 4 * NR) {
+                const int k = i - 20, r = k >> 2, w = k & 3;
+                const bf16x2 y = __builtin_convertvector(f2{S[w >> 1][r][2 * (w & 1)], S[w >> 1][r][2 * (w & 1) + 1]}, bf16x2);
+                pf[r][2 * w] = y[0];
+                pf[r][2 * w + 1] = y[1];
+            }
+        };
+        auto rescale = [&](const Soft &x) __attribute__((always_inline)) {
+            if (!__ballot(x.moved)) return;
+            wait();
+#pragma unroll
+            for (int r = 0; r < NR; r++) lacc[r] *= x.al[r];
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc_scale(acc[d][r], x.al[r]);
+            wait();
+        };
+        auto publish = [](int left) __attribute__((always_inline)) {   // this wave's loads but the last `left`, then every wave's
+            if (left) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        auto pages_of = [&](int s) __attribute__((always_inline)) { return reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)]; };
+        auto mask_pages = [&](uint32_t held, f32x4 (&S)[2][NR]) __attribute__((always_inline)) {
+            const uint32_t ok = __builtin_amdgcn_readfirstlane(held);
+            if (ok == 0xffffffffu) return;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int bit = 16 * i + 4 * e + q4;
-                    const float seen = bad >> bit & 1 ? NAN : 0.0f;
-                    S[i][r][e] = w >> bit & 1 ? S[i][r][e] + seen : -INFINITY;
-                }
+                for (int e = 0; e < 4; e++)
+                    if (!(ok >> (16 * i + 4 * e + kq) & 1))
+#pragma unroll
+                        for (int r = 0; r < NR; r++) S[i][r][e] = -INFINITY;
+        };
+
+        if (s0 < sm) {
+            f32x4 S[2][NR];
+            bf16x8 kf[AH], vf[AH], pf[NR];
+            Soft x;
+            publish(9);
+            {
+                lds_cchar *cur = lds + buf_of(s0) * TB_BUF;
+#pragma unroll
+                for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
+                scores(cur, cur, kf, vf, S, nothing);
+                wait();
+                mask_pages(pages_of(s0), S);
+#pragma unroll
+                for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
+                cur = lds + buf_of(s0 + 1) * TB_BUF;
+#pragma unroll
+                for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
+            }
+            // the sums are zeros yet: nothing to rescale
+            // Step s's sum and step s + 1's scores. The buffers as parameters that do not alias: else the compiler
+            // has every transposed read wait for the loads in flight.
+            auto step = [&](lds_cchar *__restrict__ cur, lds_cchar *__restrict__ nxt, lds_cchar *__restrict__ nx2,
+                            lds_char *__restrict__ fill, int s) __attribute__((always_inline)) {
+                uint32_t held = 0;
+                scores(nxt, cur, kf, vf, S, [&](int f) __attribute__((always_inline)) {
+                    if (f == 6) held = pages_of(s + 1);
+                    if (f == 2) load_row(buf_of(s + 3));
+                    if (f == 4) find_rows();
+                    if (f >= 8 && f < 26 && f % 2 == 0) load_group(fill, (f - 8) / 2);
+                });
+                bf16x8 pn[NR];
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_sum(pf[r], lacc[r]);   // with its wait states, S is there
+                __builtin_amdgcn_sched_barrier(0);
+                mask_pages(held, S);
+                values(cur, vf, pf, [&](int d) __attribute__((always_inline)) {
+                    if (d < 28) soft_piece(d, S, x, pn);
+                    if (d == 28) {
+                        // every fragment of step s is in registers: its buffer is free behind the barrier
+                        publish(9);
+#pragma unroll
+                        for (int f = 0; f < 4; f++) kf[f] = kread(nx2, f);
+                    }
+                    if (d > 28) kf[d - 25] = kread(nx2, d - 25);
+                    if (d == 31) kf[7] = kread(nx2, 7);
+                });
+                rescale(x);
+#pragma unroll
+                for (int r = 0; r < NR; r++) pf[r] = pn[r];
+            };
+            for (int s = s0; s + 1 < sm; s++)
+                step(lds + buf_of(s) * TB_BUF, lds + buf_of(s + 1) * TB_BUF, lds + buf_of(s + 2) * TB_BUF, lds + buf_of(s + 3) * TB_BUF, s);
+            wait();
+            {
+                lds_cchar *cur = lds + buf_of(sm - 1) * TB_BUF;
+                publish(0);
+                load_step(lds + buf_of(sm + 2) * TB_BUF, buf_of(sm + 2));
+#pragma unroll
+                for (int d = 0; d < AH; d++) vf[d] = vread(cur, d);
+#pragma unroll
+                for (int r = 0; r < NR; r++) mfma_sum(pf[r], lacc[r]);
+                values(cur, vf, pf, nothing);
+                wait();
+            }
         }
+        // the steps that hold nodes: at most three, on their way by now
+        for (int s = sm; s < s1; s++) {
+            publish(0);
+            const int ln = opaque(tid) & 63, pr = 8 * wv + (ln >> 3), q4 = ln >> 4;
+            char *at = smem + buf_of(s) * TB_BUF + 1024 * wv + 16 * ln;
+            lds_cchar *cur = lds + buf_of(s) * TB_BUF;
+            const uint32_t ok = reinterpret_cast<const uint32_t *>(s_ok)[buf_of(s)];
+            const int n0 = len - s * TB_TP;   // place of the first node in the step
+            // Zeros in the rows behind the last node, and in rows of nodes that hold an infinity or a NaN, which are
+            // noted, so that the query rows that see them become NaN and no others
+            bool inf = false;
+            if (cnt > 1) {
 #pragma unroll
-        for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
-        rescale(x);
+                for (int g = 0; g < 9; g++) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(at + TB_GRP * g);
+                    inf = inf || not_finite16(w.x) || not_finite16(w.y) || not_finite16(w.z) || not_finite16(w.w);
+                }
+            }
+            const bool behind = s * TB_TP + pr >= end;
+            const uint64_t m = __ballot(inf && pr >= n0);
+            const bool mine = (m >> (ln & 56) & 0xff) != 0 && !behind;
+            if (mine || behind)
 #pragma unroll
-        for (int r = 0; r < NR; r++) mfma_sum<ASM>(pf[r], lacc[r]);
-        values(cur, vf, pf, nothing);
-        wait<ASM>();
-    }
+                for (int g = 0; g < 9; g++) *reinterpret_cast<uint4 *>(at + TB_GRP * g) = uint4{0, 0, 0, 0};
+            s_ok[16 + wv] = (uint8_t)gather_rows(__ballot(mine));
+            __syncthreads();
+            const uint32_t bad = reinterpret_cast<const uint32_t *>(s_ok)[4];
+            f32x4 S[2][NR];
+            bf16x8 kf[AH], vf[AH], pf[NR];
+            Soft x;
+#pragma unroll
+            for (int f = 0; f < AH; f++) kf[f] = kread(cur, f);
+            scores(cur, cur, kf, vf, S, nothing);
+            wait();
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const int row = row_of(r);
+                const uint64_t anc = s_anc[row < rows ? row / H : 0];
+                uint32_t w = n0 >= 32 ? ~0u : n0 <= 0 ? 0u : (1u << n0) - 1;
+                if (n0 >= 0 && n0 < 32) w |= (uint32_t)(anc << n0);
+                else if (n0 < 0 && n0 > -64) w |= (uint32_t)(anc >> -n0);
+                w &= ok;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int bit = 16 * i + 4 * e + q4;
+                        const float seen = bad >> bit & 1 ? NAN : 0.0f;
+                        S[i][r][e] = w >> bit & 1 ? S[i][r][e] + seen : -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 28; i++) soft_piece(i, S, x, pf);
+            rescale(x);
+#pragma unroll
+            for (int r = 0; r < NR; r++) mfma_sum(pf[r], lacc[r]);
+            values(cur, vf, pf, nothing);
+            wait();
+        }
 
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const int row = row_of(r);
-        if (row >= rows) continue;
-        const float l = lacc[r][0];
-        const int q4 = (opaque(tid) & 63) >> 4;
-        const size_t orow = (size_t)b * a.t.N * H + row, prow = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
-        if (split) {
-            if (q4 == 0) {
-                a.pm[prow] = M[r];
-                a.pl[prow] = l;
-            }
-            if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
-            float *dst = a.po + prow * KL + 4 * q4;
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-                if (16 * d + 4 * q4 < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r];
-        } else {
-            if (q4 == 0 && a.lse) a.lse[orow] = l == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(l)) * TA_LN2;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (a.o_dt == K3HIP_F32) {
-                float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * q4;
+        for (int r = 0; r < NR; r++) {
+            const int row = row_of(r);
+            if (row >= rows) continue;
+            const float l = lacc[r][0];
+            const int q4 = (opaque(tid) & 63) >> 4;
+            const size_t orow = (size_t)b * a.t.N * H + row, prow = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
+            if (split) {
+                if (q4 == 0) {
+                    a.pm[prow] = M[r];
+                    a.pl[prow] = l;
+                }
+                if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
+                float *dst = a.po + prow * KL + 4 * q4;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + 4 * q4 < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r] * inv;
+                    if (16 * d + 4 * q4 < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r];
             } else {
-                uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * q4;
+                if (q4 == 0 && a.lse) a.lse[orow] = l == 0.0f ? -INFINITY : (M[r] + __builtin_amdgcn_logf(l)) * TA_LN2;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                if (a.o_dt == K3HIP_F32) {
+                    float *dst = reinterpret_cast<float *>(a.o) + orow * KL + 4 * q4;
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-                    if (16 * d + 4 * q4 < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d][r] * inv);
+                    for (int d = 0; d < DT; d++)
+                        if (16 * d + 4 * q4 < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d][r] * inv;
+                } else {
+                    uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + 4 * q4;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+                        if (16 * d + 4 * q4 < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d][r] * inv);
+                }
             }
         }
-    }
     }
 }
 
-// fp32 caches. The products run on the fp16 matrix cores at fp32's accuracy: a row is scaled by a power of
-// two that puts its largest value just under 2^15 and split into fp16 hi + lo, 22 bits together (what
-// falls under fp16's smallest step is under 2^-39 of the row's largest value), and hi hi + hi lo + lo hi are summed in
+// fp32 caches. The products run on the fp16 matrix cores near fp32's accuracy: a row is scaled by a power of
+// two that puts its largest value just under 2^15 and split into fp16 hi + 2^-11 lo, 22 bits together (down to
+// 2^-29 of the row's largest value; what is left out is under 2^-51 of it), and hi hi + hi lo + lo hi are summed in
 // fp32, three matrix instructions where six are needed on bf16 parts and sixteen times the rate of the fp32
 // instruction. A cache row's scale 2^k goes with its weight: the reference that weights are taken
-// against is the largest of (score - k), so the scaled weight 2^(score - k - M) is at most 2^TS_UP ahead of its own
-// split, whatever the rows' sizes, and the sum of the weights takes the 2^k back out.
+// against is the largest of (score - k), so the scaled weight 2^(score - k - M) is at most 2^(TS_UP + TA_LAZY) whatever
+// the rows' sizes, and the sum of the weights takes the 2^k back out.
 //
 // A step is 32 positions, staged as two planes of column groups as in the bf16 kernel, two buffers. Eight
 // waves, two a SIMD: waves w and w + 4 own 16 query rows; each scores half of the cache row's channels (so it holds half
@@ -724,21 +705,27 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // latent's channels (64 registers). A step has two barriers, behind the halves of the scores and behind the
 // sum; a wave keeps 4 rows on their way to registers and converts and stages them, a column group at a time, between the
 // products: groups 4 .. 8 beside the scores, where groups 0 .. 3 of the buffer carry the halves, those beside the sum.
+// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 140 us with the merge, 200 TFLOP/s of the fp32 work, 3.3k
+// of a step's 8.7k cycles matrix instructions and 3.4k LDS accesses; what binds is the wait of two waves in step for
+// LDS fragments (registers allow one K-step of look-ahead), the hand-over (800 cycles) and the softmax (700). With
+// four waves of whole rows, one a SIMD, 238 us: nothing stood beside their waits, and they spilled.
 constexpr int TS_BUF = 2 * TB_BUF;
 constexpr int TS_NT = 512;
 constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 8 + 64 + TREE_MAX * 8;
 constexpr float TS_UP = 7.0f;     // log2 of the weight of the reference
+constexpr float TS_LO = 2048.0f;  // what lo parts are scaled by
 static_assert(TS_LDS <= 160 * 1024, "LDS");
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+// x = hi + 2^-11 lo
 __device__ __forceinline__ void split16(const float (&x)[8], f16x8 &hi, f16x8 &lo)
 {
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
         const f16x2 h = __builtin_convertvector(f2{x[e], x[e + 1]}, f16x2);
-        const f16x2 l = __builtin_convertvector(f2{x[e] - (float)h[0], x[e + 1] - (float)h[1]}, f16x2);
+        const f16x2 l = __builtin_convertvector(f2{(x[e] - (float)h[0]) * TS_LO, (x[e + 1] - (float)h[1]) * TS_LO}, f16x2);
         hi[e] = h[0];
         hi[e + 1] = h[1];
         lo[e] = l[0];
@@ -750,17 +737,22 @@ __device__ __forceinline__ void split16(const float (&x)[8], f16x8 &hi, f16x8 &l
 // register, or one that writes and one that reads it, stands another.
 __device__ __forceinline__ void split4(const f4 &x, float scale, uint2 &hi, uint2 &lo)
 {
-    asm("v_fma_mixlo_f16 %0, %4, %8, 0\n\t"
-        "v_fma_mixlo_f16 %1, %6, %8, 0\n\t"
-        "v_fma_mixhi_f16 %0, %5, %8, 0\n\t"
-        "v_fma_mixhi_f16 %1, %7, %8, 0\n\t"
-        "v_fma_mixlo_f16 %2, %4, %8, -%0 op_sel_hi:[0,0,1]\n\t"
-        "v_fma_mixlo_f16 %3, %6, %8, -%1 op_sel_hi:[0,0,1]\n\t"
-        "v_fma_mixhi_f16 %2, %5, %8, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
-        "v_fma_mixhi_f16 %3, %7, %8, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+    float t0, t1, t2, t3;
+    asm("v_fma_mixlo_f16 %0, %8, %12, 0\n\t"
+        "v_fma_mixlo_f16 %1, %10, %12, 0\n\t"
+        "v_fma_mixhi_f16 %0, %9, %12, 0\n\t"
+        "v_fma_mixhi_f16 %1, %11, %12, 0\n\t"
+        "v_fma_mix_f32 %4, %8, %12, -%0 op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mix_f32 %6, %10, %12, -%1 op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mix_f32 %5, %9, %12, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mix_f32 %7, %11, %12, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixlo_f16 %2, %4, %13, 0\n\t"
+        "v_fma_mixlo_f16 %3, %6, %13, 0\n\t"
+        "v_fma_mixhi_f16 %2, %5, %13, 0\n\t"
+        "v_fma_mixhi_f16 %3, %7, %13, 0\n\t"
         "s_nop 0"
-        : "=&v"(hi.x), "=&v"(hi.y), "=&v"(lo.x), "=&v"(lo.y)
-        : "v"(x.x), "v"(x.y), "v"(x.z), "v"(x.w), "v"(scale));
+        : "=&v"(hi.x), "=&v"(hi.y), "=&v"(lo.x), "=&v"(lo.y), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+        : "v"(x.x), "v"(x.y), "v"(x.z), "v"(x.w), "v"(scale), "s"(TS_LO));
 }
 
 // The power of two that a row whose largest magnitude has these bits is scaled by.
@@ -810,7 +802,8 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 
         // staging: rows 4 wv .. + 3 of a step, channels 4 (lane & 15) .. + 3 of each column group
         const int prow = 4 * wv + kq;
-        const int ecol = min(end / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? end - ecol * a.c.page : 0;
+        const int stop = min(end, s1 * TB_TP);   // what lies behind is not brought in
+        const int ecol = min(stop / a.c.page, a.c.max_pages), erow = ecol < a.c.max_pages ? stop - ecol * a.c.page : 0;
         int col = (s0 * TB_TP + prow) / a.c.page, prw = s0 * TB_TP + prow - col * a.c.page;   // of the row to load next
         const int *table = a.c.table + (size_t)b * a.c.max_pages;
         auto has_page = [&]() __attribute__((always_inline)) { return (col < ecol) | ((col == ecol) & (prw < erow)); };
@@ -1003,7 +996,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             const int ht = opaque(tid);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                S[i] = (S[i] + Sl[i]) * qscale;
+                S[i] = (S[i] + Sl[i] * (1.0f / TS_LO)) * qscale;
                 asm volatile("" : "+v"(S[i]));   // rounded here, as its partner gets it: both have to come to the same bits
                 *half_at(s, wv ^ 4, i, ht) = f4{S[i][0], S[i][1], S[i][2], S[i][3]};
             }
@@ -1064,11 +1057,23 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
                 pw[x] = __builtin_amdgcn_exp2f(y[x] - ref);
                 lsum = __builtin_fmaf(pw[x], __uint_as_float(0x7f000000u - __float_as_uint(k[x].x)), lsum);   // times 2^k
             }
-            split16(pw, ph, pl);
+            f16x8 pd;   // for the rows' lo parts
+#pragma unroll
+            for (int x = 0; x < 8; x += 2) {
+                const f16x2 h = __builtin_convertvector(f2{pw[x], pw[x + 1]}, f16x2);
+                const f16x2 l = __builtin_convertvector(f2{pw[x] - (float)h[0], pw[x + 1] - (float)h[1]}, f16x2);
+                const f16x2 d = __builtin_convertvector(f2{pw[x] * (1.0f / TS_LO), pw[x + 1] * (1.0f / TS_LO)}, f16x2);
+                ph[x] = h[0];
+                ph[x + 1] = h[1];
+                pl[x] = l[0];
+                pl[x + 1] = l[1];
+                pd[x] = d[0];
+                pd[x + 1] = d[1];
+            }
 #pragma unroll
             for (int d = 0; d < DT; d += 2) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[(d + i) % AV], ph, acc[d + i], 0, 0, 0);
+                for (int i = 0; i < 2; i++) acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[(d + i) % AV], pd, acc[d + i], 0, 0, 0);
 #pragma unroll
                 for (int i = 0; i < 2; i++) acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[(d + i) % AV], pl, acc[d + i], 0, 0, 0);
 #pragma unroll
@@ -1222,7 +1227,7 @@ __global__ __launch_bounds__(TM_NT) void tree_attn_merge_kernel(const AttnArgs a
 }
 
 // Query rows a workgroup takes: 128 only on bf16, where a sequence fills them.
-int ta_rows(bool f32, long rows) { return f32 || rows <= 64 ? 64 : 128; }
+int ta_rows(bool f32, long rows) { return f32 || rows <= 128 ? 64 : 128; }
 
 // The workgroups of a launch, the least multiple of the CUs whose slots of n leave no more than a
 // tenth of them without work.

@@ -68,7 +68,7 @@ def test_attention_long_chains_and_small_pages(gpu, page, ctx, bf16):
 def test_attention_rows_of_all_sizes(gpu):
     """fp32 caches whose rows are of size 2^-60 or 2^60, with queries that make up for it, and of sizes 2^-15 .. 2^15 mixed,
     zeros among them: each keeps its accuracy. There the queries have no latent part, so that the scores stay small
-    and every row counts. (A value under 2^-18 of its row's largest has fewer than 22 bits in two fp16 parts.)"""
+    and every row counts."""
     rng = np.random.default_rng(SEED + 131)
     B, N, H, KL, R, ctx = 4, 3, 5, 512, 64, 90
     lens, counts = np.full(B, ctx, np.int32), np.full(B, N, np.int32)
@@ -87,6 +87,21 @@ def test_attention_rows_of_all_sizes(gpu):
     parents = random_tree(rng, B, N)
     got, lse = run_attention(gpu, q, cache, lens, counts, parents, 0.05, KL, False, False)
     check_attention(got, lse, q, cache, lens, counts, parents, 0.05, KL, False, False)
+
+
+@pytest.mark.parametrize("k", [-28, -20, -10])
+def test_attention_small_values_beside_large(gpu, k):
+    """fp32 caches whose latents are 2^k of their rope slots, and queries whose latent part makes up for half of it."""
+    rng = np.random.default_rng(SEED + 136)
+    B, N, H, KL, R, ctx = 2, 3, 5, 512, 64, 80
+    lens, counts = np.full(B, ctx, np.int32), np.full(B, N, np.int32)
+    cache = Cache(rng, B, ctx + N, 16, KL + R)
+    cache.pages[..., :KL] *= np.float32(2.0 ** k)
+    q = rng.standard_normal((B, N, H, KL + R)).astype(np.float32)
+    q[..., :KL] *= np.float32(2.0 ** (-k // 2))
+    parents = random_tree(rng, B, N)
+    got, lse = run_attention(gpu, q, cache, lens, counts, parents, 0.1, KL, False, False)
+    check_attention(got, lse, q, cache, lens, counts, parents, 0.1, KL, False, False)
 
 
 @pytest.mark.parametrize("bf16", [True, False])
