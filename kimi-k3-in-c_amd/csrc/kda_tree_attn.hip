@@ -264,6 +264,10 @@ __device__ __forceinline__ float quarter_max(float x)
 // s + 1's scores are followed by the products of step s's sum with step s + 1's softmax spread between
 // them, two or three vector instructions to a product; the barrier of a step stands before the sum's last
 // eight products, behind which the next scores' first fragments arrive.
+//
+// Measured: 4 sequences x 64 nodes x 64 heads over up to 32,768 positions 798 us, 1.24 PFLOP/s (a large library product
+// reaches 1.36), bound by the matrix cores; 64 tokens over up to 8192 positions 121 us, of which the loop 76 (6 TB/s of
+// cache), first loads 9, 42 MB of parts written and merged the rest.
 constexpr int TB_TP = 32, TB_GRP = TB_TP * 128, TB_BUF = 9 * TB_GRP, TB_NB = 4;
 constexpr int TB_LDS = TB_NB * TB_BUF + 64 + TREE_MAX * 8;
 static_assert(TB_LDS <= 160 * 1024, "LDS");
@@ -1128,18 +1132,21 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 }
 
 // The parts of a row merged, by W waves: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s, wave w the parts
-// w, w + W, ..., the waves' sums in order. Four waves a row where there are few rows, and long sequences have many parts; one
-// where there are many (16,384 rows of two parts: 40 us with four waves, 21 with one). Every part's (M_s, l_s) is asked for at once, a part a lane, and
-// the sums four parts at a time (one after the other their latencies made a merge of 16 parts 27 us). A
-// part that saw nothing (M_s = -inf) left no sums: its memory is read, its weight not used.
-constexpr int TM_NT = 256, TM_PER = 4;
+// w, w + W, ..., the waves' sums in order. Eight waves a row up to 512 rows, where long sequences have many parts each
+// (with the first launch, 64 rows of 125 parts: 28 us, 31 with four waves; of 256 parts: 34, 40), one beyond (1024 rows
+// of 17 parts: 38, 40 with eight; 16,384 rows of 3: 40 us for the merge with four waves, 21 with one). The sums are
+// asked for four parts at a time, the next four before these are added, and
+// at the start every part's (M_s, l_s), a part a lane, before they are needed: one after the other their latencies
+// made a merge of 16 parts 27 us. A part that saw nothing (M_s = -inf) left no sums: its memory is read, its
+// weight not used.
+constexpr int TM_PER = 4;
 template <int W>
-__global__ __launch_bounds__(TM_NT) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows, float up)
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows, float up)
 {
-    __shared__ float s_m[4], s_l[4];
-    __shared__ f32x4 s_v[3][TA_KL / 4];
-    const int b = blockIdx.y, lane = threadIdx.x & 63, wv = W == 4 ? threadIdx.x >> 6 : 0;
-    const int row = W == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ float s_m[W], s_l[W];
+    __shared__ f32x4 s_v[W == 1 ? 1 : W][TA_KL / 4];
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = W == 1 ? 0 : tid >> 6;
+    const int row = W == 1 ? blockIdx.x * 4 + (tid >> 6) : blockIdx.x;
     if (row >= tree_count(a.t, b) * a.H) return;
     const int rt = row / tile_rows, in = row % tile_rows;
     const int4 p = a.plan[b];
@@ -1148,8 +1155,21 @@ __global__ __launch_bounds__(TM_NT) void tree_attn_merge_kernel(const AttnArgs a
     // part s: the first slot's second part, then the others' first
     auto at = [&](int s) -> size_t { return (2 * ((size_t)(p.x + s) * p.z + rt) + (s == 0)) * tile_rows + in; };
     const int mine = n > wv ? (n - wv + W - 1) / W : 0;   // this wave's parts
+    f32x4 x[TM_PER][2];
+    auto ask = [&](int i) {   // for parts i .. i + TM_PER - 1 of this wave's
+#pragma unroll
+        for (int k = 0; k < TM_PER; k++) {
+            const float *src = a.po + at(wv + W * max(min(i + k, mine - 1), 0)) * a.KL;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int ch = 256 * c + 4 * lane;
+                x[k][c] = ch < a.KL ? *reinterpret_cast<const f32x4 *>(src + ch) : f32x4(0.0f);
+            }
+        }
+    };
     float M = -INFINITY, l = 0.0f;
     f32x4 v[2] = {f32x4(0.0f), f32x4(0.0f)};
+    if (mine > 0) ask(0);
     for (int i0 = 0; i0 < mine; i0 += 64) {
         const bool has = i0 + lane < mine;
         const size_t pa = at(wv + W * (has ? i0 + lane : 0));
@@ -1157,7 +1177,6 @@ __global__ __launch_bounds__(TM_NT) void tree_attn_merge_kernel(const AttnArgs a
         float mx = m;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-        if (mx == -INFINITY) continue;
         const float mn = fmaxf(M, mx), old = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
         const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
         float ls = w == 0.0f ? 0.0f : w * pl;
@@ -1168,65 +1187,61 @@ __global__ __launch_bounds__(TM_NT) void tree_attn_merge_kernel(const AttnArgs a
         v[1] *= old;
         M = mn;
         for (int i = 0; i < min(64, mine - i0); i += TM_PER) {
-            f32x4 x[TM_PER][2];
-            float ws[TM_PER];
-#pragma unroll
-            for (int k = 0; k < TM_PER; k++) {
-                const bool ok = i0 + i + k < mine;
-                ws[k] = ok ? __shfl(w, i + k, 64) : 0.0f;
-                const float *src = a.po + at(wv + W * (ok ? i0 + i + k : i0 + i)) * a.KL;
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const int ch = 256 * c + 4 * lane;
-                    x[k][c] = ch < a.KL ? *reinterpret_cast<const f32x4 *>(src + ch) : f32x4(0.0f);
-                }
-            }
+            f32x4 y[TM_PER][2];
 #pragma unroll
             for (int k = 0; k < TM_PER; k++)
-                if (ws[k] != 0.0f) {
-                    v[0] += ws[k] * x[k][0];
-                    v[1] += ws[k] * x[k][1];
+#pragma unroll
+                for (int c = 0; c < 2; c++) y[k][c] = x[k][c];
+            if (i0 + i + TM_PER < mine) ask(i0 + i + TM_PER);
+#pragma unroll
+            for (int k = 0; k < TM_PER; k++) {
+                const float ws = __shfl(w, i + k, 64);   // zero past the last
+                if (ws != 0.0f) {
+                    v[0] += ws * y[k][0];
+                    v[1] += ws * y[k][1];
                 }
+            }
         }
     }
     float Mx = M;
-    f32x4 t[2] = {v[0], v[1]};
-    if constexpr (W == 4) {
+    if constexpr (W > 1) {
         if (lane == 0) {
             s_m[wv] = M;
             s_l[wv] = l;
         }
-        if (wv > 0) {
-            s_v[wv - 1][lane] = v[0];
-            s_v[wv - 1][64 + lane] = v[1];
-        }
+        s_v[wv][lane] = v[0];
+        s_v[wv][64 + lane] = v[1];
         __syncthreads();
-        if (wv > 0) return;
-        Mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-        l = 0.0f;
-        t[0] = t[1] = f32x4(0.0f);
+        if (wv > 1) return;   // wave c takes channels 256 c .. + 255
+        Mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < W; k++) Mx = fmaxf(Mx, s_m[k]);
+        l = 0.0f;
+        v[0] = v[1] = f32x4(0.0f);
+#pragma unroll
+        for (int k = 0; k < W; k++) {
             if (s_m[k] == -INFINITY) continue;
             const float w = __builtin_amdgcn_exp2f(s_m[k] - Mx);
             l += w * s_l[k];
-            t[0] += w * (k ? s_v[k ? k - 1 : 0][lane] : v[0]);
-            t[1] += w * (k ? s_v[k ? k - 1 : 0][64 + lane] : v[1]);
+            v[0] += w * s_v[k][64 * wv + lane];
         }
+        v[1] = v[0];
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const size_t orow = (size_t)b * a.t.N * a.H + row;
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         const int ch = 256 * c + 4 * lane;
-        if (ch >= a.KL) continue;
-        if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * a.KL + ch) = t[c] * inv;
-        else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * a.KL + ch) = pack4(t[c] * inv);
+        if (ch >= a.KL || (W > 1 && c != wv)) continue;
+        if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * a.KL + ch) = v[c] * inv;
+        else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * a.KL + ch) = pack4(v[c] * inv);
     }
-    if (a.lse && lane == 0) a.lse[orow] = l == 0.0f ? -INFINITY : (Mx - up + __builtin_amdgcn_logf(l)) * TA_LN2;
+    if (a.lse && lane == 0 && wv == 0) a.lse[orow] = l == 0.0f ? -INFINITY : (Mx - up + __builtin_amdgcn_logf(l)) * TA_LN2;
 }
 
-// Query rows a workgroup takes: 128 only on bf16, where a sequence fills them.
+// Query rows a workgroup takes: 128 on bf16 where a sequence has more (64 and 128 measured: 64 sequences of 128 rows
+// 150 and 157 us, of 256 rows 270 and 240, 4 of 4096 rows 997 and 798): half the LDS reads a product, but larger
+// parts.
 int ta_rows(bool f32, long rows) { return f32 || rows <= 128 ? 64 : 128; }
 
 // The workgroups of a launch, the least multiple of the CUs whose slots of n leave no more than a
@@ -1326,7 +1341,8 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     a.pm = (float *)((char *)workspace + up256(r * kv_lora * 4));
     a.pl = (float *)((char *)a.pm + up256(r * 4));
     a.plan = (int4 *)((char *)a.pl + up256(r * 4));
-    // bf16: whole rows of eight in one page go by buffer loads
+    // bf16: eight rows of full width in one page go by buffer loads from one address (otherwise an address a lane, by
+    // global loads: 830 us for 798 at 4 sequences of 64 nodes over 32,768 positions, 125 for 121 at 64 tokens over 8192)
     const void *kern;
     const size_t lds = f32 ? TS_LDS : TB_LDS;
     if (f32) kern = CW == TA_CW ? (const void *)tree_attn32_kernel<true> : (const void *)tree_attn32_kernel<false>;
@@ -1338,10 +1354,10 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     K3_HIP(hipLaunchKernel(kern, dim3((unsigned)grid), dim3(f32 ? TS_NT : TA_NT), args, lds, st));
     K3_LAUNCHED();
     const float up = f32 ? TS_UP : 0.0f;
-    if ((long)B * N * H <= 2048)
-        hipLaunchKernelGGL((tree_attn_merge_kernel<4>), dim3((unsigned)(N * H), (unsigned)B), dim3(TM_NT), 0, st, a, rows, up);
+    if ((long)B * N * H <= 512)
+        hipLaunchKernelGGL((tree_attn_merge_kernel<8>), dim3((unsigned)(N * H), (unsigned)B), dim3(512), 0, st, a, rows, up);
     else
-        hipLaunchKernelGGL((tree_attn_merge_kernel<1>), dim3((unsigned)((N * H + 3) / 4), (unsigned)B), dim3(TM_NT), 0, st, a, rows, up);
+        hipLaunchKernelGGL((tree_attn_merge_kernel<1>), dim3((unsigned)((N * H + 3) / 4), (unsigned)B), dim3(256), 0, st, a, rows, up);
     K3_LAUNCHED();
     return K3HIP_OK;
 }
