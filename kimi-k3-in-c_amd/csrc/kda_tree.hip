@@ -100,6 +100,7 @@ struct alignas(16) TreeLds {
     };
     float beta[R];
     uint64_t anc[R];   // the node and its ancestors, a bit each
+    uint64_t bad[D];   // [value column] the nodes whose w is not finite there
     uint32_t up[R];    // the node, its parent, the parent's and the one after, a byte each; 0x80 + i: i back in the history
 };
 
@@ -343,8 +344,10 @@ __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tre
     for (int e = 0; e < CPL; e++) on[e] = a.o_norm[cl + e];
 
     // forward substitution, a thread per value column, 16 rows at a time in registers: w_m = rhs_m - sum_j
-    // beta_m A_mj w_j
+    // beta_m A_mj w_j. A w that is not finite is noted and taken as zero: zeros of A would spread it to nodes
+    // that do not follow it, and those that do are set below.
     if (tid < D) {
+        uint64_t bad = 0;
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
             float w[16];
@@ -357,7 +360,10 @@ __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tre
                 for (int i = 0; i < 16; i++) w[i] = __builtin_fmaf(-Aj[i], x, w[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 15; i++) {
+            for (int i = 0; i < 16; i++) {
+                const bool inf = !(fabsf(w[i]) < INFINITY);
+                bad |= (uint64_t)inf << (16 * t + i);
+                w[i] = inf ? 0.0f : w[i];
                 const float *Ai = s.A + (16 * t + i) * AP + 16 * t;
 #pragma unroll
                 for (int q = (i + 1) / 4; q < 4; q++) {
@@ -370,10 +376,12 @@ __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tre
 #pragma unroll
             for (int i = 0; i < 16; i++) s.a[(16 * t + i) * DP + tid] = w[i];
         }
+        s.bad[tid] = bad;
     }
     __syncthreads();
 
     // o = (E q)^T S_0 + A_qk w, into s.v
+    const uint64_t bad = s.bad[16 * wv + c16];
 #pragma unroll
     for (int t = 0; t < TILES; t++) {
 #pragma unroll
@@ -383,7 +391,10 @@ __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tre
             oq[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f, s.a[j * DP + 16 * wv + c16], oq[t], 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) s.v[(16 * t + 4 * kq + i) * DP + 16 * wv + c16] = oq[t][i];
+        for (int i = 0; i < 4; i++) {
+            const int n = 16 * t + 4 * kq + i;
+            s.v[n * DP + 16 * wv + c16] = s.anc[n] & bad ? NAN : oq[t][i];
+        }
     }
     __syncthreads();
 

@@ -233,3 +233,37 @@ def test_graphs_side_by_side(gpu, bf16):
         torch.cuda.synchronize()
         for i in range(4):
             assert torch.equal(o[i], want[i]), f"graph {i} in round {step}"
+
+
+# -------------------------------------------------------- not finite nodes ----
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+@pytest.mark.parametrize("name", ["k", "v", "z", "b"])
+@pytest.mark.parametrize("D,N", [(128, 12), (64, 40), (16, 20)])
+def test_kda_nodes_that_are_not_finite(gpu, D, N, name, what):
+    """A node whose inputs hold an infinity or a NaN: nodes that do not follow it are as without it, and so is a commit
+    along another branch."""
+    import torch
+    rng = np.random.default_rng(SEED + 181 + D)
+    B, H, K, lb, eps, qs = 1, 2, 4, -5.0, 1e-5, float(np.float32(D ** -0.5))
+    w, x, S0, h0 = kda_case(rng, B, N, H, D, K, lb, False, False)
+    parents = np.arange(N, dtype=np.int32)[None] - 2   # two branches, a node of each in turn
+    parents[0][:6] = [-1, 0, 1, 1, 3, 2]
+    hit = np.array([2 in path_of(parents[0], n) for n in range(N)])
+    assert hit.sum() >= 2 and (~hit[3:]).sum() >= 3
+    clean = {n: a.copy() for n, a in x.items()}
+    x[name][0, 2, ::3] = what
+    accept = int(np.flatnonzero(~hit)[-1])
+    ins, ws, o_norm = kda_inputs(w, x, False)
+    S, hist, y = cu(S0), cu(h0), torch.zeros((B, N, H * D), device="cuda")
+    kw = {"parents": cu(parents)}
+    gpu.kda_tree_step(*ins, cu(x["gate"]), *ws, o_norm, hist, S, y, H, D, K, lb, eps, qs, **kw)
+    gpu.kda_tree_commit(*ins, *ws, hist, S, cu(np.array([accept], np.int32)), H, D, K, lb, **kw)
+    torch.cuda.synchronize()
+    ref = Kda(w, H, D, K, lb, eps, qs)
+    want, states = ref.step({n: a[0] for n, a in clean.items()}, N, parents[0], S0[0], h0[0])
+    got = host(y)[0]
+    assert_close(got[~hit], want[~hit], 1e-4 * np.sqrt(np.mean(want ** 2)), 1e-4, "y")
+    if what is np.nan:
+        assert np.isnan(got[2]).any(), "the node itself"
+    st = states[accept]
+    assert_close(host(S)[0], st, 1e-4 * np.sqrt(np.mean(st ** 2)), 1e-4, "S")
