@@ -309,6 +309,8 @@ extern "C" int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pa
               q_head < rope || q_out_head < rope || rope == 0))
         K3_FAIL(K3HIP_EINVAL, "%s: queries H=%d dtypes %d -> %d, head strides %ld -> %ld, rope=%d", who, H, q_dtype,
                 q_out_dtype, q_head, q_out_head, rope);
+    if (q && (long)B * N > 1 && q_out_ld < rope)
+        K3_FAIL(K3HIP_EINVAL, "%s: rows of rotated queries %ld elements apart", who, q_out_ld);
     if (B == 0 || N == 0) return K3HIP_OK;
     if (!rows || rows_ld < kv_lora + rope) K3_FAIL(K3HIP_EINVAL, "%s: rows NULL or stride %ld", who, rows_ld);
     AppendArgs a{};

@@ -110,3 +110,8 @@ def test_binding_refuses_host_and_misshapen_tensors():
         k3kda.mla_tree_attention(z(1, 2, 3, 72), z(2, 16, 72).bfloat16(), z(1, 1), z(1), z(1, 2, 3, 64), 64, 0.1)
     with pytest.raises(ValueError):
         k3kda.latent_commit(z(2, 16, 72), z(1, 1), z(1), z(1), 2)
+
+
+def test_rotated_queries_that_overlap_are_refused():
+    rc, msg = call("k3hip_latent_append", APPEND, q_out_ld=63)
+    assert rc == k3kda.EINVAL and msg.startswith("k3hip_latent_append")
