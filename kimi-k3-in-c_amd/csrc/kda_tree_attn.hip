@@ -159,13 +159,21 @@ __device__ __forceinline__ uint2 pack4(const f32x4 &v)
     return uint2{__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y)};
 }
 
-// Which workgroup takes what. All sequences' steps stand on one axis, cut into equal slots; a slot takes the n
+// Which workgroup takes what. All sequences' steps stand on one axis, cut into slots; a slot takes the n
 // workgroups that the most row tiles of a sequence need, one each, so the workgroups of a slot walk the same
 // positions (and stand on one XCD, where they share its L2), and sequences of different lengths cost no
 // one a wait. A slot that ends inside a sequence leaves that sequence's sums as a part, merged after.
+//
+// The slots end where sequences end, each of at most L steps, if that takes no more slots than there are and
+// L is at most `over` steps over the average: a slot that goes on into a second sequence reads its queries and fills its
+// pipeline anew, and leaves two parts. Otherwise the axis is cut into equal slots. (Equal slots, and this, bf16: 16
+// sequences of one token over up to 1024 positions 37.5 and 31.5 us, of 8 tokens 66 and 52, 64 of one over up to
+// 8192 118 and 113; fp32: 4 of 8 tokens over up to 2000 70 and 58. With a step of fp32 at 3.7 us, four more than
+// the average cost more than they save: 7 of 13 tokens 144 and 152.)
+constexpr int TB_OVER = 6, TS_OVER = 2;
 struct Slots {
-    int n, count;   // workgroups a slot, slots
-    int steps;      // of all sequences (the host checks that this fits an int)
+    int n;          // workgroups a slot
+    int from, to;   // the slot's steps on the axis
 };
 
 // Sequence b's row tiles (of `rows` rows) and steps (of `tp` positions).
@@ -176,25 +184,19 @@ __device__ __forceinline__ void seq_size(const AttnArgs &a, int b, int rows, int
     steps = cnt ? (paged_len(a.c, a.t.lens, b) + cnt + tp - 1) / tp : 0;
 }
 
-__device__ __forceinline__ int slot_start(const Slots &s, int k) { return (int)((uint64_t)s.steps * (uint32_t)k / (uint32_t)s.count); }
-__device__ __forceinline__ int slot_of(const Slots &s, int step) { return (int)(((uint64_t)(step + 1) * (uint32_t)s.count - 1) / (uint32_t)s.steps); }
-
-// The slots, and the sequence b that step `slot_start` of workgroup id's slot lies in, with the step that
+// Workgroup id's slot, and the sequence b that it begins in, with the step of the axis that
 // sequence begins at; every wave works it out for itself, a sequence a lane. Workgroup 0 writes down for the
 // merge which slots each sequence begins and ends in.
-__device__ __forceinline__ bool find_slot(const AttnArgs &a, int rows, int tp, int id, int most, Slots &s, int &b, int &begin)
+__device__ __forceinline__ bool find_slot(const AttnArgs &a, int rows, int tp, int over, int id, int most, Slots &s, int &b, int &begin)
 {
     const int lane = threadIdx.x & 63;
-    int n = 0, nrt0 = 0, steps0 = 0, T = 0;
+    int n = 0, steps0 = 0, T = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int nrt = 0, steps = 0;
         if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
         n = max(n, nrt);
         T += steps;
-        if (b0 == 0) {
-            nrt0 = nrt;
-            steps0 = steps;
-        }
+        if (b0 == 0) steps0 = steps;
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
@@ -204,39 +206,66 @@ __device__ __forceinline__ bool find_slot(const AttnArgs &a, int rows, int tp, i
     n = __builtin_amdgcn_readfirstlane(n);
     if (n == 0) return false;
     s.n = n;
-    s.steps = __builtin_amdgcn_readfirstlane(T);
-    s.count = min(max(1, most / n), s.steps);
+    T = __builtin_amdgcn_readfirstlane(T);   // the host checks that it fits an int
+    int count = min(max(1, most / n), T), L = 0;   // slots; their most steps, 0: equal slots
+    if (a.B > 1 && a.B <= 64 && count < 0x8000) {
+        const int avg = (T + count - 1) / count;
+        const int l[4] = {avg, avg + 1, avg + over / 2, avg + over};
+        uint32_t sum[2];   // of the slots that each needs: at most T / l + 64, two a register
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            sum[i] = (uint32_t)((steps0 + l[2 * i] - 1) / l[2 * i]) | (uint32_t)((steps0 + l[2 * i + 1] - 1) / l[2 * i + 1]) << 16;
+#pragma unroll
+            for (int m = 32; m >= 1; m >>= 1) sum[i] += (uint32_t)__shfl_xor((int)sum[i], m, 64);
+        }
+#pragma unroll
+        for (int i = 3; i >= 0; i--) L = (int)(sum[i >> 1] >> (16 * (i & 1)) & 0xffff) <= count ? l[i] : L;
+        L = __builtin_amdgcn_readfirstlane(L);
+    }
     const int k = id / n;
-    if (k >= s.count) return false;
-    const int from = slot_start(s, k);
-    int base = 0;
+    if (k >= count) return false;
+    s.from = (int)((uint64_t)T * (uint32_t)k / (uint32_t)count);
+    s.to = (int)((uint64_t)T * (uint32_t)(k + 1) / (uint32_t)count);
+    auto slot_of = [&](int step) { return (int)(((uint64_t)(step + 1) * (uint32_t)count - 1) / (uint32_t)T); };
+    int base = 0, base_slot = 0;   // steps and slots of the sequences before
     bool found = false;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        int nrt = nrt0, steps = steps0;
+        int nrt = 0, steps = steps0;
         if (b0 > 0) {
             steps = 0;
             if (b0 + lane < a.B) seq_size(a, b0 + lane, rows, tp, nrt, steps);
         }
-        int end = steps;
+        const int mine = L ? (steps + L - 1) / L : 0;
+        int end = steps, end_slot = mine;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
-            const int x = __shfl_up(end, m, 64);
-            if (lane >= m) end += x;
+            const int x = __shfl_up(end, m, 64), y = __shfl_up(end_slot, m, 64);
+            if (lane >= m) {
+                end += x;
+                end_slot += y;
+            }
         }
-        const int first = base + end - steps;
+        const int first = base + end - steps, first_slot = base_slot + end_slot - mine;
         if (id == 0 && threadIdx.x < 64 && b0 + lane < a.B && steps)
-            a.plan[b0 + lane] = int4{slot_of(s, first), slot_of(s, first + steps - 1), n, 0};
-        const uint64_t in = __ballot(from >= first && from < first + steps);
+            a.plan[b0 + lane] = L ? int4{first_slot, first_slot + mine - 1, n, 0} : int4{slot_of(first), slot_of(first + steps - 1), n, 0};
+        const uint64_t in = L ? __ballot(k >= first_slot && k < first_slot + mine) : __ballot(s.from >= first && s.from < first + steps);
         if (in && !found) {
-            const int l = __builtin_ctzll(in);
-            b = b0 + l;
-            begin = __builtin_amdgcn_readlane(first, l);
+            const int at = __builtin_ctzll(in);
+            b = b0 + at;
+            begin = __builtin_amdgcn_readlane(first, at);
+            if (L) {
+                const int all = __builtin_amdgcn_readlane(steps, at), of = __builtin_amdgcn_readlane(mine, at);
+                const int place = k - __builtin_amdgcn_readlane(first_slot, at);
+                s.from = begin + (int)((uint64_t)all * (uint32_t)place / (uint32_t)of);
+                s.to = begin + (int)((uint64_t)all * (uint32_t)(place + 1) / (uint32_t)of);
+            }
             found = true;
             if (id != 0) break;
         }
         base += __builtin_amdgcn_readlane(end, 63);
+        base_slot += __builtin_amdgcn_readlane(end_slot, 63);
     }
-    return true;
+    return found;   // with L there can be slots to spare
 }
 
 // x, worked out anew from here on: what the compiler would else keep in registers over the whole loop.
@@ -286,10 +315,10 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
     const int H = a.H, CW = FAST ? TA_CW : a.CW, KL = a.KL;
     Slots sl;
     int seq = 0, begin = 0;
-    if (!find_slot(a, ROWS, TB_TP, id, gridDim.x, sl, seq, begin)) return;
-    const int slot = id / sl.n, rt = id - slot * sl.n;
-    const int to = slot_start(sl, slot + 1);
-    int from = slot_start(sl, slot);
+    if (!find_slot(a, ROWS, TB_TP, TB_OVER, id, gridDim.x, sl, seq, begin)) return;
+    const int rt = id % sl.n;   // its row tile
+    const int to = sl.to;
+    int from = sl.from;
     for (int b = seq; from < to; b++) {
         const int cnt = tree_count(a.t, b), rows = cnt * H, r0 = rt * ROWS;
         const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
@@ -786,10 +815,10 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     const int H = a.H, CW = FULL ? TA_CW : a.CW, KL = a.KL;
     Slots sl;
     int seq = 0, begin = 0;
-    if (!find_slot(a, ROWS, TB_TP, id, gridDim.x, sl, seq, begin)) return;
-    const int slot = id / sl.n, rt = id - slot * sl.n;
-    const int to = slot_start(sl, slot + 1);
-    int from = slot_start(sl, slot);
+    if (!find_slot(a, ROWS, TB_TP, TS_OVER, id, gridDim.x, sl, seq, begin)) return;
+    const int rt = id % sl.n;   // its row tile
+    const int to = sl.to;
+    int from = sl.from;
     for (int b = seq; from < to; b++) {
         const int cnt = tree_count(a.t, b), rows = cnt * H, r0 = rt * ROWS;
         const int len = paged_len(a.c, a.t.lens, b), end = len + cnt;
