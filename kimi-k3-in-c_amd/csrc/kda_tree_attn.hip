@@ -9,7 +9,7 @@
 // its cache: bytes bind for one node, the matrix cores from a few nodes on.
 //
 //  * A workgroup owns a tile of query rows and a range of steps of 32 positions, which it walks once; all
-//    sequences' steps stand on one axis that is cut into equal ranges, one for as many workgroups as the largest
+//    sequences' steps stand on one axis that is cut into ranges, one for as many workgroups as the largest
 //    sequence has row tiles (find_slot). A range that ends inside a sequence leaves unnormalised sums with (M, l); a
 //    second launch merges them in order, so results do not depend on timing.
 //  * Scores^T (positions x query rows), the softmax in base 2 and o^T (latent channels x query rows) += latents^T . p.
@@ -295,8 +295,8 @@ __device__ __forceinline__ float quarter_max(float x)
 // eight products, behind which the next scores' first fragments arrive.
 //
 // Measured: 4 sequences x 64 nodes x 64 heads over up to 32,768 positions 798 us, 1.24 PFLOP/s (a large library product
-// reaches 1.36), bound by the matrix cores; 64 tokens over up to 8192 positions 121 us, of which the loop 76 (6 TB/s of
-// cache), first loads 9, 42 MB of parts written and merged the rest.
+// reaches 1.36), bound by the matrix cores; 64 tokens over up to 8192 positions 113 us, of which the loop 76 (6 TB/s of
+// cache), first loads 9, 33 MB of parts written and merged most of the rest.
 constexpr int TB_TP = 32, TB_GRP = TB_TP * 128, TB_BUF = 9 * TB_GRP, TB_NB = 4;
 constexpr int TB_LDS = TB_NB * TB_BUF + 64 + TREE_MAX * 8;
 static_assert(TB_LDS <= 160 * 1024, "LDS");
@@ -734,11 +734,11 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 //
 // A step is 32 positions, staged as two planes of column groups as in the bf16 kernel, two buffers. Eight
 // waves, two a SIMD: waves w and w + 4 own 16 query rows; each scores half of the cache row's channels (so it holds half
-// of the query's hi + lo, 72 registers), they add their halves through LDS, both work out the softmax, and each sums half of the
-// latent's channels (64 registers). A step has two barriers, behind the halves of the scores and behind the
+// of the query's hi + lo, 72 registers), they add their halves through LDS, both work out the softmax, and each sums half of
+// the latent's channels (64 registers). A step has two barriers, behind the halves of the scores and behind the
 // sum; a wave keeps 4 rows on their way to registers and converts and stages them, a column group at a time, between the
 // products: groups 4 .. 8 beside the scores, where groups 0 .. 3 of the buffer carry the halves, those beside the sum.
-// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 140 us with the merge, 200 TFLOP/s of the fp32 work, 3.3k
+// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 144 us with the merge, 195 TFLOP/s of fp32 work, 3.3k
 // of a step's 8.7k cycles matrix instructions and 3.4k LDS accesses; what binds is the wait of two waves in step for
 // LDS fragments (registers allow one K-step of look-ahead), the hand-over (800 cycles) and the softmax (700). With
 // four waves of whole rows, one a SIMD, 238 us: nothing stood beside their waits, and they spilled.
@@ -1371,7 +1371,7 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     a.pl = (float *)((char *)a.pm + up256(r * 4));
     a.plan = (int4 *)((char *)a.pl + up256(r * 4));
     // bf16: eight rows of full width in one page go by buffer loads from one address (otherwise an address a lane, by
-    // global loads: 830 us for 798 at 4 sequences of 64 nodes over 32,768 positions, 125 for 121 at 64 tokens over 8192)
+    // global loads: 830 us for 798 at 4 sequences of 64 nodes over 32,768 positions, 4% more at 64 tokens over 8192)
     const void *kern;
     const size_t lds = f32 ? TS_LDS : TB_LDS;
     if (f32) kern = CW == TA_CW ? (const void *)tree_attn32_kernel<true> : (const void *)tree_attn32_kernel<false>;
