@@ -224,7 +224,8 @@ __global__ __launch_bounds__(AP_NT) void latent_append_kernel(const AppendArgs a
 // A destination may be another node's source, so a workgroup holds what it moves in registers, UM units
 // of U a thread, and stores after a barrier; wider paths go in blocks of columns, whose units never
 // meet. A row whose source or destination has no page stays. Latency bound (one table
-// lookup, one load, one store): 4.2 us for 64 sequences of 16 nodes and for one of 64.
+// lookup, one load, one store): 3.9 us for 64 sequences of 16 nodes, 3.4 for one of 64 (4.3 with units of the
+// runtime's vector type, which went through scratch memory).
 constexpr int CM_NT = 512, CM_UM = 8;
 template <typename U>
 __global__ __launch_bounds__(CM_NT) void latent_commit_kernel(TreeSeqs t, PagedRows c, U *pages, int units,
@@ -352,7 +353,7 @@ extern "C" int k3hip_latent_commit(int B, int N, int width, void *pages, int dty
     const PagedRows c{table, n_pages, page, max_pages};
 #define K3_CM(U) hipLaunchKernelGGL((latent_commit_kernel<U>), dim3(B), dim3(CM_NT), 0, as_stream(stream), t, c, \
                                     reinterpret_cast<U *>(pages), (int)(bytes / sizeof(U)), accept, lens_out)
-    if (bytes % 16 == 0 && !((uintptr_t)pages & 15)) K3_CM(uint4);
+    if (bytes % 16 == 0 && !((uintptr_t)pages & 15)) K3_CM(f4);
     else if (dtype == K3HIP_F32) K3_CM(uint32_t);
     else K3_CM(uint16_t);
 #undef K3_CM
