@@ -284,6 +284,11 @@ __device__ __forceinline__ float quarter_max(float x)
     return fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 }
 
+// The largest score M that a part is merged by, l its sum of weights. Maxima pass over NaNs, so a part that
+// saw a NaN can have any M, -inf if it saw nothing else: it gets +inf, which makes its weight in the merge,
+// 2^(inf - inf), and with it the row NaN whatever the other parts hold.
+__device__ __forceinline__ float part_max(float M, float l) { return l != l ? INFINITY : M; }
+
 // bf16 caches. A step is 32 positions, staged as nine column groups [32 rows][8 units of 16 bytes] so that one
 // load of 64 lanes fills 8 rows of a group and a lane's row, unit and swizzle are the same in all of
 // them: one row address a lane and step, the groups by immediate offset. Four buffers: while step s is
@@ -696,11 +701,12 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
             const int q4 = (opaque(tid) & 63) >> 4;
             const size_t orow = (size_t)b * a.t.N * H + row, prow = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
             if (split) {
+                const float m = part_max(M[r], l);
                 if (q4 == 0) {
-                    a.pm[prow] = M[r];
+                    a.pm[prow] = m;
                     a.pl[prow] = l;
                 }
-                if (M[r] == -INFINITY) continue;   // nothing seen: the merge does not read its sums
+                if (m == -INFINITY) continue;   // nothing seen: the merge does not read its sums
                 float *dst = a.po + prow * KL + 4 * q4;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
@@ -1133,11 +1139,12 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         const size_t orow = (size_t)b * a.t.N * H + row, part = ((size_t)2 * id + (s0 == 0)) * ROWS + (row - r0);
         const int ch = 16 * DT * half + 4 * kq;   // this lane's first channels
         if (split) {
+            const float m = part_max(M, lsum);
             if (kq == 0 && half == 0) {
-                a.pm[part] = M;
+                a.pm[part] = m;
                 a.pl[part] = lsum;
             }
-            if (M == -INFINITY) continue;   // nothing seen: the merge does not read its sums
+            if (m == -INFINITY) continue;   // nothing seen: the merge does not read its sums
             float *dst = a.po + part * KL + ch;
 #pragma unroll
             for (int d = 0; d < DT; d++)
@@ -1167,7 +1174,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 // asked for four parts at a time, the next four before these are added, and
 // at the start every part's (M_s, l_s), a part a lane, before they are needed: one after the other their latencies
 // made a merge of 16 parts 27 us. A part that saw nothing (M_s = -inf) left no sums: its memory is read, its
-// weight not used.
+// weight not used. One that saw a NaN (M_s = inf) makes the row NaN.
 constexpr int TM_PER = 4;
 template <int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows, float up)
