@@ -68,6 +68,7 @@ struct AttnArgs {
     uint32_t page_bytes;
     int tcol, trow;        // a step in table columns and rows
     float *po, *pm, *pl;   // parts, two a workgroup [rows of a tile] ( x KL): their sums, M and l
+    float *pr;             // fp32 caches: what l is taken against (bf16: M)
     int4 *plan;            // [B] first and last slot, workgroups a slot
 };
 
@@ -734,9 +735,12 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // two that puts its largest value just under 2^15 and split into fp16 hi + 2^-11 lo, 22 bits together (down to
 // 2^-29 of the row's largest value; what is left out is under 2^-51 of it), and hi hi + hi lo + lo hi are summed in
 // fp32, three matrix instructions where six are needed on bf16 parts and sixteen times the rate of the fp32
-// instruction. A cache row's scale 2^k goes with its weight: the reference that weights are taken
-// against is the largest of (score - k), so the scaled weight 2^(score - k - M) is at most 2^(TS_UP + TA_LAZY) whatever
-// the rows' sizes, and the sum of the weights takes the 2^k back out.
+// instruction. A cache row's scale 2^k goes with its weight: the reference that the second product's weights are taken
+// against is the largest of (score - k), so the scaled weight 2^(score - k - M + TS_UP) is at most 2^(TS_UP + TA_LAZY)
+// whatever the rows' sizes. The sum of the weights is that of 2^(score - R) with R the largest score itself: a sum of
+// the scaled weights with their 2^k taken back out leaves fp32's range where rows are tiny, and loses the weights of
+// rows that are tiny beside others. M and R are whole numbers, so that one weight is the other times 2^-k and
+// 2^(R - M + TS_UP), exactly, and the output takes 2^(M - TS_UP - R) back out at the end.
 //
 // A step is 32 positions, staged as two planes of column groups as in the bf16 kernel, two buffers. Eight
 // waves, two a SIMD: waves w and w + 4 own 16 query rows; each scores half of the cache row's channels (so it holds half
@@ -751,7 +755,11 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 constexpr int TS_BUF = 2 * TB_BUF;
 constexpr int TS_NT = 512;
 constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 8 + 64 + TREE_MAX * 8;
-constexpr float TS_UP = 7.0f;     // log2 of the weight of the reference
+constexpr int TS_UP = 7;          // log2 of the weight of the reference
+// The largest scale of a row: R - M + TS_UP is at most TS_KMAX + 1 + TA_LAZY + TS_UP, an exponent of fp32 (and at least
+// -116: a scale is at least 2^-114). A row under 2^-96 stays further under 2^15, and its values are whole
+// multiples of 2^-145 rather than 22 bits.
+constexpr int TS_KMAX = 110;
 constexpr float TS_LO = 2048.0f;  // what lo parts are scaled by
 static_assert(TS_LDS <= 160 * 1024, "LDS");
 
@@ -794,10 +802,13 @@ __device__ __forceinline__ void split4(const f4 &x, float scale, uint2 &hi, uint
         : "v"(x.x), "v"(x.y), "v"(x.z), "v"(x.w), "v"(scale), "s"(TS_LO));
 }
 
+// 2^(x + add), x a whole number (of a row that has seen nothing, or an infinity: any).
+__device__ __forceinline__ float exp2_int(float x, int add) { return __builtin_amdgcn_ldexpf(1.0f, (int)x + add); }
+
 // The power of two that a row whose largest magnitude has these bits is scaled by.
 __device__ __forceinline__ int row_scale(uint32_t most)
 {
-    return most == 0 ? 0 : min(14 - ((int)(most >> 23) - 127), 126);
+    return most == 0 ? 0 : min(14 - ((int)(most >> 23) - 127), TS_KMAX);
 }
 
 // Behind it every wave's LDS accesses before it; loads to registers stay on their way.
@@ -973,7 +984,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             return reinterpret_cast<f4 *>(smem + ((s + 1) & 1) * TS_BUF + TB_GRP * 2 * i + (t >> 5 & 1) * TB_GRP + 512 * w + 16 * (t & 31));
         };
         f32x4 acc[DT];
-        float M = -INFINITY, lsum = 0.0f;
+        float M = -INFINITY, Rf = -INFINITY, lsum = 0.0f;   // references of the sums and of the weights
 #pragma unroll
         for (int d = 0; d < DT; d++) acc[d] = 0.0f;
         if (tid < 64) s_anc[lane] = tree_ancestors(par);
@@ -1053,7 +1064,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             const uint64_t *okw = reinterpret_cast<const uint64_t *>(s_ok) + 2 * (s & 1);
             const uint64_t ok = okw[0], bad = okw[1];
             lds_barrier();
-            float y[8];   // scores in base 2 less k
+            float y[8];   // scores in base 2
             f4 other[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) other[i] = *half_at(s, wv, i, ht);
@@ -1061,7 +1072,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[4 * i + e] = __builtin_fmaf(S[i][e] + other[i][e], k[4 * i + e].x, -k[4 * i + e].y);
+                for (int e = 0; e < 4; e++) y[4 * i + e] = (S[i][e] + other[i][e]) * k[4 * i + e].x;
             if (ok != 0x0f0f0f0f0f0f0f0full || (s + 1) * TB_TP > len) {
                 const int n0 = len - s * TB_TP;   // place of the first node in the step
                 const int q4 = opaque(tid) >> 4 & 3, row = r0 + 16 * (wv & 3) + (opaque(tid) & 15);
@@ -1076,25 +1087,31 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
                     y[x] = (w >> bit & 1) && (ok >> byte & 1) ? y[x] + seen : -INFINITY;
                 }
             }
-            float mt = -INFINITY;
+            float mt = -INFINITY, rt = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 8; x++) mt = fmaxf(mt, y[x]);
+            for (int x = 0; x < 8; x++) {
+                mt = fmaxf(mt, y[x] - k[x].y);
+                rt = fmaxf(rt, y[x]);
+            }
             mt = quarter_max(mt);
-            if (__ballot(mt > M + TA_LAZY)) {
-                const float mn = mt > M + TA_LAZY ? mt : M;
+            rt = quarter_max(rt);
+            if (__ballot(mt > M + TA_LAZY || rt > Rf + TA_LAZY)) {
+                const float mn = mt > M + TA_LAZY ? ceilf(mt) : M, rn = rt > Rf + TA_LAZY ? ceilf(rt) : Rf;
                 const float al = mn == M ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+                lsum *= rn == Rf ? 1.0f : __builtin_amdgcn_exp2f(Rf - rn);
                 M = mn;
-                lsum *= al;
+                Rf = rn;
 #pragma unroll
                 for (int d = 0; d < DT; d++) acc[d] *= al;
             }
-            const float ref = M == -INFINITY ? 0.0f : M - TS_UP;
+            const float ref = Rf == -INFINITY ? 0.0f : Rf, up = exp2_int(Rf - M, TS_UP);
             f16x8 ph, pl;
             float pw[8];
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                pw[x] = __builtin_amdgcn_exp2f(y[x] - ref);
-                lsum = __builtin_fmaf(pw[x], __uint_as_float(0x7f000000u - __float_as_uint(k[x].x)), lsum);   // times 2^k
+                const float p = __builtin_amdgcn_exp2f(y[x] - ref);
+                lsum += p;
+                pw[x] = p * k[x].x * up;   // the second factor first: p 2^-k is at most 2^122
             }
             f16x8 pd;   // for the rows' lo parts
 #pragma unroll
@@ -1142,6 +1159,7 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             const float m = part_max(M, lsum);
             if (kq == 0 && half == 0) {
                 a.pm[part] = m;
+                a.pr[part] = part_max(Rf, lsum);
                 a.pl[part] = lsum;
             }
             if (m == -INFINITY) continue;   // nothing seen: the merge does not read its sums
@@ -1150,25 +1168,25 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
             for (int d = 0; d < DT; d++)
                 if (16 * d + ch < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d];
         } else {
-            if (kq == 0 && half == 0 && a.lse) a.lse[orow] = lsum == 0.0f ? -INFINITY : (M - TS_UP + __builtin_amdgcn_logf(lsum)) * TA_LN2;
-            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+            if (kq == 0 && half == 0 && a.lse) a.lse[orow] = lsum == 0.0f ? -INFINITY : (Rf + __builtin_amdgcn_logf(lsum)) * TA_LN2;
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum, down = exp2_int(M - Rf, -TS_UP);
             if (a.o_dt == K3HIP_F32) {
                 float *dst = reinterpret_cast<float *>(a.o) + orow * KL + ch;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + ch < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d] * inv;
+                    if (16 * d + ch < KL) *reinterpret_cast<f32x4 *>(dst + 16 * d) = acc[d] * inv * down;
             } else {
                 uint16_t *dst = reinterpret_cast<uint16_t *>(a.o) + orow * KL + ch;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
-                    if (16 * d + ch < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d] * inv);
+                    if (16 * d + ch < KL) *reinterpret_cast<uint2 *>(dst + 16 * d) = pack4(acc[d] * inv * down);
             }
         }
     }
 }
 
 // The parts of a row merged, by W waves: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s, wave w the parts
-// w, w + W, ..., the waves' sums in order. Eight waves a row up to 512 rows, where long sequences have many parts each
+// w, w + W, ..., the waves' sums in order. Of fp32 caches l_s is taken against R_s, not M_s, and o takes 2^(M - TS_UP - R). Eight waves a row up to 512 rows, where long sequences have many parts each
 // (with the first launch, 64 rows of 125 parts: 28 us, 31 with four waves; of 256 parts: 34, 40), one beyond (1024 rows
 // of 17 parts: 38, 40 with eight; 16,384 rows of 3: 40 us for the merge with four waves, 21 with one). The sums are
 // asked for four parts at a time, the next four before these are added, and
@@ -1176,10 +1194,10 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 // made a merge of 16 parts 27 us. A part that saw nothing (M_s = -inf) left no sums: its memory is read, its
 // weight not used. One that saw a NaN (M_s = inf) makes the row NaN.
 constexpr int TM_PER = 4;
-template <int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows, float up)
+template <int W, bool F32>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(const AttnArgs a, int tile_rows)
 {
-    __shared__ float s_m[W], s_l[W];
+    __shared__ float s_m[W], s_r[W], s_l[W];
     __shared__ f32x4 s_v[W == 1 ? 1 : W][TA_KL / 4];
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = W == 1 ? 0 : tid >> 6;
     const int row = W == 1 ? blockIdx.x * 4 + (tid >> 6) : blockIdx.x;
@@ -1203,7 +1221,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(
             }
         }
     };
-    float M = -INFINITY, l = 0.0f;
+    float M = -INFINITY, R = -INFINITY, l = 0.0f;
     f32x4 v[2] = {f32x4(0.0f), f32x4(0.0f)};
     if (mine > 0) ask(0);
     for (int i0 = 0; i0 < mine; i0 += 64) {
@@ -1215,10 +1233,21 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(
         for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
         const float mn = fmaxf(M, mx), old = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
         const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        float ls = w == 0.0f ? 0.0f : w * pl;
+        float wl = w, oldl = old;
+        if constexpr (F32) {
+            const float r = has ? a.pr[pa] : -INFINITY;
+            float rx = r;
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) rx = fmaxf(rx, __shfl_xor(rx, o, 64));
+            const float rn = fmaxf(R, rx);
+            oldl = R == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(R - rn);
+            wl = r == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(r - rn);
+            R = rn;
+        }
+        float ls = wl == 0.0f ? 0.0f : wl * pl;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o, 64);
-        l = l * old + ls;
+        l = l * oldl + ls;
         v[0] *= old;
         v[1] *= old;
         M = mn;
@@ -1239,40 +1268,44 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void tree_attn_merge_kernel(
             }
         }
     }
-    float Mx = M;
+    float Mx = M, Rx = F32 ? R : M;
     if constexpr (W > 1) {
         if (lane == 0) {
             s_m[wv] = M;
+            s_r[wv] = Rx;
             s_l[wv] = l;
         }
         s_v[wv][lane] = v[0];
         s_v[wv][64 + lane] = v[1];
         __syncthreads();
         if (wv > 1) return;   // wave c takes channels 256 c .. + 255
-        Mx = -INFINITY;
+        Mx = Rx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < W; k++) Mx = fmaxf(Mx, s_m[k]);
+        for (int k = 0; k < W; k++) {
+            Mx = fmaxf(Mx, s_m[k]);
+            Rx = fmaxf(Rx, s_r[k]);
+        }
         l = 0.0f;
         v[0] = v[1] = f32x4(0.0f);
 #pragma unroll
         for (int k = 0; k < W; k++) {
             if (s_m[k] == -INFINITY) continue;
             const float w = __builtin_amdgcn_exp2f(s_m[k] - Mx);
-            l += w * s_l[k];
+            l += (F32 ? __builtin_amdgcn_exp2f(s_r[k] - Rx) : w) * s_l[k];
             v[0] += w * s_v[k][64 * wv + lane];
         }
         v[1] = v[0];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l, down = F32 ? exp2_int(Mx - Rx, -TS_UP) : 1.0f;
     const size_t orow = (size_t)b * a.t.N * a.H + row;
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         const int ch = 256 * c + 4 * lane;
         if (ch >= a.KL || (W > 1 && c != wv)) continue;
-        if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * a.KL + ch) = v[c] * inv;
-        else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * a.KL + ch) = pack4(v[c] * inv);
+        if (a.o_dt == K3HIP_F32) *reinterpret_cast<f32x4 *>(reinterpret_cast<float *>(a.o) + orow * a.KL + ch) = v[c] * inv * down;
+        else *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + orow * a.KL + ch) = pack4(v[c] * inv * down);
     }
-    if (a.lse && lane == 0 && wv == 0) a.lse[orow] = l == 0.0f ? -INFINITY : (Mx - up + __builtin_amdgcn_logf(l)) * TA_LN2;
+    if (a.lse && lane == 0 && wv == 0) a.lse[orow] = l == 0.0f ? -INFINITY : (Rx + __builtin_amdgcn_logf(l)) * TA_LN2;
 }
 
 // Query rows a workgroup takes: 128 on bf16 where a sequence has more (64 and 128 measured: 64 sequences of 128 rows
@@ -1305,7 +1338,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 size_t ta_ws_bytes(long parts, int rows, int KL, int B)
 {
     const size_t r = (size_t)parts * rows;
-    return up256(r * KL * 4) + 2 * up256(r * 4) + up256((size_t)B * sizeof(int4));
+    return up256(r * KL * 4) + 3 * up256(r * 4) + up256((size_t)B * sizeof(int4));
 }
 
 }  // namespace
@@ -1376,7 +1409,8 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     a.po = (float *)workspace;
     a.pm = (float *)((char *)workspace + up256(r * kv_lora * 4));
     a.pl = (float *)((char *)a.pm + up256(r * 4));
-    a.plan = (int4 *)((char *)a.pl + up256(r * 4));
+    a.pr = (float *)((char *)a.pl + up256(r * 4));
+    a.plan = (int4 *)((char *)a.pr + up256(r * 4));
     // bf16: eight rows of full width in one page go by buffer loads from one address (otherwise an address a lane, by
     // global loads: 830 us for 798 at 4 sequences of 64 nodes over 32,768 positions, 4% more at 64 tokens over 8192)
     const void *kern;
@@ -1389,11 +1423,12 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     void *args[] = {&a};
     K3_HIP(hipLaunchKernel(kern, dim3((unsigned)grid), dim3(f32 ? TS_NT : TA_NT), args, lds, st));
     K3_LAUNCHED();
-    const float up = f32 ? TS_UP : 0.0f;
-    if ((long)B * N * H <= 512)
-        hipLaunchKernelGGL((tree_attn_merge_kernel<8>), dim3((unsigned)(N * H), (unsigned)B), dim3(512), 0, st, a, rows, up);
-    else
-        hipLaunchKernelGGL((tree_attn_merge_kernel<1>), dim3((unsigned)((N * H + 3) / 4), (unsigned)B), dim3(256), 0, st, a, rows, up);
+    const bool few = (long)B * N * H <= 512;
+    const dim3 mg(few ? (unsigned)(N * H) : (unsigned)((N * H + 3) / 4), (unsigned)B);
+    if (few && f32) hipLaunchKernelGGL((tree_attn_merge_kernel<8, true>), mg, dim3(512), 0, st, a, rows);
+    else if (few) hipLaunchKernelGGL((tree_attn_merge_kernel<8, false>), mg, dim3(512), 0, st, a, rows);
+    else if (f32) hipLaunchKernelGGL((tree_attn_merge_kernel<1, true>), mg, dim3(256), 0, st, a, rows);
+    else hipLaunchKernelGGL((tree_attn_merge_kernel<1, false>), mg, dim3(256), 0, st, a, rows);
     K3_LAUNCHED();
     return K3HIP_OK;
 }

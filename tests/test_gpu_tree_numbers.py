@@ -1,14 +1,15 @@
 # SPDX-License-Identifier: Apache-2.0
 """Attention over trees of drafted tokens where its numbers leave the ordinary: queries, nodes and whole
 pages that are not finite, in every place a sequence can be cut into parts. Plain form and tolerances:
-test_gpu_tree.py; what such a value does not reach is compared bit for bit with the call without it."""
+test_gpu_tree.py; what such a value does not reach is compared bit for bit with the call without it. And
+finite rows of sizes near the ends of fp32, or far apart."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
-from test_gpu_tree import SEED, rounded, run_attention
-from tree_form import Cache, path_of, random_tree
+from test_gpu_tree import SEED, U, rounded, run_attention, within
+from tree_form import Cache, attention, path_of, random_tree
 
 pytestmark = pytest.mark.gpu
 KL, R = 512, 64
@@ -93,3 +94,48 @@ def test_committed_pages_of_nan(gpu, first, last, H, bf16):
     hit = np.zeros((B, N, H), bool)
     hit[0] = True
     only_these(attend(gpu, q, with_pages(cache, pages), lens, parents, bf16), clean, hit, "pages")
+
+
+# ------------------------------------------------------ rows of any size (fp32) ----
+def sized(gpu, rng, sizes, q_size, lens, N, H, scale, zeros=()):
+    """Sequences whose positions' rows are of size 2^sizes[b](t) (None: zero), queries of 2^q_size[b]. The check
+    is test_gpu_tree's bound without its floor, everything of a sequence times a power of two that makes its
+    largest row's size 1."""
+    B = len(sizes)
+    cache = Cache(rng, B, max(lens) + N, 16, KL + R)
+    q = rng.standard_normal((B, N, H, KL + R)).astype(np.float32)
+    top = np.full(B, -200)
+    for b in range(B):
+        q[b] *= np.float32(2.0 ** q_size[b])
+        for t in range(lens[b] + N):
+            k = sizes[b](t)
+            cache.pages[cache.at(b, t)] *= np.float32(0 if k is None else 2.0 ** k)
+            top[b] = max(top[b], -200 if k is None else k)
+    lens, parents = np.asarray(lens, np.int32), random_tree(rng, B, N)
+    got, got_lse = run_attention(gpu, q, cache, lens, None, parents, scale, KL, False, False)
+    o, lse, mag, dot = attention(q, cache, lens, np.full(B, N), parents, scale, KL)
+    T = int(lens.max()) + N
+    e = 2 * (KL + R + 4) * U * dot + (T + 16) * U
+    unit = (2.0 ** -top.astype(np.float64))[:, None, None, None]
+    within(got.astype(np.float64) * unit, o * unit, e[..., None] * mag * unit, "o")
+    within(got_lse, lse, e + 8 * U * np.abs(lse), "lse")
+
+
+@pytest.mark.parametrize("k", [-105, -90, -120, 110])
+@pytest.mark.parametrize("ctx", [20, 500])
+def test_rows_of_one_far_size(gpu, ctx, k):
+    """All rows of one size near the ends of fp32, the queries of ordinary size or (scores over rows of 2^110) of 2^-110."""
+    rng = np.random.default_rng(SEED + 231 + ctx - k)
+    sized(gpu, rng, [lambda t: k, lambda t: k], [min(0, -k)] * 2, [ctx, ctx // 3], 3, 8, 0.05)
+
+
+@pytest.mark.parametrize("big,small", [(75, -60), (100, -100), (120, 0)])
+@pytest.mark.parametrize("ctx", [20, 700])
+def test_rows_of_far_sizes_together(gpu, ctx, big, small):
+    """Rows of size 2^big among rows of size 2^small, in turn, one half behind the other and zeros among them: scores are
+    alike, so that every row counts in the sum of the weights, within a part and between parts."""
+    rng = np.random.default_rng(SEED + 241 + ctx + big)
+    half = ctx // 2
+    sizes = [lambda t: big if t % 2 else small, lambda t: big if t < half else small, lambda t: small if t < half else big,
+             lambda t: (big, small, None)[t % 3]]
+    sized(gpu, rng, sizes, [-big] * 4, [ctx] * 4, 3, 8, 0.05)
