@@ -406,8 +406,8 @@ int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pages, int dt
  * bf16 caches: the products on bf16, weights rounded to bf16, sums in fp32; o is divided by the sum of the
  * rounded weights and lse is its log, so that parts of a context merge by (o, lse). fp32 caches: values of
  * cache and queries as two fp16 parts of their row scaled by its largest value, 22 bits down to 2^-29 of
- * that value (and to 2^-124), sums in fp32. Rows of any finite size, and of sizes far apart, are summed alike;
- * queries may be as large as 2^100.
+ * that value (and to 2^-124), weights to 2^-22 of themselves or to 2^-30 of the largest p_t max|c_t| over max|c_t|,
+ * sums in fp32. Rows of any finite size, and of sizes far apart, are summed alike; queries may be as large as 2^100.
  * kv_lora at most 512, kv_lora + rope at most 576, both multiples of 8; q, pages, o 16-byte aligned.
  * workspace: k3hip_mla_tree_workspace bytes (of any call with these B, N, H, kv_lora), 16-byte aligned,
  * used by one call at a time; NULL: taken from the library's scratch for the call. */

@@ -805,10 +805,12 @@ __device__ __forceinline__ void split4(const f4 &x, float scale, uint2 &hi, uint
 // 2^(x + add), x a whole number (of a row that has seen nothing, or an infinity: any).
 __device__ __forceinline__ float exp2_int(float x, int add) { return __builtin_amdgcn_ldexpf(1.0f, (int)x + add); }
 
-// The power of two that a row whose largest magnitude has these bits is scaled by.
+// The power of two that a row whose largest magnitude has these bits is scaled by. Zeros by the largest: they add
+// nothing to the second product, and by a smaller one they would make the others' weights small in it (by 1, those of
+// rows of 1e-4 some 2^-19, fp16 subnormals).
 __device__ __forceinline__ int row_scale(uint32_t most)
 {
-    return most == 0 ? 0 : min(14 - ((int)(most >> 23) - 127), TS_KMAX);
+    return min(14 - ((int)(most >> 23) - 127), TS_KMAX);
 }
 
 // Behind it every wave's LDS accesses before it; loads to registers stay on their way.

@@ -139,3 +139,12 @@ def test_rows_of_far_sizes_together(gpu, ctx, big, small):
     sizes = [lambda t: big if t % 2 else small, lambda t: big if t < half else small, lambda t: small if t < half else big,
              lambda t: (big, small, None)[t % 3]]
     sized(gpu, rng, sizes, [-big] * 4, [ctx] * 4, 3, 8, 0.05)
+
+
+@pytest.mark.parametrize("k", [0, -7, -10, -14, -40])
+@pytest.mark.parametrize("ctx", [25, 100])
+def test_zero_rows_among_small_ones(gpu, ctx, k):
+    """Rows of one small size and one, some or nothing but zero rows: what the others add to o keeps its accuracy."""
+    rng = np.random.default_rng(SEED + 251 + ctx - k)
+    sizes = [lambda t: None if t == 3 else k, lambda t: None if t % 4 == 1 else k, lambda t: None if t > 1 else k, lambda t: None]
+    sized(gpu, rng, sizes, [0] * 4, [ctx] * 4, 3, 5, 0.05)
