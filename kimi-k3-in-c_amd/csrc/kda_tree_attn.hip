@@ -207,7 +207,7 @@ __device__ __forceinline__ bool find_slot(const AttnArgs &a, int rows, int tp, i
     n = __builtin_amdgcn_readfirstlane(n);
     if (n == 0) return false;
     s.n = n;
-    T = __builtin_amdgcn_readfirstlane(T);   // the host checks that it fits an int
+    T = __builtin_amdgcn_readfirstlane(T);   // the host checks that two of them fit an int
     int count = min(max(1, most / n), T), L = 0;   // slots; their most steps, 0: equal slots
     if (a.B > 1 && a.B <= 64 && count < 0x8000) {
         const int avg = (T + count - 1) / count;
@@ -1377,7 +1377,7 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
         K3_FAIL(K3HIP_EUNSUPPORTED, "%s: kv_lora=%d rope=%d (multiples of 8, at most %d and %d together)", who, kv_lora,
                 rope, TA_KL, TA_CW);
     if (!(scale > 0.0f)) K3_FAIL(K3HIP_EINVAL, "%s: scale=%g (positive)", who, scale);
-    if (B * (((long)max_pages * page + N) / 32 + 1) > 0x7fffffffL)
+    if (B * (((long)max_pages * page + N) / TB_TP + 1) > 0x3fffff00L)   // steps: sums of two counts fit an int
         K3_FAIL(K3HIP_EINVAL, "%s: %d sequences of up to %ld positions", who, B, (long)max_pages * page);
     if ((long)page * CW * 4 > 0x7fffffffL) K3_FAIL(K3HIP_EINVAL, "%s: pages of %d rows", who, page);
     if (B > 65535 || (long)N * H > 65535L * 16) K3_FAIL(K3HIP_EINVAL, "%s: B=%d N=%d H=%d", who, B, N, H);
