@@ -409,8 +409,8 @@ int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pages, int dt
  * that value (and to 2^-124), weights to 2^-22 of themselves or to 2^-30 of the largest p_t max|c_t| over max|c_t|,
  * sums in fp32. Rows of any finite size, and of sizes far apart, are summed alike; queries may be as large as 2^100.
  * kv_lora at most 512, kv_lora + rope at most 576, both multiples of 8; q, pages, o 16-byte aligned.
- * workspace: k3hip_mla_tree_workspace bytes (of any call with these B, N, H, kv_lora), 16-byte aligned,
- * used by one call at a time; NULL: taken from the library's scratch for the call. */
+ * workspace: k3hip_mla_tree_workspace bytes (of any call with these B, N, H, kv_lora; 0: none is taken, or the call
+ * is refused), 16-byte aligned, used by one call at a time; NULL: taken from the library's scratch for the call. */
 size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora);
 int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int rope, float scale, const void *q,
                              const void *pages, int dtype, int n_pages, int page, const int *table, int max_pages,

@@ -1336,6 +1336,9 @@ long ta_grid(int n)
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// Sequences and query rows that the launches hold.
+bool ta_fits(int B, int N, int H) { return B <= 65535 && (long)N * H <= 65535L * 16; }
+
 // `parts` partial sums of `rows` rows, and the plan of B sequences.
 size_t ta_ws_bytes(long parts, int rows, int KL, int B)
 {
@@ -1351,7 +1354,7 @@ using namespace k3kda;
 
 extern "C" size_t k3hip_mla_tree_workspace(int B, int N, int H, int kv_lora)
 {
-    if (B <= 0 || N <= 0 || N > TREE_MAX || H <= 0 || kv_lora <= 0 || kv_lora > TA_KL) return 0;
+    if (B <= 0 || N <= 0 || N > TREE_MAX || H <= 0 || kv_lora <= 0 || kv_lora > TA_KL || !ta_fits(B, N, H)) return 0;
     size_t most = 0;
     for (bool f32 : {false, true}) {
         const int rows = ta_rows(f32, (long)N * H);
@@ -1380,7 +1383,7 @@ extern "C" int k3hip_mla_tree_attention(int B, int N, int H, int kv_lora, int ro
     if (B * (((long)max_pages * page + N) / TB_TP + 1) > 0x3fffff00L)   // steps: sums of two counts fit an int
         K3_FAIL(K3HIP_EINVAL, "%s: %d sequences of up to %ld positions", who, B, (long)max_pages * page);
     if ((long)page * CW * 4 > 0x7fffffffL) K3_FAIL(K3HIP_EINVAL, "%s: pages of %d rows", who, page);
-    if (B > 65535 || (long)N * H > 65535L * 16) K3_FAIL(K3HIP_EINVAL, "%s: B=%d N=%d H=%d", who, B, N, H);
+    if (!ta_fits(B, N, H)) K3_FAIL(K3HIP_EINVAL, "%s: B=%d N=%d H=%d", who, B, N, H);
     if (B == 0 || N == 0) return K3HIP_OK;
     if (!q || !o) K3_FAIL(K3HIP_EINVAL, "%s: NULL q or o", who);
     if (((uintptr_t)q | (uintptr_t)pages | (uintptr_t)o) & 15)
