@@ -281,6 +281,18 @@ __global__ __launch_bounds__(CM_NT) void latent_commit_kernel(TreeSeqs t, PagedR
     }
 }
 
+// rows x H pieces of `width` elements, rows `ld` apart and heads `head` apart (each at least width): no two meet.
+// Row i and head j meet where j heads and i rows are less than a width apart.
+bool apart(long rows, long H, long ld, long head, long width)
+{
+    if (rows <= 1 || H <= 1 || (H - 1) * head + width <= ld || (rows - 1) * ld + width <= head) return true;
+    for (long j = 1; j < H; j++) {
+        const long i = j * head / ld, over = j * head - i * ld;
+        if ((i >= 1 && i < rows && over < width) || (i + 1 < rows && ld - over < width)) return false;
+    }
+    return true;
+}
+
 bool act_dtype(int dt) { return dt == K3HIP_F32 || dt == K3HIP_BF16; }
 
 }  // namespace
@@ -313,6 +325,8 @@ extern "C" int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pa
     if (q && (long)B * N > 1 && q_out_ld < rope)
         K3_FAIL(K3HIP_EINVAL, "%s: rows of rotated queries %ld elements apart", who, q_out_ld);
     if (B == 0 || N == 0) return K3HIP_OK;
+    if (q && !apart((long)B * N, H, q_out_ld, q_out_head, rope))
+        K3_FAIL(K3HIP_EINVAL, "%s: rotated queries overlap: rows %ld, heads %ld elements apart", who, q_out_ld, q_out_head);
     if (!rows || rows_ld < kv_lora + rope) K3_FAIL(K3HIP_EINVAL, "%s: rows NULL or stride %ld", who, rows_ld);
     AppendArgs a{};
     a.t = TreeSeqs{N, lens, counts, parents};

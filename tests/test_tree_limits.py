@@ -3,10 +3,12 @@
 any device call, so no GPU is needed and the pointers are never read."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 
 import k3kda
-from test_tree_refusals import ATTENTION, call
+from test_tree_refusals import APPEND, ATTENTION, call
 
 
 def refused(name, defaults, subject, **changed):
@@ -23,3 +25,28 @@ def test_attention_over_more_steps_than_two_of_which_fit_an_int():
 def test_workspace_of_calls_that_are_too_large(bad):
     """What the call refuses has no workspace (not the size of a count that passed an int)."""
     assert k3kda.lib().k3hip_mla_tree_workspace(*bad) == 0
+
+
+A2 = C.c_void_p(1 << 24)
+
+
+@pytest.mark.parametrize("B,N,H,ld,head", [
+    (1, 4, 2, 64, 64),       # row n + 1's first head on row n's second
+    (1, 4, 3, 100, 150),     # row 3 (300) on head 2 (300)
+    (2, 3, 5, 128, 200),     # row 3 (384) ends inside head 2 (400)
+    (1, 9, 2, 64, 500),      # head 1 inside the rows' range
+])
+def test_rotated_queries_whose_heads_overlap_rows(B, N, H, ld, head):
+    refused("k3hip_latent_append", APPEND, "overlap", B=B, N=N, H=H, q_out=A2, q_out_ld=ld, q_out_head=head)
+
+
+@pytest.mark.parametrize("B,N,H,ld,head", [
+    (2, 9, 3, 192, 64), (2, 9, 3, 64, 18 * 64), (1, 4, 2, 1 << 20, 64), (1, 1, 5, 64, 64), (1, 9, 1, 64, 64),
+    (1, 3, 3, 160, 224),     # rows at 0, 160, 320, heads at 0, 224, 448: between each other
+])
+def test_rotated_queries_that_do_not_overlap(B, N, H, ld, head):
+    """Every layout in which no two heads of rows meet stands (no queries to rotate here: the check is all there is)."""
+    starts = sorted(r * ld + h * head for r in range(B * N) for h in range(H))
+    assert all(b - a >= 64 for a, b in zip(starts, starts[1:]))
+    rc, msg = call("k3hip_latent_append", APPEND, B=B, N=N, H=H, q_out=A2, q_out_ld=ld, q_out_head=head, rows=None)
+    assert rc == k3kda.EINVAL and "overlap" not in msg and "rows NULL" in msg
