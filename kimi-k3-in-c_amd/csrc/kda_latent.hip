@@ -327,6 +327,9 @@ extern "C" int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pa
     if (B == 0 || N == 0) return K3HIP_OK;
     if (q && !apart((long)B * N, H, q_out_ld, q_out_head, rope))
         K3_FAIL(K3HIP_EINVAL, "%s: rotated queries overlap: rows %ld, heads %ld elements apart", who, q_out_ld, q_out_head);
+    if (q && q == q_out && (q_dtype != q_out_dtype || ((long)B * N > 1 && q_ld != q_out_ld) || (H > 1 && q_head != q_out_head)))
+        K3_FAIL(K3HIP_EINVAL, "%s: queries rotated in place: dtypes %d -> %d, strides %ld, %ld -> %ld, %ld", who, q_dtype, q_out_dtype,
+                q_ld, q_head, q_out_ld, q_out_head);
     if (!rows || rows_ld < kv_lora + rope) K3_FAIL(K3HIP_EINVAL, "%s: rows NULL or stride %ld", who, rows_ld);
     AppendArgs a{};
     a.t = TreeSeqs{N, lens, counts, parents};

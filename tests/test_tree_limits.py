@@ -50,3 +50,10 @@ def test_rotated_queries_that_do_not_overlap(B, N, H, ld, head):
     assert all(b - a >= 64 for a, b in zip(starts, starts[1:]))
     rc, msg = call("k3hip_latent_append", APPEND, B=B, N=N, H=H, q_out=A2, q_out_ld=ld, q_out_head=head, rows=None)
     assert rc == k3kda.EINVAL and "overlap" not in msg and "rows NULL" in msg
+
+
+@pytest.mark.parametrize("changed", [dict(q_out_dtype=1), dict(q_out_ld=256), dict(q_out_head=72, q_out_ld=144)])
+def test_queries_rotated_in_place_in_another_layout(changed):
+    """A workgroup would write over what another has not read yet."""
+    same = dict(q_out=A, q_out_dtype=0, q_out_ld=128, q_out_head=64)
+    refused("k3hip_latent_append", APPEND, "in place", **{**same, **changed})
