@@ -319,7 +319,7 @@ extern "C" int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pa
     if (parents && N > TREE_MAX) K3_FAIL(K3HIP_EUNSUPPORTED, "%s: a tree of %d nodes (at most %d)", who, N, TREE_MAX);
     if (B > 65535) K3_FAIL(K3HIP_EINVAL, "%s: B=%d", who, B);
     if (q && (H <= 0 || !q_out || !act_dtype(q_dtype) || !act_dtype(q_out_dtype) || q_ld < 0 || q_out_ld < 0 ||
-              q_head < rope || q_out_head < rope || rope == 0))
+              q_head < rope || q_out_head < rope || rope == 0 || (long)H * rope > 0x7fffff00L))
         K3_FAIL(K3HIP_EINVAL, "%s: queries H=%d dtypes %d -> %d, head strides %ld -> %ld, rope=%d", who, H, q_dtype,
                 q_out_dtype, q_head, q_out_head, rope);
     if (q && (long)B * N > 1 && q_out_ld < rope)

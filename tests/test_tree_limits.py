@@ -57,3 +57,7 @@ def test_queries_rotated_in_place_in_another_layout(changed):
     """A workgroup would write over what another has not read yet."""
     same = dict(q_out=A, q_out_dtype=0, q_out_ld=128, q_out_head=64)
     refused("k3hip_latent_append", APPEND, "in place", **{**same, **changed})
+
+
+def test_rotated_queries_of_more_elements_a_row_than_an_int():
+    refused("k3hip_latent_append", APPEND, "H=", H=(1 << 25), q_out=A2, q_out_ld=1 << 40, q_out_head=64)
