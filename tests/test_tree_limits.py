@@ -8,7 +8,7 @@ import ctypes as C
 import pytest
 
 import k3kda
-from test_tree_refusals import APPEND, ATTENTION, call
+from test_tree_refusals import APPEND, ATTENTION, A, call
 
 
 def refused(name, defaults, subject, **changed):
