@@ -389,7 +389,8 @@ enum { K3HIP_ROPE_PAIRS = 0, K3HIP_ROPE_HALVES = 1 };
  * src/core/k3_ops.c:94-102), its rope slot rotated: pair i by position * inv_freq[i], pairs (2i, 2i+1)
  * or (i, i + rope/2) by rope_style; inv_freq NULL: copied (NoPE). With q, the rope slots of the
  * queries, q [B][N][H][rope] (row stride q_ld, head stride q_head), are rotated the same way into q_out
- * (its own strides; it may be q itself with q's strides and dtype). rope even, at most 256.
+ * (its own strides, by which no two heads may meet; it may be q itself, with q's strides and dtype only). rope even,
+ * at most 256.
  * Dtypes K3HIP_F32 or K3HIP_BF16 each. */
 int k3hip_latent_append(int B, int N, int kv_lora, int rope, void *pages, int dtype, int n_pages, int page,
                         const int *table, int max_pages, const int *lens, const int *counts, const int *parents,

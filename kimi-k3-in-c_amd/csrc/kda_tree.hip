@@ -111,7 +111,9 @@ struct alignas(16) TreeLds {
 // workgroup for 42 us at 64 sequences x 16 nodes: 200 us a launch.) TILES: 16-row node tiles.
 // Measured at 32 heads x 128: 64 sequences x 16 nodes 62 us (3.2 TB/s; three workgroups a CU in 80 registers, 2.7 rounds
 // of 18 us: loads 5, conv 5, walk 2, products 3, solve 3), one sequence x 8 nodes 10 us, a chain of memory waits
-// and barriers.
+// and barriers. Larger trees leave less beside each other: up to 32 nodes 127 registers and 78 KB, two workgroups a CU
+// (16 sequences x 32 nodes 38 us, 32 x 32 69); up to 64 nodes 221 and 151 KB, one, whose chain nothing covers (16 x 64
+// 119 us, one x 64 55).
 template <int D, int TILES>
 __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tree_kernel(const TreeArgs a)
 {
@@ -435,7 +437,7 @@ __global__ __launch_bounds__(4 * D, D == 128 && TILES == 1 ? 6 : 1) void kda_tre
 // the path's length. K1 of up to TREE_CK nodes at a time runs before them, from their inputs and the three before
 // them in LDS. The conv history of the head's channels becomes the last K - 1 inputs of history and path.
 // Measured at 32 heads x 128: 64 sequences x 16 nodes 59 us (4.4 TB/s, reading and writing the state; a plain copy
-// reaches 4.9), one sequence 9.3 us. Loading taps, inputs and history where they were used: 88 us.
+// reaches 4.9, kda_decode_kernel 5.8 on the same states in place, with a store that no cache keeps), one sequence 9.3 us. Loading taps, inputs and history where they were used: 88 us.
 constexpr int TREE_CK = 16;
 
 template <int D>

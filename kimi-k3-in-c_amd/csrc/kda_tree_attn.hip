@@ -170,7 +170,12 @@ __device__ __forceinline__ uint2 pack4(const f32x4 &v)
 // pipeline anew, and leaves two parts. Otherwise the axis is cut into equal slots. (Equal slots, and this, bf16: 16
 // sequences of one token over up to 1024 positions 37.5 and 31.5 us, of 8 tokens 66 and 52, 64 of one over up to
 // 8192 118 and 113; fp32: 4 of 8 tokens over up to 2000 70 and 58. With a step of fp32 at 3.7 us, four more than
-// the average cost more than they save: 7 of 13 tokens 144 and 152.)
+// the average cost more than they save: 7 of 13 tokens 144 and 152. Both values of `over` come from these sizes.)
+// Slots that end where sequences end are worked out a sequence a lane, so for up to 64 sequences: one more and
+// the slots are equal (one token each over up to 2048 positions: 64 sequences 43 us, 65 50, 96 61). Two costs stay: there are
+// as many slots as workgroups allow whatever a part costs to write and merge (one sequence of 4000 positions is 125
+// slots of a step, 27 us), and every slot takes as many workgroups as the largest sequence has row tiles, so one tree
+// of 64 nodes among single tokens leaves 31 of 32 workgroups of the others' slots without work.
 constexpr int TB_OVER = 6, TS_OVER = 2;
 struct Slots {
     int n;          // workgroups a slot
@@ -302,7 +307,8 @@ __device__ __forceinline__ float part_max(float M, float l) { return l != l ? IN
 //
 // Measured: 4 sequences x 64 nodes x 64 heads over up to 32,768 positions 798 us, 1.24 PFLOP/s (a large library product
 // reaches 1.36), bound by the matrix cores; 64 tokens over up to 8192 positions 113 us, of which the loop 76 (6 TB/s of
-// cache), first loads 9, 33 MB of parts written and merged most of the rest.
+// cache), first loads 9, 33 MB of parts written and merged most of the rest. The form of 128 rows spills 52 registers, none
+// of them in the loop.
 constexpr int TB_TP = 32, TB_GRP = TB_TP * 128, TB_BUF = 9 * TB_GRP, TB_NB = 4;
 constexpr int TB_LDS = TB_NB * TB_BUF + 64 + TREE_MAX * 8;
 static_assert(TB_LDS <= 160 * 1024, "LDS");
@@ -748,10 +754,12 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // the latent's channels (64 registers). A step has two barriers, behind the halves of the scores and behind the
 // sum; a wave keeps 4 rows on their way to registers and converts and stages them, a column group at a time, between the
 // products: groups 4 .. 8 beside the scores, where groups 0 .. 3 of the buffer carry the halves, those beside the sum.
-// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 144 us with the merge, 195 TFLOP/s of fp32 work, 3.3k
-// of a step's 8.7k cycles matrix instructions and 3.4k LDS accesses; what binds is the wait of two waves in step for
-// LDS fragments (registers allow one K-step of look-ahead), the hand-over (800 cycles) and the softmax (700). With
-// four waves of whole rows, one a SIMD, 238 us: nothing stood beside their waits, and they spilled.
+// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 146 us with the merge, 193 TFLOP/s of fp32 work (144 before
+// the weights' sum had its own reference), 3.3k of a step's 8.7k cycles matrix instructions and 3.4k LDS accesses; what
+// binds is the wait of two waves in step for LDS fragments (registers allow one K-step of look-ahead), the hand-over
+// (800 cycles) and the softmax (about 800). 64 sequences of one token over up to 8192 positions: 265 us, 3.5 TB/s of
+// cache. All 256 registers are taken and 25 spilled (27 where rows are narrower), one of them (three) in the loop. With
+// four waves of whole rows, one a SIMD, 238 us: nothing stood beside their waits, and they spilled in it.
 constexpr int TS_BUF = 2 * TB_BUF;
 constexpr int TS_NT = 512;
 constexpr int TS_LDS = 2 * TS_BUF + 2 * 32 * 8 + 64 + TREE_MAX * 8;
