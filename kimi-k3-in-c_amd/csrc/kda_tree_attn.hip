@@ -754,9 +754,9 @@ __global__ __launch_bounds__(TA_NT) __attribute__((amdgpu_waves_per_eu(1, 1))) v
 // the latent's channels (64 registers). A step has two barriers, behind the halves of the scores and behind the
 // sum; a wave keeps 4 rows on their way to registers and converts and stages them, a column group at a time, between the
 // products: groups 4 .. 8 beside the scores, where groups 0 .. 3 of the buffer carry the halves, those beside the sum.
-// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 146 us with the merge, 193 TFLOP/s of fp32 work (144 before
-// the weights' sum had its own reference), 3.3k of a step's 8.7k cycles matrix instructions and 3.4k LDS accesses; what
-// binds is the wait of two waves in step for LDS fragments (registers allow one K-step of look-ahead), the hand-over
+// Measured (7 sequences of up to 3001 positions x 13 nodes x 64 heads): 146 us with the merge, 193 TFLOP/s of fp32 work
+// (144 before the weights' sum had its own reference), 3.3k of a step's 8.7k cycles matrix instructions and 3.4k LDS
+// accesses; what binds is the wait of two waves in step for LDS fragments (registers allow one K-step of look-ahead), the hand-over
 // (800 cycles) and the softmax (about 800). 64 sequences of one token over up to 8192 positions: 265 us, 3.5 TB/s of
 // cache. All 256 registers are taken and 25 spilled (27 where rows are narrower), one of them (three) in the loop. With
 // four waves of whole rows, one a SIMD, 238 us: nothing stood beside their waits, and they spilled in it.
@@ -1196,8 +1196,8 @@ __global__ __launch_bounds__(TS_NT) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 }
 
 // The parts of a row merged, by W waves: o = sum 2^(M_s - M) o_s / sum 2^(M_s - M) l_s, wave w the parts
-// w, w + W, ..., the waves' sums in order. Of fp32 caches l_s is taken against R_s, not M_s, and o takes 2^(M - TS_UP - R). Eight waves a row up to 512 rows, where long sequences have many parts each
-// (with the first launch, 64 rows of 125 parts: 28 us, 31 with four waves; of 256 parts: 34, 40), one beyond (1024 rows
+// w, w + W, ..., the waves' sums in order. Of fp32 caches l_s is taken against R_s, not M_s, and o takes
+// 2^(M - TS_UP - R). Eight waves a row up to 512 rows, where long sequences have many parts each (with the first launch, 64 rows of 125 parts: 28 us, 31 with four waves; of 256 parts: 34, 40), one beyond (1024 rows
 // of 17 parts: 38, 40 with eight; 16,384 rows of 3: 40 us for the merge with four waves, 21 with one). The sums are
 // asked for four parts at a time, the next four before these are added, and
 // at the start every part's (M_s, l_s), a part a lane, before they are needed: one after the other their latencies
